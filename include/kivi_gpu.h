@@ -497,6 +497,105 @@ const kivi_cache *kivi_guard_cache(const kivi_guard *guard);
 int32_t kivi_guard_policy(const kivi_guard *guard);
 uint64_t kivi_guard_sequence_length(const kivi_guard *guard);
 
+/* ------------------------------------------------------------ paged store
+ *
+ * A key/value store in pages shared by many sequences, and the attention of
+ * their newest tokens over it (no counterpart in the reference, whose caches
+ * hold one contiguous batch each and attend with one query per sequence).
+ *
+ * Page p, kv head h holds page_size rows of head_dim elements, keys and values
+ * apart: data [num_pages][num_kv_heads][page_size][row], params
+ * [num_pages][num_kv_heads][page_size][2] floats (scale, zero).  bits 16: a row
+ * is head_dim elements of `dtype` (KIVI_DTYPE_F16 or KIVI_DTYPE_BF16) and there
+ * are no params.  bits 8 or 4: a row is head_dim codes, first channel in the low
+ * bits, quantized as kivi_quantize_per_token does with group_size = head_dim
+ * (quant.rs:193-233): scale = (max - min) / (2^bits - 1), zero = min, each code
+ * standing for fma(code, scale, zero).
+ *
+ * The memory is the caller's (a serving engine reserves its pool itself); the
+ * handle keeps pointers to it and the scratch of the attention.  Every call is
+ * stream-ordered.  Calls on one handle may use several streams: an attention
+ * call waits on the device for the handle's previous one, whose scratch it
+ * shares (inside a stream capture it does not: order captured calls on one
+ * handle yourself).  Writing and attending are ordered by the caller's streams.
+ */
+#define KIVI_DTYPE_F32 0
+#define KIVI_DTYPE_F16 1
+#define KIVI_DTYPE_BF16 2
+
+typedef struct kivi_pages_config {
+    uint32_t bits;         /* 16, 8 or 4 */
+    int32_t dtype;         /* element type of 16-bit rows; ignored for codes */
+    uint64_t num_pages;
+    uint64_t page_size;    /* tokens per page: 16, 32, 64, 128 or 256 */
+    uint64_t num_kv_heads;
+    uint64_t head_dim;     /* 32, 64, 96 or 128 */
+} kivi_pages_config;
+
+/* One step's sequences; the three arrays are device memory, read when the
+ * calls run.  Sequence b's token t lies in page
+ * block_table[b * table_stride + t / page_size] at row t % page_size; entries of
+ * pages that a call does not touch may hold anything.  kv_lens[b] counts its
+ * tokens including the newest cu_tokens[b + 1] - cu_tokens[b], whose rows in the
+ * dense arrays are cu_tokens[b] .. cu_tokens[b + 1] - 1. */
+typedef struct kivi_pages_batch {
+    const int32_t *block_table;
+    uint64_t table_stride;  /* entries from one row to the next */
+    uint64_t table_width;   /* entries of a row */
+    const int32_t *cu_tokens; /* [batch + 1], ascending from 0 to total_tokens */
+    const int32_t *kv_lens;   /* [batch] */
+    uint64_t batch;
+    uint64_t total_tokens;  /* rows of the dense arrays */
+    uint64_t max_tokens;    /* at least every sequence's newest tokens */
+} kivi_pages_batch;
+
+typedef struct kivi_pages kivi_pages;
+
+/* Bytes of one side's data and floats of one side's params. */
+int32_t kivi_pages_sizes(const kivi_pages_config *config, uint64_t *data_bytes,
+                         uint64_t *param_floats, kivi_error *err);
+/* A handle over the caller's memory: d_keys / d_values of data_bytes each
+ * (16-byte aligned), d_key_params / d_value_params of param_floats each (8-byte
+ * aligned; null when bits is 16).  The memory must outlive the handle. */
+int32_t kivi_pages_new(const kivi_pages_config *config, void *d_keys, void *d_values,
+                       float *d_key_params, float *d_value_params, int32_t device,
+                       kivi_pages **out, kivi_error *err);
+void kivi_pages_free(kivi_pages *pages);
+/* Writes the batch's newest tokens: d_keys / d_values are [total_tokens][heads]
+ * rows of head_dim `dtype` elements (F32, F16 or BF16; rounded or quantized to
+ * the store's), token_stride and head_stride in elements, both sides alike.  A
+ * token whose page lies outside the store is not written. */
+int32_t kivi_pages_write_dev(kivi_pages *pages, const kivi_pages_batch *batch, int32_t dtype,
+                             const void *d_keys, const void *d_values, uint64_t token_stride,
+                             uint64_t head_stride, void *stream, kivi_error *err);
+/* Reads the batch's newest tokens (whole sequences where cu_tokens counts them
+ * whole) back into dense arrays laid out as above. */
+int32_t kivi_pages_read_dev(const kivi_pages *pages, const kivi_pages_batch *batch, int32_t dtype,
+                            void *d_keys, void *d_values, uint64_t token_stride,
+                            uint64_t head_stride, void *stream, kivi_error *err);
+/* Attention of the batch's newest tokens, themselves in the store already.
+ * The query of row cu_tokens[b] + i, head h (kv head h / (num_q_heads /
+ * num_kv_heads)) stands at position p = kv_lens[b] - n + i of its n newest and
+ * sees the tokens t <= p; with window > 0 only those with t > p - window or
+ * t < sinks.  out = sum softmax(scale q.k_t) v_t, fp32 inside, rounded once;
+ * a row that sees nothing (p < 0) gets zeros.  Tokens that a row does not see
+ * never reach it, whatever their memory holds (NaN and infinities included).
+ * dtype (F16 or BF16) is the type of d_query and d_out and, for 16-bit pages,
+ * the store's.  Strides in elements; d_lse, when not null, gets the rows'
+ * natural log-sum-exp [total_tokens][num_q_heads] (-inf where nothing is seen),
+ * with which outputs over disjoint tokens can be joined. */
+int32_t kivi_pages_attention_dev(kivi_pages *pages, const kivi_pages_batch *batch, int32_t dtype,
+                                 const void *d_query, uint64_t num_q_heads,
+                                 uint64_t query_token_stride, uint64_t query_head_stride,
+                                 float scale, uint64_t window, uint64_t sinks, void *d_out,
+                                 uint64_t out_token_stride, uint64_t out_head_stride, float *d_lse,
+                                 void *stream, kivi_error *err);
+/* What the handle's calls found wrong on the device since the last report: page
+ * numbers outside the store, or offsets and lengths outside their arrays, were
+ * clamped (KIVI_ERR_INVALID_ARGUMENT; the outputs concerned are unspecified),
+ * or a bounded wait gave up (KIVI_ERR_CUDA).  Waits for the device. */
+int32_t kivi_pages_status(kivi_pages *pages, kivi_error *err);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,11 +13,13 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
 #include "../../include/kivi_gpu.h"
 #include "kivi_internal.cuh"
+#include "kivi_pages.cuh"
 
 namespace kivi {
 
@@ -2818,4 +2820,271 @@ int32_t kivi_guard_append(kivi_guard *g, const float *keys, uint64_t keys_len, c
     }
     CUDA_TRY(cudaStreamSynchronize(g->stream), "guard append");
     return set_err(err, KIVI_OK);
+}
+
+// ---------------------------------------------------------------- paged store
+
+struct kivi_pages {
+    kivi::PagesStore st{};
+    int device = 0;
+    float *scratch = nullptr;   // the attention's partial states
+    int64_t scratch_floats = 0;
+    cudaEvent_t done = nullptr; // after the last attention call outside a capture
+    cudaStream_t last = nullptr; // its stream
+    bool used = false;
+    std::mutex mu;
+};
+
+namespace {
+
+int32_t check_pages_config(const kivi_pages_config *c, kivi_error *err) {
+    if (!c) return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "null config");
+    if (c->bits != 16 && c->bits != 8 && c->bits != 4) {
+        set_msg(err, KIVI_ERR_INVALID_BITS, "bit width %u is not supported; use 16, 8 or 4", c->bits);
+        if (err) err->a = c->bits;
+        return KIVI_ERR_INVALID_BITS;
+    }
+    if (c->bits == 16 && c->dtype != KIVI_DTYPE_F16 && c->dtype != KIVI_DTYPE_BF16)
+        return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "16-bit pages hold F16 or BF16, not type %d", (int)c->dtype);
+    if (c->num_pages == 0) return set_err(err, KIVI_ERR_ZERO_DIMENSION, 0, 0, "num_pages");
+    if (c->num_kv_heads == 0) return set_err(err, KIVI_ERR_ZERO_DIMENSION, 0, 0, "num_kv_heads");
+    if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
+        return set_msg(err, KIVI_ERR_UNSUPPORTED, "page_size %llu: use 16, 32, 64, 128 or 256",
+                       (unsigned long long)c->page_size);
+    if (c->head_dim == 0 || c->head_dim > 128 || c->head_dim % 32)
+        return set_msg(err, KIVI_ERR_UNSUPPORTED, "head_dim %llu: use 32, 64, 96 or 128",
+                       (unsigned long long)c->head_dim);
+    // a (page, head, token) row number stays below 2^31: tensor copies take 32-bit coordinates
+    if (c->num_pages > 0x7fffffffull || c->num_kv_heads > 65535 ||
+        c->num_pages * c->num_kv_heads > 0x7fffffffull / c->page_size)
+        return set_msg(err, KIVI_ERR_UNSUPPORTED, "more than 2^31 - 1 rows of head_dim elements");
+    return KIVI_OK;
+}
+
+int32_t check_pages_batch(const kivi_pages *h, const kivi_pages_batch *b, kivi::PagesBatch *out, kivi_error *err) {
+    if (!h || !b) return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, h ? "null batch" : "null pages");
+    if (b->batch > 0 && (!b->cu_tokens || !b->kv_lens || (b->table_width > 0 && !b->block_table)))
+        return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "null block table, offsets or lengths");
+    const uint64_t i31 = 0x7fffffffull;
+    if (b->batch > i31 - 1 || b->total_tokens > i31 || b->table_width > i31 / (uint64_t)h->st.page ||
+        b->table_stride > (1ull << 40))
+        return set_msg(err, KIVI_ERR_UNSUPPORTED, "a batch holds fewer than 2^31 sequences, rows and tokens each");
+    if (b->table_stride < b->table_width && b->batch > 1)
+        return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "table_stride %llu is less than table_width %llu",
+                       (unsigned long long)b->table_stride, (unsigned long long)b->table_width);
+    out->table = b->block_table;
+    out->table_stride = (int64_t)b->table_stride;
+    out->width = (int)b->table_width;
+    out->cu = b->cu_tokens;
+    out->kv_lens = b->kv_lens;
+    out->batch = (int)b->batch;
+    out->total = (int)b->total_tokens;
+    out->most = (int)std::min(b->max_tokens, b->total_tokens);
+    return KIVI_OK;
+}
+
+int32_t check_pages_strides(uint64_t token, uint64_t head, kivi_error *err) {
+    if (token > (1ull << 31) || head > (1ull << 31))
+        return set_msg(err, KIVI_ERR_UNSUPPORTED, "strides up to 2^31 elements");
+    return KIVI_OK;
+}
+
+bool rows_aligned(const void *p, uint64_t token, uint64_t head, int bytes) {
+    return ((uintptr_t)p | token * bytes | head * bytes) % 16 == 0;
+}
+
+int32_t pages_dense(int32_t dtype, const void *k, const void *v, uint64_t token, uint64_t head,
+                    const kivi::PagesBatch &b, kivi::PagesDense *x, kivi_error *err) {
+    if (dtype != KIVI_DTYPE_F32 && dtype != KIVI_DTYPE_F16 && dtype != KIVI_DTYPE_BF16)
+        return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "unknown element type %d", (int)dtype);
+    if (b.total > 0 && (!k || !v)) return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "null keys or values");
+    const int bytes = kivi::dtype_bytes(dtype);
+    if (((uintptr_t)k | (uintptr_t)v) % bytes)
+        return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "keys and values must start on an element boundary");
+    int32_t rc = check_pages_strides(token, head, err);
+    if (rc) return rc;
+    x->k = k;
+    x->v = v;
+    x->token = (int64_t)token;
+    x->head = (int64_t)head;
+    x->dtype = dtype;
+    x->vec = rows_aligned(k, token, head, bytes) && rows_aligned(v, token, head, bytes);
+    return KIVI_OK;
+}
+
+// Rows that are written may not overlap (a stride of 0 is a broadcast input).
+int32_t check_pages_target(uint64_t rows, uint64_t heads, uint64_t token, uint64_t head, uint64_t D,
+                           kivi_error *err) {
+    if ((heads > 1 && head < D) || (rows > 1 && token < D))
+        return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "output rows of %llu elements overlap", (unsigned long long)D);
+    return KIVI_OK;
+}
+
+} // namespace
+
+int32_t kivi_pages_sizes(const kivi_pages_config *config, uint64_t *data_bytes, uint64_t *param_floats,
+                         kivi_error *err) {
+    int32_t rc = check_pages_config(config, err);
+    if (rc) return rc;
+    const uint64_t rows = config->num_pages * config->num_kv_heads * config->page_size;
+    if (data_bytes) *data_bytes = rows * config->head_dim * config->bits / 8;
+    if (param_floats) *param_floats = config->bits == 16 ? 0 : 2 * rows;
+    return set_err(err, KIVI_OK);
+}
+
+int32_t kivi_pages_new(const kivi_pages_config *config, void *d_keys, void *d_values, float *d_key_params,
+                       float *d_value_params, int32_t device, kivi_pages **out, kivi_error *err) {
+    if (!out) return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "null output handle");
+    *out = nullptr;
+    int32_t rc = check_pages_config(config, err);
+    if (rc) return rc;
+    if (!d_keys || !d_values || (config->bits != 16 && (!d_key_params || !d_value_params)))
+        return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "null page memory");
+    if (((uintptr_t)d_keys | (uintptr_t)d_values) % 16 ||
+        (config->bits != 16 && ((uintptr_t)d_key_params | (uintptr_t)d_value_params) % 8))
+        return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "page data must be 16-byte aligned, params 8-byte aligned");
+    DeviceGuard dg(device);
+    if (!dg.ok) return set_msg(err, KIVI_ERR_CUDA, "cannot select device %d", device);
+    kivi_pages *h = new (std::nothrow) kivi_pages();
+    if (!h) return set_msg(err, KIVI_ERR_OUT_OF_MEMORY, "kivi_pages_new: host allocation failed");
+    kivi::PagesStore &st = h->st;
+    st.bits = (int)config->bits;
+    st.dtype = config->bits == 16 ? config->dtype : KIVI_DTYPE_BF16;
+    st.H = (int)config->num_kv_heads;
+    st.D = (int)config->head_dim;
+    st.page = (int)config->page_size;
+    st.shift = __builtin_ctz((unsigned)st.page);
+    st.num_pages = (int)config->num_pages;
+    st.row_bytes = st.D * st.bits / 8;
+    st.k = static_cast<unsigned char *>(d_keys);
+    st.v = static_cast<unsigned char *>(d_values);
+    st.kp = config->bits == 16 ? nullptr : reinterpret_cast<float2 *>(d_key_params);
+    st.vp = config->bits == 16 ? nullptr : reinterpret_cast<float2 *>(d_value_params);
+    h->device = device;
+    cudaError_t e;
+    if ((e = kivi::pages_scratch_floats(st, &h->scratch_floats)) != cudaSuccess ||
+        (e = dalloc(&st.status, 1)) != cudaSuccess ||
+        (e = cudaMemset(st.status, 0, sizeof(unsigned int))) != cudaSuccess ||
+        (e = dalloc(&h->scratch, (size_t)h->scratch_floats)) != cudaSuccess ||
+        (e = cudaEventCreateWithFlags(&h->done, cudaEventDisableTiming)) != cudaSuccess) {
+        rc = cuda_fail(err, e, "kivi_pages_new");
+        kivi_pages_free(h);
+        return rc;
+    }
+    *out = h;
+    return set_err(err, KIVI_OK);
+}
+
+void kivi_pages_free(kivi_pages *h) {
+    if (!h) return;
+    DeviceGuard dg(h->device);
+    // queued calls still use the status word and the scratch: cudaFree waits for them
+    dfree(h->st.status);
+    dfree(h->scratch);
+    if (h->done) cudaEventDestroy(h->done);
+    delete h;
+}
+
+int32_t kivi_pages_write_dev(kivi_pages *h, const kivi_pages_batch *batch, int32_t dtype, const void *d_keys,
+                             const void *d_values, uint64_t token_stride, uint64_t head_stride, void *stream,
+                             kivi_error *err) {
+    kivi::PagesBatch b;
+    kivi::PagesDense x;
+    int32_t rc = check_pages_batch(h, batch, &b, err);
+    if (!rc) rc = pages_dense(dtype, d_keys, d_values, token_stride, head_stride, b, &x, err);
+    if (rc) return rc;
+    DeviceGuard dg(h->device);
+    CUDA_TRY(kivi::launch_pages_write(h->st, b, x, (cudaStream_t)stream), "pages_write");
+    return set_err(err, KIVI_OK);
+}
+
+int32_t kivi_pages_read_dev(const kivi_pages *h, const kivi_pages_batch *batch, int32_t dtype, void *d_keys,
+                            void *d_values, uint64_t token_stride, uint64_t head_stride, void *stream,
+                            kivi_error *err) {
+    kivi::PagesBatch b;
+    kivi::PagesDense x;
+    int32_t rc = check_pages_batch(h, batch, &b, err);
+    if (!rc) rc = pages_dense(dtype, d_keys, d_values, token_stride, head_stride, b, &x, err);
+    if (!rc)
+        rc = check_pages_target((uint64_t)b.total, (uint64_t)h->st.H, token_stride, head_stride, (uint64_t)h->st.D,
+                                err);
+    if (rc) return rc;
+    DeviceGuard dg(h->device);
+    CUDA_TRY(kivi::launch_pages_read(h->st, b, x, (cudaStream_t)stream), "pages_read");
+    return set_err(err, KIVI_OK);
+}
+
+int32_t kivi_pages_attention_dev(kivi_pages *h, const kivi_pages_batch *batch, int32_t dtype, const void *d_query,
+                                 uint64_t num_q_heads, uint64_t query_token_stride, uint64_t query_head_stride,
+                                 float scale, uint64_t window, uint64_t sinks, void *d_out,
+                                 uint64_t out_token_stride, uint64_t out_head_stride, float *d_lse, void *stream,
+                                 kivi_error *err) {
+    kivi::PagesAttn a{};
+    int32_t rc = check_pages_batch(h, batch, &a.b, err);
+    if (rc) return rc;
+    if (dtype != KIVI_DTYPE_F16 && dtype != KIVI_DTYPE_BF16)
+        return set_msg(err, KIVI_ERR_UNSUPPORTED, "queries are F16 or BF16, not type %d", (int)dtype);
+    if (h->st.bits == 16 && dtype != h->st.dtype)
+        return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "queries of type %d over 16-bit pages of type %d", (int)dtype,
+                       h->st.dtype);
+    if (num_q_heads == 0 || num_q_heads % (uint64_t)h->st.H || num_q_heads > 65535)
+        return set_err(err, KIVI_ERR_QUERY_HEADS, num_q_heads, (uint64_t)h->st.H);
+    if (a.b.total > 0 && (!d_query || !d_out)) return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "null query or output");
+    if (((uintptr_t)d_query | (uintptr_t)d_out) % 2 || (uintptr_t)d_lse % 4)
+        return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "query, output and lse must start on an element boundary");
+    rc = check_pages_strides(query_token_stride, query_head_stride, err);
+    if (!rc) rc = check_pages_strides(out_token_stride, out_head_stride, err);
+    if (!rc)
+        rc = check_pages_target((uint64_t)a.b.total, num_q_heads, out_token_stride, out_head_stride,
+                                (uint64_t)h->st.D, err);
+    if (rc) return rc;
+    a.st = h->st;
+    a.q = d_query;
+    a.q_token = (int64_t)query_token_stride;
+    a.q_head = (int64_t)query_head_stride;
+    a.q_vec = rows_aligned(d_query, query_token_stride, query_head_stride, 2);
+    a.out = d_out;
+    a.o_token = (int64_t)out_token_stride;
+    a.o_head = (int64_t)out_head_stride;
+    a.o_vec = rows_aligned(d_out, out_token_stride, out_head_stride, 2);
+    a.lse = d_lse;
+    a.dtype = dtype;
+    a.Hq = (int)num_q_heads;
+    a.G = a.Hq / h->st.H;
+    a.scale = std::fabs(scale);
+    a.qsign = std::signbit(scale) ? -1.0f : 1.0f;
+    a.window = (int)std::min<uint64_t>(window, 0x7fffffffull);
+    a.sinks = window ? (int)std::min<uint64_t>(sinks, 0x7fffffffull) : 0;
+    a.part = h->scratch;
+    a.part_floats = h->scratch_floats;
+    DeviceGuard dg(h->device);
+    cudaStream_t st = (cudaStream_t)stream;
+    std::lock_guard<std::mutex> lk(h->mu);
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    CUDA_TRY(cudaStreamIsCapturing(st, &cap), "pages_attention");
+    const bool live = cap == cudaStreamCaptureStatusNone;
+    if (live && h->used && h->last != st) CUDA_TRY(cudaStreamWaitEvent(st, h->done, 0), "pages_attention");
+    CUDA_TRY(kivi::launch_pages_attention(a, st), "pages_attention");
+    if (live) {
+        CUDA_TRY(cudaEventRecord(h->done, st), "pages_attention");
+        h->last = st;
+        h->used = true;
+    }
+    return set_err(err, KIVI_OK);
+}
+
+int32_t kivi_pages_status(kivi_pages *h, kivi_error *err) {
+    if (!h) return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "null pages");
+    DeviceGuard dg(h->device);
+    CUDA_TRY(cudaDeviceSynchronize(), "pages_status");
+    unsigned int flag = 0;
+    CUDA_TRY(cudaMemcpy(&flag, h->st.status, sizeof(flag), cudaMemcpyDeviceToHost), "pages_status");
+    if (!flag) return set_err(err, KIVI_OK);
+    CUDA_TRY(cudaMemset(h->st.status, 0, sizeof(flag)), "pages_status");
+    if (flag & kivi::kPagesGaveUp)
+        return set_msg(err, KIVI_ERR_CUDA, "attention kernel gave up waiting for its copies (flag %u)", flag);
+    return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "%s%s%s",
+                   flag & kivi::kPagesBadPage ? "a block table named a page outside the store" : "",
+                   (flag & kivi::kPagesBadPage) && (flag & kivi::kPagesBadLengths) ? "; " : "",
+                   flag & kivi::kPagesBadLengths ? "offsets or lengths lie outside their arrays" : "");
 }

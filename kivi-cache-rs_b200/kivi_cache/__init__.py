@@ -195,6 +195,9 @@ def lib():
         "kivi_layer_kv_bytes": ([C.POINTER(_Config), sz, sz, sz], sz),
         "kivi_marginal_bytes_per_layer": ([C.POINTER(_Config), sz, sz], sz),
     }
+    from .pages import signatures
+
+    sig.update(signatures(P, sz, i32, f32, e))
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
         fn.argtypes = args
@@ -1243,3 +1246,7 @@ from .econ import (  # noqa: E402  (re-exported at the top level, as lib.rs does
     kv_budget_bytes,
     parse_context_tokens,
 )
+
+# ---------------------------------------------------------------- paged store
+
+from .pages import KvPages, PagesBatch, PagesConfig  # noqa: E402

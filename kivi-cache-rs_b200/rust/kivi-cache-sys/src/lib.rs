@@ -175,6 +175,44 @@ pub struct kivi_exchange {
     _private: [u8; 0],
 }
 
+pub const KIVI_DTYPE_F32: i32 = 0;
+pub const KIVI_DTYPE_F16: i32 = 1;
+pub const KIVI_DTYPE_BF16: i32 = 2;
+
+/// Geometry of a paged key/value store.
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default, PartialEq, Eq)]
+pub struct kivi_pages_config {
+    /// 16, 8 or 4
+    pub bits: u32,
+    /// element type of 16-bit rows
+    pub dtype: i32,
+    pub num_pages: u64,
+    pub page_size: u64,
+    pub num_kv_heads: u64,
+    pub head_dim: u64,
+}
+
+/// One step's sequences; the pointers are device memory.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct kivi_pages_batch {
+    pub block_table: *const i32,
+    pub table_stride: u64,
+    pub table_width: u64,
+    pub cu_tokens: *const i32,
+    pub kv_lens: *const i32,
+    pub batch: u64,
+    pub total_tokens: u64,
+    pub max_tokens: u64,
+}
+
+/// Handle over a paged key/value store, opaque.
+#[repr(C)]
+pub struct kivi_pages {
+    _private: [u8; 0],
+}
+
 #[link(name = "kivi_gpu")]
 extern "C" {
     pub fn kivi_abi_version() -> i32;
@@ -252,4 +290,11 @@ extern "C" {
     pub fn kivi_guard_cache(guard: *const kivi_guard) -> *const kivi_cache;
     pub fn kivi_guard_policy(guard: *const kivi_guard) -> i32;
     pub fn kivi_guard_sequence_length(guard: *const kivi_guard) -> u64;
+    pub fn kivi_pages_sizes(config: *const kivi_pages_config, data_bytes: *mut u64, param_floats: *mut u64, err: *mut kivi_error) -> i32;
+    pub fn kivi_pages_new(config: *const kivi_pages_config, d_keys: *mut c_void, d_values: *mut c_void, d_key_params: *mut f32, d_value_params: *mut f32, device: i32, out: *mut *mut kivi_pages, err: *mut kivi_error) -> i32;
+    pub fn kivi_pages_free(pages: *mut kivi_pages);
+    pub fn kivi_pages_write_dev(pages: *mut kivi_pages, batch: *const kivi_pages_batch, dtype: i32, d_keys: *const c_void, d_values: *const c_void, token_stride: u64, head_stride: u64, stream: *mut c_void, err: *mut kivi_error) -> i32;
+    pub fn kivi_pages_read_dev(pages: *const kivi_pages, batch: *const kivi_pages_batch, dtype: i32, d_keys: *mut c_void, d_values: *mut c_void, token_stride: u64, head_stride: u64, stream: *mut c_void, err: *mut kivi_error) -> i32;
+    pub fn kivi_pages_attention_dev(pages: *mut kivi_pages, batch: *const kivi_pages_batch, dtype: i32, d_query: *const c_void, num_q_heads: u64, query_token_stride: u64, query_head_stride: u64, scale: f32, window: u64, sinks: u64, d_out: *mut c_void, out_token_stride: u64, out_head_stride: u64, d_lse: *mut f32, stream: *mut c_void, err: *mut kivi_error) -> i32;
+    pub fn kivi_pages_status(pages: *mut kivi_pages, err: *mut kivi_error) -> i32;
 }
