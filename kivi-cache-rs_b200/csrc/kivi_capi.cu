@@ -2966,6 +2966,7 @@ int32_t kivi_pages_new(const kivi_pages_config *config, void *d_keys, void *d_va
         (e = dalloc(&st.status, 1)) != cudaSuccess ||
         (e = cudaMemset(st.status, 0, sizeof(unsigned int))) != cudaSuccess ||
         (e = dalloc(&h->scratch, (size_t)h->scratch_floats)) != cudaSuccess ||
+        (e = cudaMemset(h->scratch, 0, (size_t)h->scratch_floats * sizeof(float))) != cudaSuccess ||
         (e = cudaEventCreateWithFlags(&h->done, cudaEventDisableTiming)) != cudaSuccess) {
         rc = cuda_fail(err, e, "kivi_pages_new");
         kivi_pages_free(h);

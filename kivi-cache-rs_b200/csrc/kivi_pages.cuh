@@ -117,7 +117,13 @@ cudaError_t launch_pages_write(const PagesStore &st, const PagesBatch &b, const 
 cudaError_t launch_pages_read(const PagesStore &st, const PagesBatch &b, const PagesDense &x,
                               cudaStream_t s);
 cudaError_t launch_pages_attention(const PagesAttn &a, cudaStream_t s);
-// Floats of scratch a handle keeps for launch_pages_attention on this device.
+// Scratch that a handle keeps for launch_pages_attention on this device: partial
+// states, then kPagesCounters counters, zeroed once and left zero by every call.
+constexpr int kPagesCounters = 2048;
 cudaError_t pages_scratch_floats(const PagesStore &st, int64_t *floats);
+// One newest token per sequence, at most eight query heads per kv head
+// (kivi_pages_decode.cu).
+bool pages_decode_supported(const PagesAttn &a);
+cudaError_t launch_pages_decode(const PagesAttn &a, cudaStream_t s);
 
 } // namespace kivi

@@ -78,13 +78,17 @@ __global__ void __launch_bounds__(128) pages_rows_kernel(PagesAttn a) {
 
 } // namespace
 
-cudaError_t pages_scratch_floats(const PagesStore &, int64_t *floats) {
-    *floats = 0;
-    return cudaSuccess;
+cudaError_t pages_scratch_floats(const PagesStore &st, int64_t *floats) {
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    *floats = (int64_t)sms * 4 * 2 * 8 * (st.D + 2) + kPagesCounters;
+    return e;
 }
 
 cudaError_t launch_pages_attention(const PagesAttn &a, cudaStream_t s) {
     if (a.b.total == 0 || a.b.batch == 0 || a.b.most == 0) return cudaSuccess;
+    if (pages_decode_supported(a)) return launch_pages_decode(a, s);
     const int64_t warps = (int64_t)a.b.batch * a.b.most * a.Hq;
     const int64_t ctas = (warps + 3) / 4;
     if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
