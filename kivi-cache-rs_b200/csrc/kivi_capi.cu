@@ -2829,6 +2829,7 @@ struct kivi_pages {
     int device = 0;
     float *scratch = nullptr;   // the attention's partial states
     int64_t scratch_floats = 0;
+    kivi::PagesMaps maps{};
     cudaEvent_t done = nullptr; // after the last attention call outside a capture
     cudaStream_t last = nullptr; // its stream
     bool used = false;
@@ -2966,7 +2967,9 @@ int32_t kivi_pages_new(const kivi_pages_config *config, void *d_keys, void *d_va
         (e = dalloc(&st.status, 1)) != cudaSuccess ||
         (e = cudaMemset(st.status, 0, sizeof(unsigned int))) != cudaSuccess ||
         (e = dalloc(&h->scratch, (size_t)h->scratch_floats)) != cudaSuccess ||
-        (e = cudaMemset(h->scratch, 0, (size_t)h->scratch_floats * sizeof(float))) != cudaSuccess ||
+        (e = cudaMemset(h->scratch + h->scratch_floats - kivi::kPagesCounters, 0,
+                        kivi::kPagesCounters * sizeof(float))) != cudaSuccess ||
+        (st.bits == 16 && (e = kivi::pages_tensor_maps(st, &h->maps)) != cudaSuccess) ||
         (e = cudaEventCreateWithFlags(&h->done, cudaEventDisableTiming)) != cudaSuccess) {
         rc = cuda_fail(err, e, "kivi_pages_new");
         kivi_pages_free(h);
@@ -3052,12 +3055,14 @@ int32_t kivi_pages_attention_dev(kivi_pages *h, const kivi_pages_batch *batch, i
     a.dtype = dtype;
     a.Hq = (int)num_q_heads;
     a.G = a.Hq / h->st.H;
-    a.scale = std::fabs(scale);
+    // never 0: an unseen score is -inf, and -inf times 0 is not
+    a.scale = std::max(std::fabs(scale), 1e-37f);
     a.qsign = std::signbit(scale) ? -1.0f : 1.0f;
     a.window = (int)std::min<uint64_t>(window, 0x7fffffffull);
     a.sinks = window ? (int)std::min<uint64_t>(sinks, 0x7fffffffull) : 0;
     a.part = h->scratch;
     a.part_floats = h->scratch_floats;
+    a.maps = &h->maps;
     DeviceGuard dg(h->device);
     cudaStream_t st = (cudaStream_t)stream;
     std::lock_guard<std::mutex> lk(h->mu);

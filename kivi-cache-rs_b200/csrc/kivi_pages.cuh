@@ -16,6 +16,7 @@
 // so a step needs no host synchronisation and can be captured.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -62,6 +63,11 @@ struct PagesDense {
     bool vec; // rows start on 16-byte boundaries
 };
 
+// Tensor maps of 16-bit pages (host memory; passed to the kernel by value).
+struct PagesMaps {
+    CUtensorMap k, v;
+};
+
 struct PagesAttn {
     PagesStore st;
     PagesBatch b;
@@ -79,6 +85,7 @@ struct PagesAttn {
     int window, sinks;  // window 0: everything up to the row's own token
     float *part;        // scratch of kivi_pages handles
     int64_t part_floats;
+    const PagesMaps *maps;
 };
 
 // One sequence's span, clamped to its arrays: rows [start, start + n) of the
@@ -124,6 +131,11 @@ cudaError_t pages_scratch_floats(const PagesStore &st, int64_t *floats);
 // One newest token per sequence, at most eight query heads per kv head
 // (kivi_pages_decode.cu).
 bool pages_decode_supported(const PagesAttn &a);
+// Anything else (kivi_pages_chunk.cu).
+bool pages_chunk_supported(const PagesAttn &a);
+int64_t pages_chunk_scratch(int D, int sms); // floats
+cudaError_t pages_tensor_maps(const PagesStore &st, PagesMaps *maps);
+cudaError_t launch_pages_chunk(const PagesAttn &a, cudaStream_t s);
 cudaError_t launch_pages_decode(const PagesAttn &a, cudaStream_t s);
 
 } // namespace kivi

@@ -2,6 +2,8 @@
 // the paged store.
 #include <math.h>
 
+#include <algorithm>
+
 #include "kivi_internal.cuh"
 #include "kivi_pages.cuh"
 
@@ -82,13 +84,14 @@ cudaError_t pages_scratch_floats(const PagesStore &st, int64_t *floats) {
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    *floats = (int64_t)sms * 4 * 2 * 8 * (st.D + 2) + kPagesCounters;
+    *floats = std::max((int64_t)sms * 4 * 2 * 8 * (st.D + 2), pages_chunk_scratch(st.D, sms)) + kPagesCounters;
     return e;
 }
 
 cudaError_t launch_pages_attention(const PagesAttn &a, cudaStream_t s) {
     if (a.b.total == 0 || a.b.batch == 0 || a.b.most == 0) return cudaSuccess;
     if (pages_decode_supported(a)) return launch_pages_decode(a, s);
+    if (pages_chunk_supported(a)) return launch_pages_chunk(a, s);
     const int64_t warps = (int64_t)a.b.batch * a.b.most * a.Hq;
     const int64_t ctas = (warps + 3) / 4;
     if (ctas > 0x7fffffff) return cudaErrorInvalidValue;

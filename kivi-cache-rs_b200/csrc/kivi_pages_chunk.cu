@@ -1,0 +1,957 @@
+// kivi_pages_chunk.cu -- several new tokens per sequence (prompt chunks, drafts)
+// or many query heads per kv head against the paged store, on the
+// 5th-generation tensor cores.
+//
+// A block is the packed query rows (token, head of the kv head's group) of up to
+// 256 / G consecutive new tokens: two row tiles, A and B, of 128.  Per 128
+// cached tokens
+//   S = Q K^T  tcgen05.mma, M = N = 128, Q and K in shared memory (128-byte
+//              swizzle, K-major), S in tensor memory;
+//   softmax    one thread per row: its S row from tensor memory, running maximum
+//              and sum in fp32, P (16 bits) back over S;
+//   O += P V   P from tensor memory, V in shared memory as it lies in the page
+//              ([token][channel] = MN-major), O in tensor memory.
+// The tiles A and B take turns: while one's softmax runs, the tensor pipe does
+// the other's O += P V and its next S.  A block of at most 128 rows has one row
+// tile; A then takes its even and B its odd cached tiles, and their states are
+// joined at the end (tensor memory lanes are the rows, so A's threads read B's O
+// from their own lanes).
+//
+// The maximum that P refers to moves only when a row exceeds it by 2^8: P stays
+// within its type and O is rarely rescaled.  A row sees tokens by its position;
+// unseen scores are replaced by -inf, and in tiles of which some row does not see
+// some token, V rows that nobody sees are zeroed and infinities and NaN are taken
+// out before O += P V (0 times infinity is not 0) and added to the rows that do
+// see them apart.
+//
+// Work split: blocks x kv heads x cached tiles form one flat list, and each of
+// the persistent CTAs (one per SM) takes an equal run of it: no last wave, any
+// mix of lengths.  A (block, head) that spans CTAs leaves partial states in the
+// handle's scratch; the CTA that finishes last joins them in CTA order.
+//
+// Warps: 0-3 softmax of A, 4-7 of B, 8 MMA issue, 9 copies (TMA tensor maps over
+// the pages, a box per page and 64 channels), 10-11 the masked tiles' V rows.
+#include <cudaTypedefs.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "kivi_internal.cuh"
+#include "kivi_pages.cuh"
+
+namespace kivi {
+namespace {
+
+constexpr int kTok = 128;                 // cached tokens per tile
+constexpr int kRows = 128;                // rows of one row tile
+constexpr int kSoft = 8;                  // softmax warps
+constexpr int kMmaWarp = 8, kCopyWarp = 9, kFixWarp = 10; // and 11
+constexpr int kThreads = 384;
+constexpr int kStages = 5;                // K and V tiles in flight
+constexpr int kPanel = 16384;             // 128 rows x 64 channels
+constexpr long long kWait = 2000000000LL; // ~1 s
+constexpr float kLazy = 8.0f;
+constexpr int kSoftRegs = 200, kRoleRegs = 96;
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColS = 0, kColO = 256; // + 128 for B
+
+__device__ __forceinline__ uint32_t su32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint64_t *b, uint32_t n) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t *b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(b)) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t *b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(su32(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t *b, uint32_t par) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done)
+                 : "r"(su32(b)), "r"(par)
+                 : "memory");
+    return done != 0;
+}
+// Bounded wait of a whole warp, one verdict for all its lanes; on timeout the
+// handle's status records it.
+__device__ __forceinline__ bool warp_wait(uint64_t *b, uint32_t par, unsigned int *status) {
+    bool ok = bar_try(b, par);
+    if (!ok) {
+        const long long t0 = clock64();
+        while (!(ok = bar_try(b, par)))
+            if (clock64() - t0 > kWait) {
+                atomicOr(status, kPagesGaveUp);
+                break;
+            }
+    }
+    return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// The 256 softmax threads (every other warp may be elsewhere).
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// Shared-memory matrix descriptor, 128-byte swizzle (layout 2), version 1.
+// K-major: sbo = 1024 between groups of 8 rows.  MN-major: sbo = 1024 between
+// groups of 8 tokens, lbo = one 64-channel panel.
+__device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
+           ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// kind::f16: fp32 D, A and B of one type (1 = bf16), A K-major
+__device__ __forceinline__ uint32_t idesc(int bf16, int N, int b_mn_major) {
+    return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)b_mn_major << 16) |
+           ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+}
+
+// MMAs over up to one 64-channel panel (both operands in shared memory, 32 bytes
+// a step), N of them, by one elected lane; the first accumulates iff acc.
+#define KIVI_SS_HEAD                                                                                     \
+    "{\n\t.reg .pred p, e, t;\n\t.reg .b64 a, b;\n\telect.sync _|e, 0xffffffff;\n\t"                      \
+    "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 t, %5, 0;\n\tmov.b64 a, %1;\n\tmov.b64 b, %2;\n\t"              \
+    "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
+#define KIVI_SS_STEP                                                                                     \
+    "add.u64 a, a, 2;\n\tadd.u64 b, b, 2;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+template <int N> __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    static_assert(N == 2 || N == 4, "steps");
+    if constexpr (N == 4)
+        asm volatile(KIVI_SS_HEAD KIVI_SS_STEP KIVI_SS_STEP KIVI_SS_STEP "}" ::"r"(d), "l"(a), "l"(b), "r"(id),
+                     "r"(acc), "r"(1u));
+    else
+        asm volatile(KIVI_SS_HEAD KIVI_SS_STEP "}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc), "r"(1u));
+}
+// O += P V over 128 tokens: 8 steps, P 8 columns and V 2048 bytes a step.
+#define KIVI_TS_STEP                                                                                     \
+    "add.u32 a, a, 8;\n\tadd.u64 b, b, 128;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+__device__ __forceinline__ void mma_pv(uint32_t d, uint32_t a, uint64_t b, uint32_t id) {
+    asm volatile("{\n\t.reg .pred e, t;\n\t.reg .b32 a;\n\t.reg .b64 b;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "setp.ne.b32 t, %4, 0;\n\tmov.b32 a, %1;\n\tmov.b64 b, %2;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t" KIVI_TS_STEP KIVI_TS_STEP KIVI_TS_STEP
+                     KIVI_TS_STEP KIVI_TS_STEP KIVI_TS_STEP KIVI_TS_STEP "}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(id), "r"(1u));
+}
+#undef KIVI_SS_HEAD
+#undef KIVI_SS_STEP
+#undef KIVI_TS_STEP
+// Arrives on b when every MMA issued so far has completed.
+__device__ __forceinline__ void mma_commit(uint64_t *b) {
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(su32(b))
+                 : "memory");
+}
+__device__ __forceinline__ void copy_box(void *dst, const CUtensorMap *map, int x, int y, uint64_t *b) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+                 "[%4];" ::"r"(su32(dst)),
+                 "l"(map), "r"(x), "r"(y), "r"(su32(b))
+                 : "memory");
+}
+
+// 64 consecutive 32-bit columns of this thread's tensor-memory lane.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float *v) {
+    uint32_t r[64];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+                 "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+                 "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+                 "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+                   "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+                   "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+                   "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+                   "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+                 : "r"(taddr)
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
+// 32 consecutive 32-bit columns of this thread's tensor-memory lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *v) {
+    uint32_t r[32];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+                 "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr)
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
+                 "%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+                 ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                 "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+                 "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+                 "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+                 : "memory");
+}
+
+// 2^x (relative error 2^-22, -inf -> 0)
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// (a0, a1) * m + c, one instruction
+__device__ __forceinline__ void fma2s(float &a0, float &a1, float m, float c) {
+    asm("{\n\t.reg .b64 ra, rm, rc;\n\tmov.b64 ra, {%0, %1};\n\tmov.b64 rm, {%2, %2};\n\tmov.b64 rc, {%3, %3};\n\t"
+        "fma.rn.f32x2 ra, ra, rm, rc;\n\tmov.b64 {%0, %1}, ra;\n\t}"
+        : "+f"(a0), "+f"(a1)
+        : "f"(m), "f"(c));
+}
+__device__ __forceinline__ void add2(float &a0, float &a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 ra, rb;\n\tmov.b64 ra, {%0, %1};\n\tmov.b64 rb, {%2, %3};\n\tadd.rn.f32x2 ra, ra, rb;\n\t"
+        "mov.b64 {%0, %1}, ra;\n\t}"
+        : "+f"(a0), "+f"(a1)
+        : "f"(b0), "f"(b1));
+}
+template <bool F16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (F16) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+__device__ __forceinline__ float unpack(bool f16, uint16_t x) {
+    return f16 ? __half2float(__ushort_as_half(x)) : __uint_as_float((uint32_t)x << 16);
+}
+
+// ---------------------------------------------------------------- the flat list
+
+// One block of one sequence: its rows, what they see, its cached tiles (the
+// first `ns` hold first tokens, then come tiles ws ..).
+struct Block {
+    int b, i0, ntok;       // sequence, first new token and number of them
+    int start, n, kv;      // the sequence's span
+    int p0, p1;            // positions of the first and last token
+    int lo, ns, ws, nt;
+};
+__device__ __forceinline__ Block make_block(const PagesAttn &a, int TB, int b, const Span &s, int i) {
+    Block k;
+    k.b = b, k.start = s.start, k.n = s.n, k.kv = s.kv;
+    k.i0 = i * TB;
+    k.ntok = min(TB, s.n - k.i0);
+    k.p0 = s.kv - s.n + k.i0;
+    k.p1 = k.p0 + k.ntok - 1;
+    k.lo = a.window ? max(0, k.p0 - a.window + 1) : 0;
+    k.ws = k.lo / kTok;
+    k.ns = min((min(a.sinks, k.lo) + kTok - 1) / kTok, k.ws);
+    // rows that see nothing still need a tile: it writes their zeros
+    k.nt = max(1, k.ns + max(0, (k.p1 >= 0 ? k.p1 / kTok + 1 : 0) - k.ws));
+    return k;
+}
+__device__ __forceinline__ int blocks_of(int n, int TB) { return (n + TB - 1) / TB; }
+
+// A CTA's run of the list, walked the same way by every role.
+struct Walk {
+    long long f, end, row0; // tiles of the flat list; first tile of the current (block, head)
+    int i, h;               // block of the sequence, head
+    Block k;
+};
+// One (block, head)'s part in this CTA: tiles t0 .. t1 - 1 of its nt.
+struct Seg {
+    int t0, t1;
+    int rows;     // query rows
+    bool dual;    // one row tile: A takes even tiles, B odd ones
+    int nA, nB;   // tiles of each
+};
+__device__ __forceinline__ Seg seg_of(const PagesAttn &a, const Walk &w) {
+    Seg s;
+    s.t0 = (int)(w.f - w.row0);
+    s.t1 = (int)min((long long)w.k.nt, w.end - w.row0);
+    const int n = s.t1 - s.t0;
+    s.rows = w.k.ntok * a.G;
+    s.dual = s.rows <= kRows;
+    if (s.dual) {
+        s.nA = (n + 1) / 2, s.nB = n / 2;
+    } else {
+        // A's last row sees no tile past its own
+        const int pA = w.k.p0 + (kRows - 1) / a.G;
+        const int tA = max(1, w.k.ns + max(0, (pA >= 0 ? pA / kTok + 1 : 0) - w.k.ws));
+        s.nA = max(0, min(tA - s.t0, n)), s.nB = n;
+    }
+    return s;
+}
+__device__ __forceinline__ bool walk_next(const PagesAttn &a, int TB, Walk &w, const Seg &s) {
+    w.f = w.row0 + s.t1;
+    if (w.f >= w.end) return false;
+    w.row0 = w.f;
+    if (++w.h < a.st.H) return true;
+    w.h = 0;
+    Span sp{w.k.start, w.k.n, w.k.kv};
+    int b = w.k.b;
+    if (++w.i >= blocks_of(w.k.n, TB)) {
+        w.i = 0;
+        do {
+            sp = pages_span(a.b, a.st, ++b);
+        } while (sp.n == 0);
+    }
+    w.k = make_block(a, TB, b, sp, w.i);
+    return true;
+}
+__device__ __forceinline__ int tile_token(const Block &k, int t) { return (t < k.ns ? t : t - k.ns + k.ws) * kTok; }
+// Some row of the block does not see some token of the tile.
+__device__ __forceinline__ bool tile_edge(const PagesAttn &a, const Block &k, int T) {
+    if (T + kTok - 1 > k.p0) return true;
+    return a.window && T < k.p1 - a.window + 1 && T + kTok > a.sinks;
+}
+// Some row of the block sees token t.
+__device__ __forceinline__ bool token_seen(const PagesAttn &a, const Block &k, int t) {
+    return t <= k.p1 && (t >= k.lo || t < a.sinks);
+}
+
+struct Shared {
+    uint64_t full[kStages], empty[kStages];
+    uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+    uint64_t edge[4], half[4], drain; // an edge tile's V has landed, before the fixing warps
+    uint32_t flags[4][4]; // tokens of an edge tile whose value row is not finite
+    uint32_t tmem;
+    int last;
+    long long scan[kThreads / 32];
+    long long begin, per;
+    Walk walk;
+    float2 ml[kRows]; // B's (m, l) when it shares A's rows
+};
+
+static_assert(sizeof(Shared) + 1024 + 7 * 2 * kPanel <= 232448, "shared memory per block");
+constexpr int smem_bytes(int np) { return 2 * np * kPanel + kStages * np * kPanel + (int)sizeof(Shared) + 1024; }
+
+template <int NP, bool F16>
+__global__ void __launch_bounds__(kThreads, 1)
+    pages_chunk_kernel(const PagesAttn a, int TB, int min_per, int *counters, const __grid_constant__ CUtensorMap kmap,
+                       const __grid_constant__ CUtensorMap vmap) {
+    extern __shared__ unsigned char raw[];
+    unsigned char *sm = raw + ((1024 - (su32(raw) & 1023)) & 1023);
+    unsigned char *sq = sm, *ring = sm + 2 * NP * kPanel;
+    Shared &sh = *reinterpret_cast<Shared *>(ring + kStages * NP * kPanel);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const PagesStore &st = a.st;
+    const int H = st.H, G = a.G, D = st.D;
+    unsigned int *status = st.status;
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) bar_init(&sh.full[i], 1), bar_init(&sh.empty[i], 1);
+        for (int x = 0; x < 2; ++x) {
+            bar_init(&sh.q_full[x], 4);
+            bar_init(&sh.s_full[x], 1);
+            bar_init(&sh.p_full[x], 4);
+            bar_init(&sh.o_full[x], 1);
+        }
+        for (int i = 0; i < 4; ++i) bar_init(&sh.edge[i], 1), bar_init(&sh.half[i], 1);
+        bar_init(&sh.drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&sh.tmem)),
+                     "n"(kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (warp == kCopyWarp && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
+    }
+    pdl_wait();
+    pdl_trigger();
+
+    // ---- the flat list: blocks of every sequence (prefix in shared memory), the
+    // tiles of all of them, this CTA's run and the block it starts in
+    int *pre = reinterpret_cast<int *>(sm); // [batch + 1], before the pipeline starts
+    const int nw = kThreads / 32;
+    auto scan = [&](long long v, long long &total) { // exclusive, over the CTA
+        long long inc = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
+        }
+        __syncthreads();
+        if (lane == 31) sh.scan[warp] = inc;
+        __syncthreads();
+        long long before = 0;
+        total = 0;
+        for (int w = 0; w < nw; ++w) {
+            if (w < warp) before += sh.scan[w];
+            total += sh.scan[w];
+        }
+        return before + inc - v;
+    };
+    long long items = 0, sum;
+    for (int b0 = 0; b0 < a.b.batch; b0 += kThreads) {
+        const int b = b0 + tid;
+        const int n = b < a.b.batch ? blocks_of(pages_span(a.b, st, b).n, TB) : 0;
+        const long long at = items + scan(n, sum);
+        if (b < a.b.batch) pre[b] = (int)at;
+        items += sum;
+    }
+    if (tid == 0) pre[a.b.batch] = (int)items;
+    __syncthreads();
+    auto block_at = [&](int k, int &i) { // item k: its sequence and block
+        int lo = 0, hi = a.b.batch; // pre[lo] <= k < pre[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (pre[mid] <= k) lo = mid;
+            else hi = mid;
+        }
+        i = k - pre[lo];
+        return make_block(a, TB, lo, pages_span(a.b, st, lo), i);
+    };
+    long long tiles = 0;
+    int bi;
+    for (int k0 = 0; k0 < items; k0 += kThreads) {
+        const int k = k0 + tid;
+        scan(k < items ? block_at(k, bi).nt : 0, sum);
+        tiles += sum;
+    }
+    tiles *= H;
+    const long long per = max((tiles + gridDim.x - 1) / gridDim.x, (long long)min_per);
+    const long long begin = per * blockIdx.x, end = min(tiles, begin + per);
+    if (begin < end) {
+        long long run = 0;
+        for (int k0 = 0; k0 < items && run <= begin; k0 += kThreads) {
+            const int k = k0 + tid;
+            Block blk{};
+            if (k < items) blk = block_at(k, bi);
+            const long long nt = k < items ? (long long)blk.nt * H : 0;
+            const long long first = run + scan(nt, sum);
+            if (nt > 0 && begin >= first && begin < first + nt) {
+                Walk w;
+                w.f = begin, w.end = end;
+                w.h = (int)((begin - first) / blk.nt);
+                w.row0 = first + (long long)w.h * blk.nt;
+                w.i = bi;
+                w.k = blk;
+                sh.walk = w;
+            }
+            run += sum;
+        }
+    }
+    proxy_fence(); // the prefix's place goes to the copies
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tm = sh.tmem;
+    Walk w = sh.walk;
+    bool more = begin < end, ok = true;
+
+    // registers: 384 x 168 at launch = 256 x kSoftRegs + 128 x kRoleRegs and a rest
+    static_assert(256 * kSoftRegs + 128 * kRoleRegs <= kThreads * 168, "register split");
+    if (warp < kSoft)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+    else
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
+    if (warp < kSoft) {
+        // ------------------------------------------------------------ softmax
+        const int X = warp >> 2;             // A or B
+        const int row = tid & 127;           // tensor-memory lane
+        const uint32_t lanes = tm + ((uint32_t)(32 * (warp & 3)) << 16);
+        const uint32_t cS = lanes + kColS + 128 * X, cO = lanes + kColO + 128 * X;
+        const float crow = a.scale * 1.4426950408889634f;
+        uint32_t ns = 0, no = 0, ne = 0, item = 0; // tiles, blocks, edge tiles and copies so far
+        while (more) {
+            const Seg s = seg_of(a, w);
+            const Block &k = w.k;
+            const int nX = X ? s.nB : s.nA;
+            const int r0 = X && !s.dual ? kRows : 0;
+            const bool live = r0 + row < s.rows;
+            const int tok = live ? (r0 + row) / G : 0, head = live ? r0 + row - tok * G : 0;
+            const int p = live ? k.p0 + tok : -1;
+            const int lo = a.window ? max(0, p - a.window + 1) : 0;
+            const bool any = __any_sync(0xffffffffu, live);
+            float m = -INFINITY, l = 0.0f;
+            if (r0 < s.rows) {
+                // ---- the row's query, and an empty O
+                if (!(X && s.dual)) {
+                    const uint16_t *q = static_cast<const uint16_t *>(a.q) + (int64_t)(k.start + k.i0 + tok) * a.q_token +
+                                        (int64_t)(w.h * G + head) * a.q_head;
+                    unsigned char *dst = sq + X * NP * kPanel + row * 128;
+                    for (int c = 0; c < D / 8; ++c) {
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (live) {
+                            if (a.q_vec) {
+                                v = __ldg(reinterpret_cast<const uint4 *>(q) + c);
+                            } else {
+                                uint32_t e[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) e[i] = q[8 * c + 2 * i] | (uint32_t)q[8 * c + 2 * i + 1] << 16;
+                                v = make_uint4(e[0], e[1], e[2], e[3]);
+                            }
+                            if (a.qsign < 0.0f) v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
+                        }
+                        *reinterpret_cast<uint4 *>(dst + (c >> 3) * kPanel + (((c & 7) ^ (row & 7)) << 4)) = v;
+                    }
+                }
+                {
+                    uint32_t z[32] = {};
+                    for (int c = 0; c < D; c += 32) tmem_st32(cO + c, z);
+                    st_wait();
+                }
+                proxy_fence();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&sh.q_full[X]);
+            }
+            for (int j = 0; ok && j < (s.dual ? s.t1 - s.t0 : nX); ++j) {
+                const int T = tile_token(k, s.t0 + j);
+                const bool edge = tile_edge(a, k, T);
+                const uint32_t e = ne;
+                if (edge) ++ne;
+                if (s.dual && (j & 1) != X) continue;
+                if (!warp_wait(&sh.s_full[X], ns & 1, status)) {
+                    ok = false;
+                    break;
+                }
+                ++ns;
+                tc_after();
+                if (any) {
+                    float x[128];
+                    tmem_ld64(cS, x);
+                    tmem_ld64(cS + 64, x + 64);
+                    if (edge) {
+                        const int hi = p - T, lw = lo - T, sk = a.sinks - T;
+#pragma unroll
+                        for (int i = 0; i < 128; ++i)
+                            if (i > hi || (i < lw && i >= sk)) x[i] = -INFINITY;
+                    }
+                    float m4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                    for (int i = 4; i < 124; i += 8) {
+                        m4[0] = max3(m4[0], x[i], x[i + 1]);
+                        m4[1] = max3(m4[1], x[i + 2], x[i + 3]);
+                        m4[2] = max3(m4[2], x[i + 4], x[i + 5]);
+                        m4[3] = max3(m4[3], x[i + 6], x[i + 7]);
+                    }
+                    const float mx = fmaxf(max3(max3(m4[0], x[124], x[125]), max3(m4[1], x[126], x[127]), m4[2]), m4[3]) * crow;
+                    const bool need = mx > m + kLazy, move = need && m != -INFINITY;
+                    const float f = move ? ex2(m - mx) : 1.0f;
+                    if (need) m = mx;
+                    if (__any_sync(0xffffffffu, move)) {
+                        l *= f;
+                        // every O += P V of earlier tiles is complete: S of this one was issued after them
+                        for (int c = 0; c < D; c += 32) {
+                            float o[32];
+                            tmem_ld32(cO + c, o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] *= f;
+                            tmem_st32(cO + c, reinterpret_cast<const uint32_t *>(o));
+                        }
+                    }
+                    const float off = m == -INFINITY ? 0.0f : -m;
+                    float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
+#pragma unroll
+                    for (int hlf = 0; hlf < 2; ++hlf) {
+                        uint32_t pk[32];
+#pragma unroll
+                        for (int i = 0; i < 64; i += 4) {
+                            float *y = x + 64 * hlf + i;
+                            fma2s(y[0], y[1], crow, off);
+                            fma2s(y[2], y[3], crow, off);
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) y[q] = ex2(y[q]);
+                            add2(a0, a1, y[0], y[1]);
+                            add2(a2, a3, y[2], y[3]);
+                            pk[i / 2] = pack2<F16>(y[0], y[1]);
+                            pk[i / 2 + 1] = pack2<F16>(y[2], y[3]);
+                        }
+                        tmem_st32(cS + 32 * hlf, pk);
+                    }
+                    l += (a0 + a1) + (a2 + a3);
+                }
+                if (edge) {
+                    // value rows with infinities or NaN: taken out of the tile, added here to
+                    // the rows that see them (p > 0, so p v is v)
+                    const uint32_t it = item + 2 * j + 1;
+                    if (!warp_wait(&sh.full[it % kStages], (it / kStages) & 1, status)) {
+                        ok = false;
+                        break;
+                    }
+                    for (int f4 = 0; f4 < 4; ++f4) {
+                        uint32_t bits = sh.flags[e & 3][f4];
+                        while (bits) {
+                            const int t = T + 32 * f4 + __ffs((int)bits) - 1;
+                            bits &= bits - 1;
+                            const bool see = t <= p && (t >= lo || t < a.sinks);
+                            const int64_t r = pages_row(st, max(pages_page(a.b, st, k.b, t), 0), w.h, t);
+                            const uint16_t *v = reinterpret_cast<const uint16_t *>(st.v + r * st.row_bytes);
+                            for (int c = 0; c < D; c += 32) {
+                                float o[32];
+                                tmem_ld32(cO + c, o);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    const float y = unpack(F16, v[c + i]);
+                                    if (see && !isfinite(y)) o[i] += y;
+                                }
+                                tmem_st32(cO + c, reinterpret_cast<const uint32_t *>(o));
+                                st_wait();
+                            }
+                        }
+                    }
+                }
+                st_wait();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&sh.p_full[X]);
+            }
+            for (int j = nX; !s.dual && j < s.t1 - s.t0; ++j) ne += tile_edge(a, k, tile_token(k, s.t0 + j));
+            item += 2 * (s.t1 - s.t0);
+            // ---- the rows out
+            if (ok && nX > 0) {
+                if (warp_wait(&sh.o_full[X], no & 1, status)) ++no;
+                else ok = false;
+                tc_after();
+            }
+            const int c0 = (int)(w.row0 / per), c1 = (int)((w.row0 + k.nt - 1) / per);
+            const bool whole = c0 == c1;
+            float fa = 1.0f, fb = 0.0f;
+            if (s.dual) {
+                if (X) sh.ml[row] = make_float2(m, l);
+                tc_before();
+                soft_sync();
+                tc_after();
+                if (!X) {
+                    const float2 y = sh.ml[row];
+                    const float nm = fmaxf(m, y.x), ref = nm == -INFINITY ? 0.0f : nm;
+                    fa = ex2(m - ref), fb = ex2(y.x - ref);
+                    m = nm;
+                    l = l * fa + y.y * fb;
+                }
+            }
+            const int64_t stride = D + 4;
+            float *part = a.part + ((int64_t)blockIdx.x * 2 + (c0 == (int)blockIdx.x ? 1 : 0)) * (2 * kRows) * stride +
+                          (r0 + row) * stride;
+            if (any && !(X && s.dual)) {
+                const bool sees = p >= 0;
+                const float inv = sees ? 1.0f / l : 0.0f;
+                const int64_t otok = k.start + k.i0 + tok;
+                uint16_t *out = static_cast<uint16_t *>(a.out) + otok * a.o_token + (int64_t)(w.h * G + head) * a.o_head;
+                for (int c = 0; c < D; c += 32) {
+                    float o[32];
+                    tmem_ld32(cO + c, o);
+                    if (s.dual) {
+                        float o2[32];
+                        tmem_ld32(cO + 128 + c, o2);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = o[i] * fa + o2[i] * fb;
+                    }
+                    uint32_t y[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        y[i] = sees ? pack2<F16>(o[2 * i] * inv, o[2 * i + 1] * inv) : 0u;
+                    // (no early exit: the tensor-memory loads are the whole warp's)
+                    if (live && !whole) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<float4 *>(part + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    } else if (live && a.o_vec) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            *reinterpret_cast<uint4 *>(out + c + 8 * i) = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                    } else if (live) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) out[c + i] = (uint16_t)(y[i / 2] >> (16 * (i & 1)));
+                    }
+                    __syncwarp();
+                }
+                if (live && whole && a.lse)
+                    a.lse[otok * a.Hq + w.h * G + head] = sees ? m * 0.6931471805599453f + logf(l) : -INFINITY;
+                if (live && !whole) {
+                    part[D] = m;
+                    part[D + 1] = l;
+                }
+            }
+            if (!whole) {
+                // ---- the last CTA of the (block, head) joins its parts
+                __threadfence();
+                soft_sync();
+                if (tid == 0) {
+                    sh.last = atomicAdd(counters + c0, 1) == c1 - c0;
+                    if (sh.last) counters[c0] = 0; // for the next call
+                }
+                soft_sync();
+                if (sh.last) {
+                    __threadfence();
+                    const int D4 = D / 4;
+                    for (int i = tid; i < s.rows * D4; i += 256) {
+                        const int r = i / D4, c = i - r * D4;
+                        const int tk = r / G, hd = r - tk * G;
+                        float mm = -INFINITY, ll = 0.0f;
+                        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        for (int x = c0; x <= c1; ++x) {
+                            const float *pp = a.part + (((int64_t)x * 2 + (x == c0 ? 1 : 0)) * (2 * kRows) + r) * stride;
+                            const float4 y = __ldcg(reinterpret_cast<const float4 *>(pp) + c);
+                            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(pp + D));
+                            const float nm = fmaxf(mm, ml.x), ref = nm == -INFINITY ? 0.0f : nm;
+                            const float f0 = ex2(mm - ref), f1 = ex2(ml.x - ref);
+                            mm = nm;
+                            ll = ll * f0 + ml.y * f1;
+                            acc.x = acc.x * f0 + y.x * f1, acc.y = acc.y * f0 + y.y * f1;
+                            acc.z = acc.z * f0 + y.z * f1, acc.w = acc.w * f0 + y.w * f1;
+                        }
+                        const bool sees = k.p0 + tk >= 0;
+                        const float inv = 1.0f / ll;
+                        uint2 y = make_uint2(0, 0);
+                        if (sees) y = make_uint2(pack2<F16>(acc.x * inv, acc.y * inv), pack2<F16>(acc.z * inv, acc.w * inv));
+                        const int64_t otok = k.start + k.i0 + tk;
+                        uint16_t *d = static_cast<uint16_t *>(a.out) + otok * a.o_token + (int64_t)(w.h * G + hd) * a.o_head + 4 * c;
+                        if (a.o_vec) {
+                            *reinterpret_cast<uint2 *>(d) = y;
+                        } else {
+                            d[0] = (uint16_t)y.x, d[1] = (uint16_t)(y.x >> 16), d[2] = (uint16_t)y.y, d[3] = (uint16_t)(y.y >> 16);
+                        }
+                        if (a.lse && c == 0)
+                            a.lse[otok * a.Hq + w.h * G + hd] = sees ? mm * 0.6931471805599453f + logf(ll) : -INFINITY;
+                    }
+                }
+            }
+            if (s.dual) { // B's O and (m, l) are read
+                tc_before();
+                soft_sync();
+                tc_after();
+            }
+            // after a wait that gave up the walk goes on without waiting, so that the
+            // 256 threads still meet at their barriers
+            more = walk_next(a, TB, w, s);
+        }
+    } else if (warp == kMmaWarp) {
+        // ------------------------------------------------------------ MMA issue
+        const uint32_t id_qk = idesc(!F16, kTok, 0), id_pv = idesc(!F16, D, 1);
+        const uint64_t dq = sdesc(su32(sq), 16, 1024), dr = sdesc(su32(ring), 16, 1024),
+                       dv = sdesc(su32(ring), kPanel, 1024);
+        uint32_t np[2] = {0, 0}, nq[2] = {0, 0}, item = 0;
+        while (more && ok) {
+            const Seg s = seg_of(a, w);
+            const int n = s.t1 - s.t0;
+            // tile (of the segment) that X takes as its i-th
+            auto tile = [&](int X, int i) { return s.dual ? 2 * i + X : i; };
+            // this use of a tile is its last
+            auto frees = [&](int X, int t) { return s.dual || X == 1 || t >= s.nB; };
+            auto qk = [&](int X, int i) {
+                const int t = tile(X, i);
+                const uint32_t it = item + 2 * t, slot = it % kStages;
+                if (i == 0 && !warp_wait(&sh.q_full[X], nq[X]++ & 1, status)) return false;
+                if (!warp_wait(&sh.full[slot], (it / kStages) & 1, status)) return false;
+                tc_after();
+                const uint32_t d = tm + kColS + 128 * X;
+                const uint64_t q = dq + (uint64_t)(s.dual ? 0 : X) * (NP * kPanel / 16);
+                const uint64_t b = dr + (uint64_t)slot * (NP * kPanel / 16);
+                if (D == 32) {
+                    mma_ss<2>(d, q, b, id_qk, 0u);
+                } else {
+                    mma_ss<4>(d, q, b, id_qk, 0u);
+                    if (D == 96) mma_ss<2>(d, q + kPanel / 16, b + kPanel / 16, id_qk, 1u);
+                    if (D == 128) mma_ss<4>(d, q + kPanel / 16, b + kPanel / 16, id_qk, 1u);
+                }
+                mma_commit(&sh.s_full[X]);
+                if (frees(X, t)) mma_commit(&sh.empty[slot]);
+                return true;
+            };
+            auto pv = [&](int X, int i) {
+                const int t = tile(X, i);
+                const uint32_t it = item + 2 * t + 1, slot = it % kStages;
+                if (!warp_wait(&sh.full[slot], (it / kStages) & 1, status)) return false;
+                if (!warp_wait(&sh.p_full[X], np[X] & 1, status)) return false;
+                ++np[X];
+                tc_after();
+                mma_pv(tm + kColO + 128 * X, tm + kColS + 128 * X, dv + (uint64_t)slot * (NP * kPanel / 16), id_pv);
+                if (frees(X, t)) mma_commit(&sh.empty[slot]);
+                if (i + 1 == (X ? s.nB : s.nA)) mma_commit(&sh.o_full[X]);
+                return true;
+            };
+            // rows without a tile in this run still load their queries
+            if (s.nA > 0) ok = qk(0, 0);
+            else if (!s.dual) ok = warp_wait(&sh.q_full[0], nq[0]++ & 1, status);
+            if (ok && s.nB > 0) ok = qk(1, 0);
+            else if (ok && s.dual) ok = warp_wait(&sh.q_full[1], nq[1]++ & 1, status);
+            for (int i = 0; ok && i < max(s.nA, s.nB); ++i) {
+                if (i < s.nA) ok = pv(0, i) && (i + 1 >= s.nA || qk(0, i + 1));
+                if (ok && i < s.nB) ok = pv(1, i) && (i + 1 >= s.nB || qk(1, i + 1));
+            }
+            item += 2 * n;
+            if (ok) more = walk_next(a, TB, w, s);
+        }
+        mma_commit(&sh.drain); // tensor memory outlives every MMA
+        warp_wait(&sh.drain, 0, status);
+    } else if (warp == kCopyWarp) {
+        // ------------------------------------------------------------ copies
+        const int box = min(st.page, kTok), pieces = kTok / box;
+        const int piece = lane / NP, panel = lane - piece * NP; // of the lane's box; pieces * NP <= 16
+        uint32_t item = 0, ne = 0;
+        while (more && ok) {
+            const Seg s = seg_of(a, w);
+            const Block &k = w.k;
+            for (int j = 0; ok && j < s.t1 - s.t0; ++j) {
+                const int T = tile_token(k, s.t0 + j), t = T + piece * box;
+                // a box is needed if some row sees one of its tokens
+                bool need = piece < pieces && t <= k.p1 && (t + box > k.lo || t < a.sinks);
+                int y = 0;
+                if (need) y = (int)pages_row(st, max(pages_page(a.b, st, k.b, t), 0), w.h, t);
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, need)) * (uint32_t)box * 128u;
+#pragma unroll
+                for (int v = 0; v < 2; ++v, ++item) {
+                    const uint32_t slot = item % kStages;
+                    if (item >= kStages && !warp_wait(&sh.empty[slot], (item / kStages - 1) & 1, status)) {
+                        ok = false;
+                        break;
+                    }
+                    // V of an edge tile goes to the fixing warps, which then publish it
+                    uint64_t *bar = v && tile_edge(a, k, T) ? &sh.edge[ne++ & 3] : &sh.full[slot];
+                    if (lane == 0) bar_expect(bar, bytes);
+                    __syncwarp();
+                    if (need)
+                        copy_box(ring + slot * (NP * kPanel) + panel * kPanel + piece * box * 128, v ? &vmap : &kmap,
+                                 64 * panel, y, bar);
+                }
+            }
+            if (ok) more = walk_next(a, TB, w, s);
+        }
+        // no copy outlives the CTA
+        for (int i = 0; i < kStages && (uint32_t)i < item; ++i) {
+            const uint32_t it = item - 1 - i;
+            warp_wait(&sh.full[it % kStages], (it / kStages) & 1, status);
+        }
+    } else {
+        // ------------------------------------------------------------ V rows of edge tiles
+        uint32_t item = 0, ne = 0;
+        while (more && ok) {
+            const Seg s = seg_of(a, w);
+            const Block &k = w.k;
+            for (int j = 0; ok && j < s.t1 - s.t0; ++j, item += 2) {
+                const int T = tile_token(k, s.t0 + j);
+                if (!tile_edge(a, k, T)) continue;
+                const uint32_t slot = (item + 1) % kStages;
+                if (!warp_wait(&sh.edge[ne & 3], (ne >> 2) & 1, status)) {
+                    ok = false;
+                    break;
+                }
+                unsigned char *v = ring + slot * (NP * kPanel);
+#pragma unroll
+                for (int h2 = 0; h2 < 2; ++h2) {
+                    const int r = 64 * (warp - kFixWarp) + 32 * h2 + lane;
+                    const bool seen = token_seen(a, k, T + r);
+                    bool bad = false;
+                    for (int c = 0; c < D / 8; ++c) {
+                        uint4 *q = reinterpret_cast<uint4 *>(v + (c >> 3) * kPanel + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                        if (!seen) {
+                            *q = make_uint4(0, 0, 0, 0);
+                            continue;
+                        }
+                        uint4 x = *q;
+                        uint32_t *e = reinterpret_cast<uint32_t *>(&x);
+                        bool hit = false;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            constexpr uint32_t ex = F16 ? 0x7c00u : 0x7f80u; // all exponent bits: not finite
+                            if ((e[i] & ex) == ex) e[i] &= 0xffff0000u, hit = true;
+                            if ((e[i] >> 16 & ex) == ex) e[i] &= 0x0000ffffu, hit = true;
+                        }
+                        if (hit) *q = x, bad = true;
+                    }
+                    const uint32_t bits = __ballot_sync(0xffffffffu, bad);
+                    if (lane == 0) sh.flags[ne & 3][2 * (warp - kFixWarp) + h2] = bits;
+                }
+                proxy_fence();
+                __syncwarp();
+                if (warp != kFixWarp) {
+                    if (lane == 0) bar_arrive(&sh.half[ne & 3]);
+                } else {
+                    ok = warp_wait(&sh.half[ne & 3], (ne >> 2) & 1, status);
+                    if (ok && lane == 0) bar_arrive(&sh.full[slot]);
+                }
+                ++ne;
+            }
+            if (ok) more = walk_next(a, TB, w, s);
+        }
+    }
+    tc_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(kTmemCols) : "memory");
+    }
+}
+
+template <int NP, bool F16> cudaError_t launch_chunk(const PagesAttn &a, int sms, cudaStream_t s) {
+    static bool configured[64] = {false};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        e = cudaFuncSetAttribute(pages_chunk_kernel<NP, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(NP));
+        if (e != cudaSuccess) return e;
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+    int *counters = reinterpret_cast<int *>(a.part + a.part_floats) - kPagesCounters;
+    const int TB = 2 * kRows / a.G;
+    return launch_pdl(pages_chunk_kernel<NP, F16>, dim3((unsigned)sms), dim3(kThreads), smem_bytes(NP), s, true, a, TB, 2,
+                      counters, a.maps->k, a.maps->v);
+}
+
+} // namespace
+
+// Blocks of at least one token: up to 256 query heads per kv head.  The batch's
+// prefix lies in shared memory while the list is built.
+bool pages_chunk_supported(const PagesAttn &a) { return a.st.bits == 16 && a.G <= 2 * kRows && a.b.batch <= 16384; }
+
+int64_t pages_chunk_scratch(int D, int sms) { return (int64_t)sms * 2 * (2 * kRows) * (D + 4); }
+
+cudaError_t launch_pages_chunk(const PagesAttn &a, cudaStream_t s) {
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return e;
+    if (sms > kPagesCounters || pages_chunk_scratch(a.st.D, sms) > a.part_floats - kPagesCounters)
+        return cudaErrorInvalidConfiguration;
+    ProfScope prof("pages_chunk", s);
+    count_launch();
+    const bool f16 = a.dtype == kF16;
+    if (a.st.D > 64) return f16 ? launch_chunk<2, true>(a, sms, s) : launch_chunk<2, false>(a, sms, s);
+    return f16 ? launch_chunk<1, true>(a, sms, s) : launch_chunk<1, false>(a, sms, s);
+}
+
+// Tensor maps over 16-bit pages: rows of D elements, boxes of one page's tokens
+// (at most a tile's) x 64 channels, 128-byte swizzle, zeros past the last channel.
+cudaError_t pages_tensor_maps(const PagesStore &st, PagesMaps *maps) {
+    static PFN_cuTensorMapEncodeTiled encode = nullptr;
+    if (!encode) {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found);
+        if (e != cudaSuccess) return e;
+        if (found != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
+        encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled>(fn);
+    }
+    const cuuint64_t dims[2] = {(cuuint64_t)st.D, (cuuint64_t)st.num_pages * st.H * st.page};
+    const cuuint64_t strides[1] = {(cuuint64_t)st.row_bytes};
+    const cuuint32_t box[2] = {64, (cuuint32_t)std::min(st.page, kTok)}, steps[2] = {1, 1};
+    const CUtensorMapDataType type = st.dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    for (int side = 0; side < 2; ++side) {
+        const CUresult r = encode(side ? &maps->v : &maps->k, type, 2, side ? st.v : st.k, dims, strides, box, steps,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) return cudaErrorInvalidValue;
+    }
+    return cudaSuccess;
+}
+
+} // namespace kivi

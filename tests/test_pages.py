@@ -292,6 +292,9 @@ CHUNK = [
     dict(new=[17, 300], kv=[2100, 400], group=1, dim=32, page=256, heads=3),
     dict(new=[4], kv=[9000], group=16, heads=1, page=64),
     dict(new=[6] * 9, kv=[150 * i + 6 for i in range(9)], group=5, heads=1, page=16),
+    dict(new=[400], kv=[3777], group=4, page=64),
+    dict(new=[90, 260], kv=[2600, 1311], group=6, heads=3, dim=64, page=16),
+    dict(new=[1100], kv=[1100], group=1, heads=1, page=256),
 ]
 MASKS = [(1, 0), (1, 3), (17, 0), (64, 4), (100, 21), (128, 200), (5000, 4)]
 
@@ -305,7 +308,7 @@ def test_attention(env, i, bits, kind):
 
 @pytest.mark.parametrize("bits,kind", [(16, "bf16"), (8, "f16"), (4, "bf16")])
 @pytest.mark.parametrize("window,sinks", MASKS)
-@pytest.mark.parametrize("i", [2, 3, 6, 9, 10, 13])
+@pytest.mark.parametrize("i", [2, 3, 6, 9, 10, 13, 16, 17, 18])
 def test_window_and_first_tokens(env, i, window, sinks, bits, kind):
     c = Case(env, bits=bits, kind=kind, seed=50 + i, **(DECODE + CHUNK)[i])
     c.check(c.queries(), 1.0 / math.sqrt(c.dim), window, sinks)
