@@ -51,7 +51,6 @@ constexpr int kStages = 5;                // K and V tiles in flight
 constexpr int kPanel = 16384;             // 128 rows x 64 channels
 constexpr long long kWait = 2000000000LL; // ~1 s
 constexpr float kLazy = 8.0f;
-constexpr int kSoftRegs = 200, kRoleRegs = 96;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0, kColO = 256; // + 128 for B
 
@@ -93,8 +92,6 @@ __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::befor
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// The 256 softmax threads (every other warp may be elsewhere).
-__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // Shared-memory matrix descriptor, 128-byte swizzle (layout 2), version 1.
 // K-major: sbo = 1024 between groups of 8 rows.  MN-major: sbo = 1024 between
@@ -151,6 +148,27 @@ __device__ __forceinline__ void copy_box(void *dst, const CUtensorMap *map, int 
                  : "memory");
 }
 
+// 16 consecutive 32-bit columns of this thread's tensor-memory lane.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float *v) {
+    uint32_t r[16];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+                 "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr)
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {"
+                 "%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                 "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
 // 64 consecutive 32-bit columns of this thread's tensor-memory lane.
 __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float *v) {
     uint32_t r[64];
@@ -264,38 +282,47 @@ __device__ __forceinline__ Block make_block(const PagesAttn &a, int TB, int b, c
 }
 __device__ __forceinline__ int blocks_of(int n, int TB) { return (n + TB - 1) / TB; }
 
-// A CTA's run of the list, walked the same way by every role.
+// A CTA's run of the list, walked by its copy warp.
 struct Walk {
     long long f, end, row0; // tiles of the flat list; first tile of the current (block, head)
     int i, h;               // block of the sequence, head
     Block k;
 };
-// One (block, head)'s part in this CTA: tiles t0 .. t1 - 1 of its nt.
+// One (block, head)'s part in a CTA, as the copy warp publishes it to the others.
 struct Seg {
-    int t0, t1;
-    int rows;     // query rows
-    bool dual;    // one row tile: A takes even tiles, B odd ones
-    int nA, nB;   // tiles of each
+    Block k;
+    int t0, n;          // its tiles t0 .. t0 + n - 1; n == 0 ends the run
+    int h, rows;        // kv head, query rows
+    int dual;           // one row tile: A takes even tiles, B odd ones
+    int nA, nB;         // tiles of each
+    int whole, c0, c1;  // no other CTA has a part; else the CTAs that do
+    int part;           // this CTA's part among the parts of all
 };
-__device__ __forceinline__ Seg seg_of(const PagesAttn &a, const Walk &w) {
-    Seg s;
+__device__ __forceinline__ void make_seg(const PagesAttn &a, const Walk &w, long long begin, long long per, Seg &s) {
+    s.k = w.k;
     s.t0 = (int)(w.f - w.row0);
-    s.t1 = (int)min((long long)w.k.nt, w.end - w.row0);
-    const int n = s.t1 - s.t0;
+    s.n = (int)min((long long)w.k.nt, w.end - w.row0) - s.t0;
+    s.h = w.h;
     s.rows = w.k.ntok * a.G;
     s.dual = s.rows <= kRows;
     if (s.dual) {
-        s.nA = (n + 1) / 2, s.nB = n / 2;
+        s.nA = (s.n + 1) / 2, s.nB = s.n / 2;
     } else {
         // A's last row sees no tile past its own
         const int pA = w.k.p0 + (kRows - 1) / a.G;
         const int tA = max(1, w.k.ns + max(0, (pA >= 0 ? pA / kTok + 1 : 0) - w.k.ws));
-        s.nA = max(0, min(tA - s.t0, n)), s.nB = n;
+        s.nA = max(0, min(tA - s.t0, s.n)), s.nB = s.n;
     }
-    return s;
+    const bool first = w.row0 >= begin; // the (block, head) starts in this CTA
+    s.whole = first && w.row0 + w.k.nt <= begin + per;
+    s.c0 = s.c1 = s.part = 0;
+    if (!s.whole) {
+        s.c0 = (int)(w.row0 / per), s.c1 = (int)((w.row0 + w.k.nt - 1) / per);
+        s.part = 2 * blockIdx.x + (first ? 1 : 0);
+    }
 }
-__device__ __forceinline__ bool walk_next(const PagesAttn &a, int TB, Walk &w, const Seg &s) {
-    w.f = w.row0 + s.t1;
+__device__ __forceinline__ bool walk_next(const PagesAttn &a, int TB, Walk &w) {
+    w.f = w.row0 + w.k.nt;
     if (w.f >= w.end) return false;
     w.row0 = w.f;
     if (++w.h < a.st.H) return true;
@@ -322,33 +349,205 @@ __device__ __forceinline__ bool token_seen(const PagesAttn &a, const Block &k, i
     return t <= k.p1 && (t >= k.lo || t < a.sinks);
 }
 
+constexpr int kSegs = 4;     // segments published ahead
+constexpr int kReaders = 11; // warps that read them: all but the copy warp
 struct Shared {
     uint64_t full[kStages], empty[kStages];
+    uint64_t seg_full[kSegs], seg_empty[kSegs];
     uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
-    uint64_t edge[4], half[4], drain; // an edge tile's V has landed, before the fixing warps
+    uint64_t edge[4], half[4]; // an edge tile's V has landed, is half through
+    uint64_t meet;             // the softmax warps
+    uint64_t drain;
     uint32_t flags[4][4]; // tokens of an edge tile whose value row is not finite
     uint32_t tmem;
     int last;
     long long scan[kThreads / 32];
-    long long begin, per;
     Walk walk;
+    Seg seg[kSegs];
     float2 ml[kRows]; // B's (m, l) when it shares A's rows
 };
 
 static_assert(sizeof(Shared) + 1024 + 7 * 2 * kPanel <= 232448, "shared memory per block");
 constexpr int smem_bytes(int np) { return 2 * np * kPanel + kStages * np * kPanel + (int)sizeof(Shared) + 1024; }
 
-template <int NP, bool F16>
+// Rows of V that are not finite were taken out of an edge tile (flags, one bit
+// per token); they are added here to the rows that see them: p > 0, so p v is v.
+template <int ND, bool F16>
+__device__ __noinline__ void add_unfinite(const PagesAttn &a, const uint32_t *flags, int b, int h, int T, int p, int lo,
+                                          uint32_t cO) {
+    for (int f = 0; f < 4; ++f) {
+        uint32_t bits = flags[f];
+        while (bits) {
+            const int t = T + 32 * f + __ffs((int)bits) - 1;
+            bits &= bits - 1;
+            const bool see = t <= p && (t >= lo || t < a.sinks);
+            const int64_t r = pages_row(a.st, max(pages_page(a.b, a.st, b, t), 0), h, t);
+            const uint16_t *v = reinterpret_cast<const uint16_t *>(a.st.v + r * a.st.row_bytes);
+#pragma unroll 1
+            for (int c = 0; c < 32 * ND; c += 32) {
+                float o[32];
+                tmem_ld32(cO + c, o);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float y = unpack(F16, v[c + i]);
+                    if (see && !isfinite(y)) o[i] += y;
+                }
+                tmem_st32(cO + c, reinterpret_cast<const uint32_t *>(o));
+                st_wait();
+            }
+        }
+    }
+}
+
+// The last CTA of a (block, head) joins its parts, in CTA order: eight float4 of
+// the block a thread at a time, one step's loads independent of one another.
+template <int ND, bool F16> __device__ __noinline__ void join_parts(const PagesAttn &a, const Seg &s) {
+    constexpr int D = 32 * ND, D4 = D / 4, N = 8;
+    constexpr int64_t stride = D + 4;
+    const int G = a.G, n = s.rows * D4;
+    for (int i0 = threadIdx.x; i0 < n; i0 += 256 * N) {
+        float4 acc[N];
+        float mm[N], ll[N];
+#pragma unroll
+        for (int u = 0; u < N; ++u) acc[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), mm[u] = -INFINITY, ll[u] = 0.0f;
+        for (int x = s.c0; x <= s.c1; ++x) {
+            const float *px = a.part + ((int64_t)x * 2 + (x == s.c0 ? 1 : 0)) * (2 * kRows) * stride;
+            float4 y[N];
+            float2 ml[N];
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const int i = min(i0 + 256 * u, n - 1);
+                const float *pp = px + (i / D4) * stride;
+                y[u] = __ldcg(reinterpret_cast<const float4 *>(pp) + i % D4);
+                ml[u] = __ldcg(reinterpret_cast<const float2 *>(pp + D));
+            }
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const float nm = fmaxf(mm[u], ml[u].x), ref = nm == -INFINITY ? 0.0f : nm;
+                const float f0 = ex2(mm[u] - ref), f1 = ex2(ml[u].x - ref);
+                mm[u] = nm;
+                ll[u] = ll[u] * f0 + ml[u].y * f1;
+                acc[u].x = acc[u].x * f0 + y[u].x * f1, acc[u].y = acc[u].y * f0 + y[u].y * f1;
+                acc[u].z = acc[u].z * f0 + y[u].z * f1, acc[u].w = acc[u].w * f0 + y[u].w * f1;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int i = i0 + 256 * u;
+            if (i >= n) break;
+            const int r = i / D4, c = i % D4, tk = r / G, hd = r - tk * G;
+            const bool sees = s.k.p0 + tk >= 0;
+            const float inv = 1.0f / ll[u];
+            uint2 y = make_uint2(0, 0);
+            if (sees) y = make_uint2(pack2<F16>(acc[u].x * inv, acc[u].y * inv), pack2<F16>(acc[u].z * inv, acc[u].w * inv));
+            const int64_t otok = s.k.start + s.k.i0 + tk;
+            uint16_t *d = static_cast<uint16_t *>(a.out) + otok * a.o_token + (int64_t)(s.h * G + hd) * a.o_head + 4 * c;
+            if (a.o_vec) {
+                *reinterpret_cast<uint2 *>(d) = y;
+            } else {
+                d[0] = (uint16_t)y.x, d[1] = (uint16_t)(y.x >> 16), d[2] = (uint16_t)y.y, d[3] = (uint16_t)(y.y >> 16);
+            }
+            if (a.lse && c == 0)
+                a.lse[otok * a.Hq + s.h * G + hd] = sees ? mm[u] * 0.6931471805599453f + logf(ll[u]) : -INFINITY;
+        }
+    }
+}
+
+// This row's O, out: normalised to the output, or as a part.  A's threads add B's
+// O where B shared their rows.
+template <int ND, bool F16>
+__device__ __noinline__ void store_row(const PagesAttn &a, const Seg &s, uint32_t cO, int r, bool live, int tok, int head,
+                                       float m, float l, float fa, float fb) {
+    constexpr int D = 32 * ND;
+    const bool sees = live && s.k.p0 + tok >= 0;
+    const float inv = sees ? 1.0f / l : 0.0f;
+    const int64_t otok = s.k.start + s.k.i0 + tok;
+    uint16_t *out = static_cast<uint16_t *>(a.out) + otok * a.o_token + (int64_t)(s.h * a.G + head) * a.o_head;
+    float *part = a.part + ((int64_t)s.part * (2 * kRows) + r) * (D + 4);
+#pragma unroll
+    for (int c = 0; c < D; c += 32) {
+        float o[32];
+        tmem_ld32(cO + c, o);
+        if (s.dual) {
+            float o2[32];
+            tmem_ld32(cO + 128 + c, o2);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = o[i] * fa + o2[i] * fb;
+        }
+        // (no early exit: the tensor-memory loads are the whole warp's)
+        if (live && !s.whole) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<float4 *>(part + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        } else if (live) {
+            uint32_t y[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = sees ? pack2<F16>(o[2 * i] * inv, o[2 * i + 1] * inv) : 0u;
+            if (a.o_vec) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<uint4 *>(out + c + 8 * i) = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) out[c + i] = (uint16_t)(y[i / 2] >> (16 * (i & 1)));
+            }
+        }
+        __syncwarp();
+    }
+    if (live && !s.whole) {
+        part[D] = m;
+        part[D + 1] = l;
+    } else if (live && a.lse) {
+        a.lse[otok * a.Hq + s.h * a.G + head] = sees ? m * 0.6931471805599453f + logf(l) : -INFINITY;
+    }
+}
+
+// A thread's query row into its tile (128-byte swizzle); rows past the block are zeros.
+template <int ND>
+__device__ __noinline__ void load_query(const PagesAttn &a, const Seg &s, unsigned char *dst, int row, bool live, int tok,
+                                        int head) {
+    constexpr int D = 32 * ND;
+    const uint16_t *q = static_cast<const uint16_t *>(a.q) + (int64_t)(s.k.start + s.k.i0 + tok) * a.q_token +
+                        (int64_t)(s.h * a.G + head) * a.q_head;
+    uint4 v[D / 8]; // all of the row in flight
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) {
+        v[c] = make_uint4(0, 0, 0, 0);
+        if (live && a.q_vec) v[c] = __ldg(reinterpret_cast<const uint4 *>(q) + c);
+    }
+    if (live && !a.q_vec) {
+#pragma unroll 1
+        for (int c = 0; c < D / 8; ++c) {
+            uint32_t e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = q[8 * c + 2 * i] | (uint32_t)q[8 * c + 2 * i + 1] << 16;
+#pragma unroll
+            for (int k = 0; k < D / 8; ++k)
+                if (k == c) v[k] = make_uint4(e[0], e[1], e[2], e[3]);
+        }
+    }
+    const uint32_t flip = a.qsign < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c)
+        *reinterpret_cast<uint4 *>(dst + (c >> 3) * kPanel + (((c & 7) ^ (row & 7)) << 4)) =
+            make_uint4(v[c].x ^ flip, v[c].y ^ flip, v[c].z ^ flip, v[c].w ^ flip);
+}
+
+// n low bits set (n may lie outside 0 .. 32)
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+
+template <int ND, bool F16>
 __global__ void __launch_bounds__(kThreads, 1)
-    pages_chunk_kernel(const PagesAttn a, int TB, int min_per, int *counters, const __grid_constant__ CUtensorMap kmap,
+    pages_chunk_kernel(const __grid_constant__ PagesAttn a, int TB, int min_per, int *counters, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
+    constexpr int D = 32 * ND, NP = (ND + 1) / 2; // channels, 64-channel panels
     extern __shared__ unsigned char raw[];
     unsigned char *sm = raw + ((1024 - (su32(raw) & 1023)) & 1023);
     unsigned char *sq = sm, *ring = sm + 2 * NP * kPanel;
     Shared &sh = *reinterpret_cast<Shared *>(ring + kStages * NP * kPanel);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PagesStore &st = a.st;
-    const int H = st.H, G = a.G, D = st.D;
+    const int H = st.H, G = a.G;
     unsigned int *status = st.status;
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) bar_init(&sh.full[i], 1), bar_init(&sh.empty[i], 1);
@@ -358,7 +557,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             bar_init(&sh.p_full[x], 4);
             bar_init(&sh.o_full[x], 1);
         }
+        for (int i = 0; i < kSegs; ++i) bar_init(&sh.seg_full[i], 1), bar_init(&sh.seg_empty[i], kReaders);
         for (int i = 0; i < 4; ++i) bar_init(&sh.edge[i], 1), bar_init(&sh.half[i], 1);
+        bar_init(&sh.meet, kSoft);
         bar_init(&sh.drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -452,56 +653,51 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_after();
     const uint32_t tm = sh.tmem;
-    Walk w = sh.walk;
-    bool more = begin < end, ok = true;
+    // a role's segments, in order: s points at the next one, false at the end
+    uint32_t nseg = 0;
+    const Seg *sp = nullptr;
+    auto next_seg = [&]() {
+        if (nseg > 0) { // done with the last one
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.seg_empty[(nseg - 1) % kSegs]);
+        }
+        if (!warp_wait(&sh.seg_full[nseg % kSegs], (nseg / kSegs) & 1, status)) return false;
+        sp = &sh.seg[nseg % kSegs];
+        ++nseg;
+        return sp->n > 0;
+    };
+    bool ok = true;
 
-    // registers: 384 x 168 at launch = 256 x kSoftRegs + 128 x kRoleRegs and a rest
-    static_assert(256 * kSoftRegs + 128 * kRoleRegs <= kThreads * 168, "register split");
-    if (warp < kSoft)
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
-    else
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
     if (warp < kSoft) {
         // ------------------------------------------------------------ softmax
-        const int X = warp >> 2;             // A or B
-        const int row = tid & 127;           // tensor-memory lane
+        const int X = warp >> 2;   // A or B
+        const int row = tid & 127; // tensor-memory lane
         const uint32_t lanes = tm + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t cS = lanes + kColS + 128 * X, cO = lanes + kColO + 128 * X;
         const float crow = a.scale * 1.4426950408889634f;
-        uint32_t ns = 0, no = 0, ne = 0, item = 0; // tiles, blocks, edge tiles and copies so far
-        while (more) {
-            const Seg s = seg_of(a, w);
-            const Block &k = w.k;
+        uint32_t ns = 0, no = 0, ne = 0, item = 0, met = 0; // tiles, blocks, edge tiles, copies, meetings so far
+        auto meet = [&]() { // of the softmax warps
+            tc_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.meet);
+            const bool r = warp_wait(&sh.meet, met++ & 1, status);
+            tc_after();
+            return r;
+        };
+        while (ok && next_seg()) {
+            const Seg &s = *sp;
+            const bool dual = s.dual;
             const int nX = X ? s.nB : s.nA;
-            const int r0 = X && !s.dual ? kRows : 0;
+            const int r0 = X && !dual ? kRows : 0;
             const bool live = r0 + row < s.rows;
             const int tok = live ? (r0 + row) / G : 0, head = live ? r0 + row - tok * G : 0;
-            const int p = live ? k.p0 + tok : -1;
+            const int p = live ? s.k.p0 + tok : -1;
             const int lo = a.window ? max(0, p - a.window + 1) : 0;
             const bool any = __any_sync(0xffffffffu, live);
             float m = -INFINITY, l = 0.0f;
             if (r0 < s.rows) {
                 // ---- the row's query, and an empty O
-                if (!(X && s.dual)) {
-                    const uint16_t *q = static_cast<const uint16_t *>(a.q) + (int64_t)(k.start + k.i0 + tok) * a.q_token +
-                                        (int64_t)(w.h * G + head) * a.q_head;
-                    unsigned char *dst = sq + X * NP * kPanel + row * 128;
-                    for (int c = 0; c < D / 8; ++c) {
-                        uint4 v = make_uint4(0, 0, 0, 0);
-                        if (live) {
-                            if (a.q_vec) {
-                                v = __ldg(reinterpret_cast<const uint4 *>(q) + c);
-                            } else {
-                                uint32_t e[4];
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) e[i] = q[8 * c + 2 * i] | (uint32_t)q[8 * c + 2 * i + 1] << 16;
-                                v = make_uint4(e[0], e[1], e[2], e[3]);
-                            }
-                            if (a.qsign < 0.0f) v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
-                        }
-                        *reinterpret_cast<uint4 *>(dst + (c >> 3) * kPanel + (((c & 7) ^ (row & 7)) << 4)) = v;
-                    }
-                }
+                if (!(X && dual)) load_query<ND>(a, s, sq + X * NP * kPanel + row * 128, row, live, tok, head);
                 {
                     uint32_t z[32] = {};
                     for (int c = 0; c < D; c += 32) tmem_st32(cO + c, z);
@@ -512,16 +708,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.q_full[X]);
             }
-            for (int j = 0; ok && j < (s.dual ? s.t1 - s.t0 : nX); ++j) {
-                const int T = tile_token(k, s.t0 + j);
-                const bool edge = tile_edge(a, k, T);
+            const int n = dual ? s.n : nX;
+            for (int j = 0; j < n; ++j) {
+                const int T = tile_token(s.k, s.t0 + j);
+                const bool edge = tile_edge(a, s.k, T);
                 const uint32_t e = ne;
                 if (edge) ++ne;
-                if (s.dual && (j & 1) != X) continue;
-                if (!warp_wait(&sh.s_full[X], ns & 1, status)) {
-                    ok = false;
-                    break;
-                }
+                if (dual && (j & 1) != X) continue;
+                if (!(ok = warp_wait(&sh.s_full[X], ns & 1, status))) break;
                 ++ns;
                 tc_after();
                 if (any) {
@@ -529,10 +723,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_ld64(cS, x);
                     tmem_ld64(cS + 64, x + 64);
                     if (edge) {
-                        const int hi = p - T, lw = lo - T, sk = a.sinks - T;
 #pragma unroll
-                        for (int i = 0; i < 128; ++i)
-                            if (i > hi || (i < lw && i >= sk)) x[i] = -INFINITY;
+                        for (int q = 0; q < 4; ++q) {
+                            const int base = T + 32 * q;
+                            const uint32_t see = low_bits(p + 1 - base) & (~low_bits(lo - base) | low_bits(a.sinks - base));
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                x[32 * q + i] = see >> i & 1u ? x[32 * q + i] : -INFINITY;
+                        }
                     }
                     float m4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
@@ -549,12 +747,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (__any_sync(0xffffffffu, move)) {
                         l *= f;
                         // every O += P V of earlier tiles is complete: S of this one was issued after them
-                        for (int c = 0; c < D; c += 32) {
-                            float o[32];
-                            tmem_ld32(cO + c, o);
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {
+                            float o[16];
+                            tmem_ld16(cO + c, o);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] *= f;
-                            tmem_st32(cO + c, reinterpret_cast<const uint32_t *>(o));
+                            for (int i = 0; i < 16; ++i) o[i] *= f;
+                            tmem_st16(cO + c, reinterpret_cast<const uint32_t *>(o));
                         }
                     }
                     const float off = m == -INFINITY ? 0.0f : -m;
@@ -578,57 +777,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     l += (a0 + a1) + (a2 + a3);
                 }
-                if (edge) {
-                    // value rows with infinities or NaN: taken out of the tile, added here to
-                    // the rows that see them (p > 0, so p v is v)
+                if (edge) { // the tile's V has been through the fixing warps
                     const uint32_t it = item + 2 * j + 1;
-                    if (!warp_wait(&sh.full[it % kStages], (it / kStages) & 1, status)) {
-                        ok = false;
-                        break;
-                    }
-                    for (int f4 = 0; f4 < 4; ++f4) {
-                        uint32_t bits = sh.flags[e & 3][f4];
-                        while (bits) {
-                            const int t = T + 32 * f4 + __ffs((int)bits) - 1;
-                            bits &= bits - 1;
-                            const bool see = t <= p && (t >= lo || t < a.sinks);
-                            const int64_t r = pages_row(st, max(pages_page(a.b, st, k.b, t), 0), w.h, t);
-                            const uint16_t *v = reinterpret_cast<const uint16_t *>(st.v + r * st.row_bytes);
-                            for (int c = 0; c < D; c += 32) {
-                                float o[32];
-                                tmem_ld32(cO + c, o);
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) {
-                                    const float y = unpack(F16, v[c + i]);
-                                    if (see && !isfinite(y)) o[i] += y;
-                                }
-                                tmem_st32(cO + c, reinterpret_cast<const uint32_t *>(o));
-                                st_wait();
-                            }
-                        }
-                    }
+                    if (!(ok = warp_wait(&sh.full[it % kStages], (it / kStages) & 1, status))) break;
+                    const uint32_t *fl = sh.flags[e & 3];
+                    if (fl[0] | fl[1] | fl[2] | fl[3]) add_unfinite<ND, F16>(a, fl, s.k.b, s.h, T, p, lo, cO);
                 }
                 st_wait();
                 tc_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.p_full[X]);
             }
-            for (int j = nX; !s.dual && j < s.t1 - s.t0; ++j) ne += tile_edge(a, k, tile_token(k, s.t0 + j));
-            item += 2 * (s.t1 - s.t0);
+            for (int j = nX; !dual && j < s.n; ++j) ne += tile_edge(a, s.k, tile_token(s.k, s.t0 + j));
+            item += 2 * s.n;
             // ---- the rows out
-            if (ok && nX > 0) {
-                if (warp_wait(&sh.o_full[X], no & 1, status)) ++no;
-                else ok = false;
-                tc_after();
-            }
-            const int c0 = (int)(w.row0 / per), c1 = (int)((w.row0 + k.nt - 1) / per);
-            const bool whole = c0 == c1;
+            if (ok && nX > 0) ok = warp_wait(&sh.o_full[X], no++ & 1, status);
+            tc_after();
             float fa = 1.0f, fb = 0.0f;
-            if (s.dual) {
+            if (dual) {
                 if (X) sh.ml[row] = make_float2(m, l);
-                tc_before();
-                soft_sync();
-                tc_after();
+                if (!(ok = ok && meet())) break;
                 if (!X) {
                     const float2 y = sh.ml[row];
                     const float nm = fmaxf(m, y.x), ref = nm == -INFINITY ? 0.0f : nm;
@@ -637,101 +805,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                     l = l * fa + y.y * fb;
                 }
             }
-            const int64_t stride = D + 4;
-            float *part = a.part + ((int64_t)blockIdx.x * 2 + (c0 == (int)blockIdx.x ? 1 : 0)) * (2 * kRows) * stride +
-                          (r0 + row) * stride;
-            if (any && !(X && s.dual)) {
-                const bool sees = p >= 0;
-                const float inv = sees ? 1.0f / l : 0.0f;
-                const int64_t otok = k.start + k.i0 + tok;
-                uint16_t *out = static_cast<uint16_t *>(a.out) + otok * a.o_token + (int64_t)(w.h * G + head) * a.o_head;
-                for (int c = 0; c < D; c += 32) {
-                    float o[32];
-                    tmem_ld32(cO + c, o);
-                    if (s.dual) {
-                        float o2[32];
-                        tmem_ld32(cO + 128 + c, o2);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = o[i] * fa + o2[i] * fb;
-                    }
-                    uint32_t y[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        y[i] = sees ? pack2<F16>(o[2 * i] * inv, o[2 * i + 1] * inv) : 0u;
-                    // (no early exit: the tensor-memory loads are the whole warp's)
-                    if (live && !whole) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<float4 *>(part + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                    } else if (live && a.o_vec) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            *reinterpret_cast<uint4 *>(out + c + 8 * i) = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-                    } else if (live) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) out[c + i] = (uint16_t)(y[i / 2] >> (16 * (i & 1)));
-                    }
-                    __syncwarp();
-                }
-                if (live && whole && a.lse)
-                    a.lse[otok * a.Hq + w.h * G + head] = sees ? m * 0.6931471805599453f + logf(l) : -INFINITY;
-                if (live && !whole) {
-                    part[D] = m;
-                    part[D + 1] = l;
-                }
-            }
-            if (!whole) {
-                // ---- the last CTA of the (block, head) joins its parts
+            if (!ok) break;
+            if (any && !(X && dual)) store_row<ND, F16>(a, s, cO, r0 + row, live, tok, head, m, l, fa, fb);
+            if (!s.whole) {
                 __threadfence();
-                soft_sync();
+                if (!(ok = meet())) break;
                 if (tid == 0) {
-                    sh.last = atomicAdd(counters + c0, 1) == c1 - c0;
-                    if (sh.last) counters[c0] = 0; // for the next call
+                    const int done = atomicAdd(counters + s.c0, 1) == s.c1 - s.c0;
+                    if (done) counters[s.c0] = 0; // for the next call
+                    sh.last = done;
                 }
-                soft_sync();
+                if (!(ok = meet())) break;
                 if (sh.last) {
                     __threadfence();
-                    const int D4 = D / 4;
-                    for (int i = tid; i < s.rows * D4; i += 256) {
-                        const int r = i / D4, c = i - r * D4;
-                        const int tk = r / G, hd = r - tk * G;
-                        float mm = -INFINITY, ll = 0.0f;
-                        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        for (int x = c0; x <= c1; ++x) {
-                            const float *pp = a.part + (((int64_t)x * 2 + (x == c0 ? 1 : 0)) * (2 * kRows) + r) * stride;
-                            const float4 y = __ldcg(reinterpret_cast<const float4 *>(pp) + c);
-                            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(pp + D));
-                            const float nm = fmaxf(mm, ml.x), ref = nm == -INFINITY ? 0.0f : nm;
-                            const float f0 = ex2(mm - ref), f1 = ex2(ml.x - ref);
-                            mm = nm;
-                            ll = ll * f0 + ml.y * f1;
-                            acc.x = acc.x * f0 + y.x * f1, acc.y = acc.y * f0 + y.y * f1;
-                            acc.z = acc.z * f0 + y.z * f1, acc.w = acc.w * f0 + y.w * f1;
-                        }
-                        const bool sees = k.p0 + tk >= 0;
-                        const float inv = 1.0f / ll;
-                        uint2 y = make_uint2(0, 0);
-                        if (sees) y = make_uint2(pack2<F16>(acc.x * inv, acc.y * inv), pack2<F16>(acc.z * inv, acc.w * inv));
-                        const int64_t otok = k.start + k.i0 + tk;
-                        uint16_t *d = static_cast<uint16_t *>(a.out) + otok * a.o_token + (int64_t)(w.h * G + hd) * a.o_head + 4 * c;
-                        if (a.o_vec) {
-                            *reinterpret_cast<uint2 *>(d) = y;
-                        } else {
-                            d[0] = (uint16_t)y.x, d[1] = (uint16_t)(y.x >> 16), d[2] = (uint16_t)y.y, d[3] = (uint16_t)(y.y >> 16);
-                        }
-                        if (a.lse && c == 0)
-                            a.lse[otok * a.Hq + w.h * G + hd] = sees ? mm * 0.6931471805599453f + logf(ll) : -INFINITY;
-                    }
+                    join_parts<ND, F16>(a, s);
                 }
             }
-            if (s.dual) { // B's O and (m, l) are read
-                tc_before();
-                soft_sync();
-                tc_after();
-            }
-            // after a wait that gave up the walk goes on without waiting, so that the
-            // 256 threads still meet at their barriers
-            more = walk_next(a, TB, w, s);
+            if (dual && !(ok = meet())) break; // B's O and (m, l) are read
         }
     } else if (warp == kMmaWarp) {
         // ------------------------------------------------------------ MMA issue
@@ -739,91 +829,93 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t dq = sdesc(su32(sq), 16, 1024), dr = sdesc(su32(ring), 16, 1024),
                        dv = sdesc(su32(ring), kPanel, 1024);
         uint32_t np[2] = {0, 0}, nq[2] = {0, 0}, item = 0;
-        while (more && ok) {
-            const Seg s = seg_of(a, w);
-            const int n = s.t1 - s.t0;
+        while (ok && next_seg()) {
+            const Seg &s = *sp;
+            const int dual = s.dual, nA = s.nA, nB = s.nB;
             // tile (of the segment) that X takes as its i-th
-            auto tile = [&](int X, int i) { return s.dual ? 2 * i + X : i; };
+            auto tile = [&](int X, int i) { return dual ? 2 * i + X : i; };
             // this use of a tile is its last
-            auto frees = [&](int X, int t) { return s.dual || X == 1 || t >= s.nB; };
+            auto frees = [&](int X) { return dual || X == 1; };
             auto qk = [&](int X, int i) {
-                const int t = tile(X, i);
-                const uint32_t it = item + 2 * t, slot = it % kStages;
+                const uint32_t it = item + 2 * tile(X, i), slot = it % kStages;
                 if (i == 0 && !warp_wait(&sh.q_full[X], nq[X]++ & 1, status)) return false;
                 if (!warp_wait(&sh.full[slot], (it / kStages) & 1, status)) return false;
                 tc_after();
                 const uint32_t d = tm + kColS + 128 * X;
-                const uint64_t q = dq + (uint64_t)(s.dual ? 0 : X) * (NP * kPanel / 16);
+                const uint64_t q = dq + (uint64_t)(dual ? 0 : X) * (NP * kPanel / 16);
                 const uint64_t b = dr + (uint64_t)slot * (NP * kPanel / 16);
-                if (D == 32) {
+                if constexpr (D == 32) {
                     mma_ss<2>(d, q, b, id_qk, 0u);
                 } else {
                     mma_ss<4>(d, q, b, id_qk, 0u);
-                    if (D == 96) mma_ss<2>(d, q + kPanel / 16, b + kPanel / 16, id_qk, 1u);
-                    if (D == 128) mma_ss<4>(d, q + kPanel / 16, b + kPanel / 16, id_qk, 1u);
+                    if constexpr (D == 96) mma_ss<2>(d, q + kPanel / 16, b + kPanel / 16, id_qk, 1u);
+                    if constexpr (D == 128) mma_ss<4>(d, q + kPanel / 16, b + kPanel / 16, id_qk, 1u);
                 }
                 mma_commit(&sh.s_full[X]);
-                if (frees(X, t)) mma_commit(&sh.empty[slot]);
+                if (frees(X)) mma_commit(&sh.empty[slot]);
                 return true;
             };
             auto pv = [&](int X, int i) {
-                const int t = tile(X, i);
-                const uint32_t it = item + 2 * t + 1, slot = it % kStages;
+                const uint32_t it = item + 2 * tile(X, i) + 1, slot = it % kStages;
                 if (!warp_wait(&sh.full[slot], (it / kStages) & 1, status)) return false;
-                if (!warp_wait(&sh.p_full[X], np[X] & 1, status)) return false;
-                ++np[X];
+                if (!warp_wait(&sh.p_full[X], np[X]++ & 1, status)) return false;
                 tc_after();
                 mma_pv(tm + kColO + 128 * X, tm + kColS + 128 * X, dv + (uint64_t)slot * (NP * kPanel / 16), id_pv);
-                if (frees(X, t)) mma_commit(&sh.empty[slot]);
-                if (i + 1 == (X ? s.nB : s.nA)) mma_commit(&sh.o_full[X]);
+                if (frees(X)) mma_commit(&sh.empty[slot]);
+                if (i + 1 == (X ? nB : nA)) mma_commit(&sh.o_full[X]);
                 return true;
             };
-            // rows without a tile in this run still load their queries
-            if (s.nA > 0) ok = qk(0, 0);
-            else if (!s.dual) ok = warp_wait(&sh.q_full[0], nq[0]++ & 1, status);
-            if (ok && s.nB > 0) ok = qk(1, 0);
-            else if (ok && s.dual) ok = warp_wait(&sh.q_full[1], nq[1]++ & 1, status);
-            for (int i = 0; ok && i < max(s.nA, s.nB); ++i) {
-                if (i < s.nA) ok = pv(0, i) && (i + 1 >= s.nA || qk(0, i + 1));
-                if (ok && i < s.nB) ok = pv(1, i) && (i + 1 >= s.nB || qk(1, i + 1));
+            // row tiles without a cached tile in this run report their queries all the same
+            ok = nA > 0 ? qk(0, 0) : warp_wait(&sh.q_full[0], nq[0]++ & 1, status);
+            if (ok) ok = nB > 0 ? qk(1, 0) : warp_wait(&sh.q_full[1], nq[1]++ & 1, status);
+            for (int i = 0; ok && i < max(nA, nB); ++i) {
+                if (i < nA) ok = pv(0, i) && (i + 1 >= nA || qk(0, i + 1));
+                if (ok && i < nB) ok = pv(1, i) && (i + 1 >= nB || qk(1, i + 1));
             }
-            item += 2 * n;
-            if (ok) more = walk_next(a, TB, w, s);
+            item += 2 * s.n;
         }
         mma_commit(&sh.drain); // tensor memory outlives every MMA
         warp_wait(&sh.drain, 0, status);
     } else if (warp == kCopyWarp) {
-        // ------------------------------------------------------------ copies
+        // ------------------------------------------------------------ segments and copies
+        Walk w = sh.walk;
+        bool more = begin < end;
         const int box = min(st.page, kTok), pieces = kTok / box;
         const int piece = lane / NP, panel = lane - piece * NP; // of the lane's box; pieces * NP <= 16
         uint32_t item = 0, ne = 0;
-        while (more && ok) {
-            const Seg s = seg_of(a, w);
+        for (; ok; ++nseg) {
+            const uint32_t slot = nseg % kSegs;
+            if (nseg >= kSegs && !(ok = warp_wait(&sh.seg_empty[slot], (nseg / kSegs - 1) & 1, status))) break;
+            Seg s;
+            s.n = 0;
+            if (more) make_seg(a, w, begin, per, s);
+            if (lane == 0) {
+                sh.seg[slot] = s;
+                bar_arrive(&sh.seg_full[slot]);
+            }
+            if (!more) break;
             const Block &k = w.k;
-            for (int j = 0; ok && j < s.t1 - s.t0; ++j) {
+            for (int j = 0; ok && j < s.n; ++j) {
                 const int T = tile_token(k, s.t0 + j), t = T + piece * box;
                 // a box is needed if some row sees one of its tokens
-                bool need = piece < pieces && t <= k.p1 && (t + box > k.lo || t < a.sinks);
+                const bool need = piece < pieces && t <= k.p1 && (t + box > k.lo || t < a.sinks);
                 int y = 0;
                 if (need) y = (int)pages_row(st, max(pages_page(a.b, st, k.b, t), 0), w.h, t);
                 const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, need)) * (uint32_t)box * 128u;
 #pragma unroll
                 for (int v = 0; v < 2; ++v, ++item) {
-                    const uint32_t slot = item % kStages;
-                    if (item >= kStages && !warp_wait(&sh.empty[slot], (item / kStages - 1) & 1, status)) {
-                        ok = false;
-                        break;
-                    }
+                    const uint32_t sl = item % kStages;
+                    if (item >= kStages && !(ok = warp_wait(&sh.empty[sl], (item / kStages - 1) & 1, status))) break;
                     // V of an edge tile goes to the fixing warps, which then publish it
-                    uint64_t *bar = v && tile_edge(a, k, T) ? &sh.edge[ne++ & 3] : &sh.full[slot];
+                    uint64_t *bar = v && tile_edge(a, k, T) ? &sh.edge[ne++ & 3] : &sh.full[sl];
                     if (lane == 0) bar_expect(bar, bytes);
                     __syncwarp();
                     if (need)
-                        copy_box(ring + slot * (NP * kPanel) + panel * kPanel + piece * box * 128, v ? &vmap : &kmap,
-                                 64 * panel, y, bar);
+                        copy_box(ring + sl * (NP * kPanel) + panel * kPanel + piece * box * 128, v ? &vmap : &kmap, 64 * panel, y,
+                                 bar);
                 }
             }
-            if (ok) more = walk_next(a, TB, w, s);
+            if (ok) more = walk_next(a, TB, w);
         }
         // no copy outlives the CTA
         for (int i = 0; i < kStages && (uint32_t)i < item; ++i) {
@@ -833,39 +925,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         // ------------------------------------------------------------ V rows of edge tiles
         uint32_t item = 0, ne = 0;
-        while (more && ok) {
-            const Seg s = seg_of(a, w);
-            const Block &k = w.k;
-            for (int j = 0; ok && j < s.t1 - s.t0; ++j, item += 2) {
-                const int T = tile_token(k, s.t0 + j);
-                if (!tile_edge(a, k, T)) continue;
+        while (ok && next_seg()) {
+            const Seg &s = *sp;
+            for (int j = 0; ok && j < s.n; ++j, item += 2) {
+                const int T = tile_token(s.k, s.t0 + j);
+                if (!tile_edge(a, s.k, T)) continue;
                 const uint32_t slot = (item + 1) % kStages;
-                if (!warp_wait(&sh.edge[ne & 3], (ne >> 2) & 1, status)) {
-                    ok = false;
-                    break;
-                }
+                if (!(ok = warp_wait(&sh.edge[ne & 3], (ne >> 2) & 1, status))) break;
                 unsigned char *v = ring + slot * (NP * kPanel);
-#pragma unroll
+#pragma unroll 1
                 for (int h2 = 0; h2 < 2; ++h2) {
                     const int r = 64 * (warp - kFixWarp) + 32 * h2 + lane;
-                    const bool seen = token_seen(a, k, T + r);
+                    const bool seen = token_seen(a, s.k, T + r);
                     bool bad = false;
+#pragma unroll 4
                     for (int c = 0; c < D / 8; ++c) {
                         uint4 *q = reinterpret_cast<uint4 *>(v + (c >> 3) * kPanel + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-                        if (!seen) {
-                            *q = make_uint4(0, 0, 0, 0);
-                            continue;
-                        }
                         uint4 x = *q;
                         uint32_t *e = reinterpret_cast<uint32_t *>(&x);
-                        bool hit = false;
+                        bool hit = !seen;
+                        if (!seen) x = make_uint4(0, 0, 0, 0);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             constexpr uint32_t ex = F16 ? 0x7c00u : 0x7f80u; // all exponent bits: not finite
-                            if ((e[i] & ex) == ex) e[i] &= 0xffff0000u, hit = true;
-                            if ((e[i] >> 16 & ex) == ex) e[i] &= 0x0000ffffu, hit = true;
+                            if ((e[i] & ex) == ex) e[i] &= 0xffff0000u, hit = bad = true;
+                            if ((e[i] >> 16 & ex) == ex) e[i] &= 0x0000ffffu, hit = bad = true;
                         }
-                        if (hit) *q = x, bad = true;
+                        if (hit) *q = x;
                     }
                     const uint32_t bits = __ballot_sync(0xffffffffu, bad);
                     if (lane == 0) sh.flags[ne & 3][2 * (warp - kFixWarp) + h2] = bits;
@@ -880,7 +966,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 ++ne;
             }
-            if (ok) more = walk_next(a, TB, w, s);
         }
     }
     tc_before();
@@ -891,19 +976,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-template <int NP, bool F16> cudaError_t launch_chunk(const PagesAttn &a, int sms, cudaStream_t s) {
+template <int ND, bool F16> cudaError_t launch_chunk(const PagesAttn &a, int sms, cudaStream_t s) {
     static bool configured[64] = {false};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-        e = cudaFuncSetAttribute(pages_chunk_kernel<NP, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(NP));
+        e = cudaFuncSetAttribute(pages_chunk_kernel<ND, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes((ND + 1) / 2));
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
     int *counters = reinterpret_cast<int *>(a.part + a.part_floats) - kPagesCounters;
     const int TB = 2 * kRows / a.G;
-    return launch_pdl(pages_chunk_kernel<NP, F16>, dim3((unsigned)sms), dim3(kThreads), smem_bytes(NP), s, true, a, TB, 2,
+    return launch_pdl(pages_chunk_kernel<ND, F16>, dim3((unsigned)sms), dim3(kThreads), smem_bytes((ND + 1) / 2), s, true, a, TB, 2,
                       counters, a.maps->k, a.maps->v);
 }
 
@@ -925,8 +1010,12 @@ cudaError_t launch_pages_chunk(const PagesAttn &a, cudaStream_t s) {
     ProfScope prof("pages_chunk", s);
     count_launch();
     const bool f16 = a.dtype == kF16;
-    if (a.st.D > 64) return f16 ? launch_chunk<2, true>(a, sms, s) : launch_chunk<2, false>(a, sms, s);
-    return f16 ? launch_chunk<1, true>(a, sms, s) : launch_chunk<1, false>(a, sms, s);
+    switch (a.st.D) {
+    case 32: return f16 ? launch_chunk<1, true>(a, sms, s) : launch_chunk<1, false>(a, sms, s);
+    case 64: return f16 ? launch_chunk<2, true>(a, sms, s) : launch_chunk<2, false>(a, sms, s);
+    case 96: return f16 ? launch_chunk<3, true>(a, sms, s) : launch_chunk<3, false>(a, sms, s);
+    default: return f16 ? launch_chunk<4, true>(a, sms, s) : launch_chunk<4, false>(a, sms, s);
+    }
 }
 
 // Tensor maps over 16-bit pages: rows of D elements, boxes of one page's tokens
