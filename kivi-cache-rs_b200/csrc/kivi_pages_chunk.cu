@@ -51,6 +51,7 @@ constexpr int kStages = 5;                // K and V tiles in flight
 constexpr int kPanel = 16384;             // 128 rows x 64 channels
 constexpr long long kWait = 2000000000LL; // ~1 s
 constexpr float kLazy = 8.0f;
+constexpr int kSoftRegs = 200, kRoleRegs = 96;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0, kColO = 256; // + 128 for B
 
@@ -344,6 +345,15 @@ __device__ __forceinline__ bool tile_edge(const PagesAttn &a, const Block &k, in
     if (T + kTok - 1 > k.p0) return true;
     return a.window && T < k.p1 - a.window + 1 && T + kTok > a.sinks;
 }
+// The same of one segment's tiles, from registers.
+struct Tiles {
+    int t0, ns, skip, p0, low, sinks;
+    __device__ __forceinline__ Tiles(const PagesAttn &a, const Seg &s)
+        : t0(s.t0), ns(s.k.ns), skip((s.k.ws - s.k.ns) * kTok), p0(s.k.p0), low(a.window ? s.k.p1 - a.window + 1 : 0),
+          sinks(a.sinks) {}
+    __device__ __forceinline__ int token(int j) const { return (t0 + j) * kTok + (t0 + j < ns ? 0 : skip); }
+    __device__ __forceinline__ bool edge(int T) const { return T + kTok - 1 > p0 || (T < low && T + kTok > sinks); }
+};
 // Some row of the block sees token t.
 __device__ __forceinline__ bool token_seen(const PagesAttn &a, const Block &k, int t) {
     return t <= k.p1 && (t >= k.lo || t < a.sinks);
@@ -364,7 +374,7 @@ struct Shared {
     long long scan[kThreads / 32];
     Walk walk;
     Seg seg[kSegs];
-    float2 ml[kRows]; // B's (m, l) when it shares A's rows
+    PagesAttn args; // for the functions out of line: the parameters' own place is slow to read by address
 };
 
 static_assert(sizeof(Shared) + 1024 + 7 * 2 * kPanel <= 232448, "shared memory per block");
@@ -399,27 +409,35 @@ __device__ __noinline__ void add_unfinite(const PagesAttn &a, const uint32_t *fl
     }
 }
 
-// The last CTA of a (block, head) joins its parts, in CTA order: eight float4 of
-// the block a thread at a time, one step's loads independent of one another.
+// Floats of one part: [D / 4][256 rows] float4 of O, then [256 rows] (m, l).
+__host__ __device__ constexpr int64_t kPartFloats(int D) { return (int64_t)2 * kRows * (D + 2); }
+
+// The last CTA of a (block, head) joins its parts, in CTA order.  A thread takes
+// (row, four channels) four at a time, one step's loads independent of one
+// another; eight lanes share a row, so outputs leave in runs of 64 bytes.
 template <int ND, bool F16> __device__ __noinline__ void join_parts(const PagesAttn &a, const Seg &s) {
-    constexpr int D = 32 * ND, D4 = D / 4, N = 8;
-    constexpr int64_t stride = D + 4;
-    const int G = a.G, n = s.rows * D4;
-    for (int i0 = threadIdx.x; i0 < n; i0 += 256 * N) {
+    constexpr int D = 32 * ND, N = 4;
+    const int G = a.G, n = (s.rows + 3) / 4 * 4 * (D / 4), tid = threadIdx.x;
+    // item i: groups of 8 channels-of-four x 4 rows
+    for (int i0 = tid; i0 < n; i0 += 256 * N) {
         float4 acc[N];
         float mm[N], ll[N];
+        int row[N], c4[N];
 #pragma unroll
-        for (int u = 0; u < N; ++u) acc[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), mm[u] = -INFINITY, ll[u] = 0.0f;
+        for (int u = 0; u < N; ++u) {
+            const int i = min(i0 + 256 * u, n - 1), g = i / 32; // 32 items: one warp's
+            row[u] = g / ND * 4 + (i % 32) / 8;
+            c4[u] = g % ND * 8 + i % 8;
+            acc[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), mm[u] = -INFINITY, ll[u] = 0.0f;
+        }
         for (int x = s.c0; x <= s.c1; ++x) {
-            const float *px = a.part + ((int64_t)x * 2 + (x == s.c0 ? 1 : 0)) * (2 * kRows) * stride;
+            const float *px = a.part + ((int64_t)x * 2 + (x == s.c0 ? 1 : 0)) * kPartFloats(D);
             float4 y[N];
             float2 ml[N];
 #pragma unroll
             for (int u = 0; u < N; ++u) {
-                const int i = min(i0 + 256 * u, n - 1);
-                const float *pp = px + (i / D4) * stride;
-                y[u] = __ldcg(reinterpret_cast<const float4 *>(pp) + i % D4);
-                ml[u] = __ldcg(reinterpret_cast<const float2 *>(pp + D));
+                y[u] = __ldcg(reinterpret_cast<const float4 *>(px) + c4[u] * (2 * kRows) + row[u]);
+                ml[u] = __ldcg(reinterpret_cast<const float2 *>(px + (int64_t)D * 2 * kRows) + row[u]);
             }
 #pragma unroll
             for (int u = 0; u < N; ++u) {
@@ -433,9 +451,9 @@ template <int ND, bool F16> __device__ __noinline__ void join_parts(const PagesA
         }
 #pragma unroll
         for (int u = 0; u < N; ++u) {
-            const int i = i0 + 256 * u;
-            if (i >= n) break;
-            const int r = i / D4, c = i % D4, tk = r / G, hd = r - tk * G;
+            const int r = row[u], c = c4[u];
+            if (i0 + 256 * u >= n || r >= s.rows) continue;
+            const int tk = r / G, hd = r - tk * G;
             const bool sees = s.k.p0 + tk >= 0;
             const float inv = 1.0f / ll[u];
             uint2 y = make_uint2(0, 0);
@@ -453,84 +471,118 @@ template <int ND, bool F16> __device__ __noinline__ void join_parts(const PagesA
     }
 }
 
-// This row's O, out: normalised to the output, or as a part.  A's threads add B's
-// O where B shared their rows.
+__device__ __noinline__ uint4 load_unaligned(const uint16_t *x) {
+    return make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16,
+                      x[6] | (uint32_t)x[7] << 16);
+}
+__device__ __noinline__ void store_unaligned(uint16_t *x, uint4 y) {
+    const uint32_t e[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = (uint16_t)(e[k / 2] >> (16 * (k & 1)));
+}
+
+// The warp's 32 rows of O, out: normalised to the output (through the warp's part
+// of its query tile, which is free by now, so that whole rows are stored a step),
+// or as a part ([channels / 4][row] float4: a step's stores are contiguous).  A's
+// threads add B's O where B shared their rows.  `off`: the row's output, as load_query's.
 template <int ND, bool F16>
-__device__ __noinline__ void store_row(const PagesAttn &a, const Seg &s, uint32_t cO, int r, bool live, int tok, int head,
-                                       float m, float l, float fa, float fb) {
+__device__ __noinline__ void store_rows(const PagesAttn &a, const Seg &s, unsigned char *tile, uint32_t cO, int row0,
+                                        int r0, int64_t off, bool sees, float m, float l, float fa, float fb) {
     constexpr int D = 32 * ND;
-    const bool sees = live && s.k.p0 + tok >= 0;
+    const int lane = threadIdx.x & 31, row = row0 + lane;
     const float inv = sees ? 1.0f / l : 0.0f;
-    const int64_t otok = s.k.start + s.k.i0 + tok;
-    uint16_t *out = static_cast<uint16_t *>(a.out) + otok * a.o_token + (int64_t)(s.h * a.G + head) * a.o_head;
-    float *part = a.part + ((int64_t)s.part * (2 * kRows) + r) * (D + 4);
+    float4 *part = reinterpret_cast<float4 *>(a.part + (int64_t)s.part * kPartFloats(D)) + r0 + row;
+    const bool whole = s.whole, dual = s.dual;
+    if (whole) fa *= inv, fb *= inv;
+#pragma unroll 1
+    for (int c = 0; c < D; c += 16) {
+        float o[16];
+        tmem_ld16(cO + c, o);
 #pragma unroll
-    for (int c = 0; c < D; c += 32) {
-        float o[32];
-        tmem_ld32(cO + c, o);
-        if (s.dual) {
-            float o2[32];
-            tmem_ld32(cO + 128 + c, o2);
+        for (int i = 0; i < 16; ++i) o[i] *= fa;
+        if (dual) {
+            float o2[16];
+            tmem_ld16(cO + 128 + c, o2);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = o[i] * fa + o2[i] * fb;
+            for (int i = 0; i < 16; ++i) o[i] = fmaf(o2[i], fb, o[i]);
         }
-        // (no early exit: the tensor-memory loads are the whole warp's)
-        if (live && !s.whole) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<float4 *>(part + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        } else if (live) {
-            uint32_t y[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) y[i] = sees ? pack2<F16>(o[2 * i] * inv, o[2 * i + 1] * inv) : 0u;
-            if (a.o_vec) {
+        if (!whole) {
+            if (off >= 0) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<uint4 *>(out + c + 8 * i) = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-            } else {
+                    part[(c / 4 + i) * (2 * kRows)] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
+        } else {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) out[c + i] = (uint16_t)(y[i / 2] >> (16 * (i & 1)));
+            for (int i = 0; i < 2; ++i) {
+                const uint4 y =
+                    make_uint4(pack2<F16>(o[8 * i], o[8 * i + 1]), pack2<F16>(o[8 * i + 2], o[8 * i + 3]),
+                               pack2<F16>(o[8 * i + 4], o[8 * i + 5]), pack2<F16>(o[8 * i + 6], o[8 * i + 7]));
+                const int cc = c / 8 + i;
+                *reinterpret_cast<uint4 *>(tile + (cc >> 3) * kPanel + row * 128 + (((cc & 7) ^ (row & 7)) << 4)) =
+                    sees ? y : make_uint4(0, 0, 0, 0);
             }
         }
         __syncwarp();
     }
-    if (live && !s.whole) {
-        part[D] = m;
-        part[D + 1] = l;
-    } else if (live && a.lse) {
-        a.lse[otok * a.Hq + s.h * a.G + head] = sees ? m * 0.6931471805599453f + logf(l) : -INFINITY;
+    if (!s.whole) {
+        if (off >= 0)
+            reinterpret_cast<float2 *>(a.part + (int64_t)s.part * kPartFloats(D) + (int64_t)D * 2 * kRows)[r0 + row] =
+                make_float2(m, l);
+        return;
+    }
+    if (off >= 0 && a.lse) {
+        const int tok = (r0 + row) / a.G;
+        a.lse[(int64_t)(s.k.start + s.k.i0 + tok) * a.Hq + s.h * a.G + (r0 + row - tok * a.G)] =
+            sees ? m * 0.6931471805599453f + logf(l) : -INFINITY;
+    }
+    constexpr int C = D / 8, R = 32 / (C > 8 ? 16 : C > 4 ? 8 : 4), L = 32 / R;
+    const int c = lane % L, sub = lane / L;
+    uint16_t *out = static_cast<uint16_t *>(a.out) + 8 * c;
+#pragma unroll 2
+    for (int i = 0; i < 32; i += R) {
+        const int64_t d = __shfl_sync(0xffffffffu, (long long)off, i + sub);
+        const int r = row0 + i + sub;
+        if (d >= 0 && c < C) {
+            const uint4 y = *reinterpret_cast<const uint4 *>(tile + (c >> 3) * kPanel + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+            if (a.o_vec) *reinterpret_cast<uint4 *>(out + d) = y;
+            else store_unaligned(out + d, y);
+        }
     }
 }
 
-// A thread's query row into its tile (128-byte swizzle); rows past the block are zeros.
+// The warp's 32 query rows into their tile (128-byte swizzle): 16 bytes a lane,
+// whole rows a step (a lane reading its own row would touch 32 lines a load).
+// `off` is the lane's own row, element offset from a.q, or -1 past the block.
 template <int ND>
-__device__ __noinline__ void load_query(const PagesAttn &a, const Seg &s, unsigned char *dst, int row, bool live, int tok,
-                                        int head) {
-    constexpr int D = 32 * ND;
-    const uint16_t *q = static_cast<const uint16_t *>(a.q) + (int64_t)(s.k.start + s.k.i0 + tok) * a.q_token +
-                        (int64_t)(s.h * a.G + head) * a.q_head;
-    uint4 v[D / 8]; // all of the row in flight
-#pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
-        v[c] = make_uint4(0, 0, 0, 0);
-        if (live && a.q_vec) v[c] = __ldg(reinterpret_cast<const uint4 *>(q) + c);
-    }
-    if (live && !a.q_vec) {
+__device__ __noinline__ void load_query(const PagesAttn &a, unsigned char *tile, int row0, int64_t off) {
+    constexpr int D = 32 * ND, C = D / 8, R = 32 / (C > 8 ? 16 : C > 4 ? 8 : 4); // chunks a row, rows a step
+    constexpr int L = 32 / R;
+    constexpr int U = 32 / R < 8 ? 32 / R : 8; // loads in flight; a short loop, since this code is rarely in the instruction cache
+    const int lane = threadIdx.x & 31, c = lane % L, sub = lane / L;
+    const uint16_t *q = static_cast<const uint16_t *>(a.q) + 8 * c;
+    const uint32_t flip = a.qsign < 0.0f ? 0x80008000u : 0u;
+    unsigned char *dst = tile + (c >> 3) * kPanel;
 #pragma unroll 1
-        for (int c = 0; c < D / 8; ++c) {
-            uint32_t e[4];
+    for (int i0 = 0; i0 < 32; i0 += R * U) {
+        uint4 v[U];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) e[i] = q[8 * c + 2 * i] | (uint32_t)q[8 * c + 2 * i + 1] << 16;
+        for (int u = 0; u < U; ++u) {
+            const int64_t o = __shfl_sync(0xffffffffu, (long long)off, i0 + R * u + sub);
+            v[u] = make_uint4(0, 0, 0, 0);
+            if (o >= 0 && c < C) {
+                if (a.q_vec) v[u] = __ldg(reinterpret_cast<const uint4 *>(q + o));
+                else v[u] = load_unaligned(q + o);
+            }
+        }
 #pragma unroll
-            for (int k = 0; k < D / 8; ++k)
-                if (k == c) v[k] = make_uint4(e[0], e[1], e[2], e[3]);
+        for (int u = 0; u < U; ++u) {
+            const int r = row0 + i0 + R * u + sub;
+            if (c < C)
+                *reinterpret_cast<uint4 *>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+                    make_uint4(v[u].x ^ flip, v[u].y ^ flip, v[u].z ^ flip, v[u].w ^ flip);
         }
     }
-    const uint32_t flip = a.qsign < 0.0f ? 0x80008000u : 0u;
-#pragma unroll
-    for (int c = 0; c < D / 8; ++c)
-        *reinterpret_cast<uint4 *>(dst + (c >> 3) * kPanel + (((c & 7) ^ (row & 7)) << 4)) =
-            make_uint4(v[c].x ^ flip, v[c].y ^ flip, v[c].z ^ flip, v[c].w ^ flip);
 }
 
 // n low bits set (n may lie outside 0 .. 32)
@@ -550,6 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int H = st.H, G = a.G;
     unsigned int *status = st.status;
     if (tid == 0) {
+        sh.args = a;
         for (int i = 0; i < kStages; ++i) bar_init(&sh.full[i], 1), bar_init(&sh.empty[i], 1);
         for (int x = 0; x < 2; ++x) {
             bar_init(&sh.q_full[x], 4);
@@ -668,6 +721,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     bool ok = true;
 
+    // A softmax thread holds a row's 128 scores.  Its spills would go to L2 (shared
+    // memory leaves almost no L1), so the registers move to where they are needed:
+    // 256 kSoftRegs + 128 kRoleRegs of the block's 384 x 168.
+    static_assert(256 * kSoftRegs + 128 * kRoleRegs <= kThreads * 168, "register split");
+    if (warp < kSoft)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+    else
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
     if (warp < kSoft) {
         // ------------------------------------------------------------ softmax
         const int X = warp >> 2;   // A or B
@@ -697,10 +758,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             float m = -INFINITY, l = 0.0f;
             if (r0 < s.rows) {
                 // ---- the row's query, and an empty O
-                if (!(X && dual)) load_query<ND>(a, s, sq + X * NP * kPanel + row * 128, row, live, tok, head);
+                if (!(X && dual))
+                    load_query<ND>(sh.args, sq + X * NP * kPanel, row & ~31,
+                                   live ? (int64_t)(s.k.start + s.k.i0 + tok) * a.q_token + (int64_t)(s.h * G + head) * a.q_head
+                                        : -1);
                 {
-                    uint32_t z[32] = {};
-                    for (int c = 0; c < D; c += 32) tmem_st32(cO + c, z);
+                    const uint32_t z[16] = {};
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) tmem_st16(cO + c, z);
                     st_wait();
                 }
                 proxy_fence();
@@ -709,9 +774,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) bar_arrive(&sh.q_full[X]);
             }
             const int n = dual ? s.n : nX;
+            Tiles tl(a, s);
             for (int j = 0; j < n; ++j) {
-                const int T = tile_token(s.k, s.t0 + j);
-                const bool edge = tile_edge(a, s.k, T);
+                const int T = tl.token(j);
+                const bool edge = tl.edge(T);
                 const uint32_t e = ne;
                 if (edge) ++ne;
                 if (dual && (j & 1) != X) continue;
@@ -781,7 +847,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t it = item + 2 * j + 1;
                     if (!(ok = warp_wait(&sh.full[it % kStages], (it / kStages) & 1, status))) break;
                     const uint32_t *fl = sh.flags[e & 3];
-                    if (fl[0] | fl[1] | fl[2] | fl[3]) add_unfinite<ND, F16>(a, fl, s.k.b, s.h, T, p, lo, cO);
+                    if (fl[0] | fl[1] | fl[2] | fl[3]) add_unfinite<ND, F16>(sh.args, fl, s.k.b, s.h, T, p, lo, cO);
                 }
                 st_wait();
                 tc_before();
@@ -795,10 +861,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_after();
             float fa = 1.0f, fb = 0.0f;
             if (dual) {
-                if (X) sh.ml[row] = make_float2(m, l);
+                float2 *ml = reinterpret_cast<float2 *>(sq + NP * kPanel); // B's query tile is not in use
+                if (X) ml[row] = make_float2(m, l);
                 if (!(ok = ok && meet())) break;
                 if (!X) {
-                    const float2 y = sh.ml[row];
+                    const float2 y = ml[row];
                     const float nm = fmaxf(m, y.x), ref = nm == -INFINITY ? 0.0f : nm;
                     fa = ex2(m - ref), fb = ex2(y.x - ref);
                     m = nm;
@@ -806,7 +873,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             if (!ok) break;
-            if (any && !(X && dual)) store_row<ND, F16>(a, s, cO, r0 + row, live, tok, head, m, l, fa, fb);
+            if (any && !(X && dual))
+                store_rows<ND, F16>(sh.args, s, sq + X * NP * kPanel, cO, row & ~31, r0,
+                                    live ? (int64_t)(s.k.start + s.k.i0 + tok) * a.o_token + (int64_t)(s.h * G + head) * a.o_head
+                                         : -1,
+                                    p >= 0, m, l, fa, fb);
             if (!s.whole) {
                 __threadfence();
                 if (!(ok = meet())) break;
@@ -818,7 +889,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = meet())) break;
                 if (sh.last) {
                     __threadfence();
-                    join_parts<ND, F16>(a, s);
+                    join_parts<ND, F16>(sh.args, s);
                 }
             }
             if (dual && !(ok = meet())) break; // B's O and (m, l) are read
@@ -895,6 +966,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (!more) break;
             const Block &k = w.k;
+            for (int r = lane; r < s.rows; r += 32) { // the queries on their way to L2
+                const int tok = r / G;
+                const uint16_t *q = static_cast<const uint16_t *>(a.q) + (int64_t)(k.start + k.i0 + tok) * a.q_token +
+                                    (int64_t)(w.h * G + r - tok * G) * a.q_head;
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(q) : "memory");
+                if constexpr (D > 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + 64) : "memory");
+            }
             for (int j = 0; ok && j < s.n; ++j) {
                 const int T = tile_token(k, s.t0 + j), t = T + piece * box;
                 // a box is needed if some row sees one of its tokens
@@ -998,7 +1076,7 @@ template <int ND, bool F16> cudaError_t launch_chunk(const PagesAttn &a, int sms
 // prefix lies in shared memory while the list is built.
 bool pages_chunk_supported(const PagesAttn &a) { return a.st.bits == 16 && a.G <= 2 * kRows && a.b.batch <= 16384; }
 
-int64_t pages_chunk_scratch(int D, int sms) { return (int64_t)sms * 2 * (2 * kRows) * (D + 4); }
+int64_t pages_chunk_scratch(int D, int sms) { return (int64_t)sms * 2 * kPartFloats(D); }
 
 cudaError_t launch_pages_chunk(const PagesAttn &a, cudaStream_t s) {
     int dev = 0, sms = 0;
