@@ -51,7 +51,14 @@ constexpr int kStages = 5;                // K and V tiles in flight
 constexpr int kPanel = 16384;             // 128 rows x 64 channels
 constexpr long long kWait = 2000000000LL; // ~1 s
 constexpr float kLazy = 8.0f;
+#ifndef POLY
+#define POLY 1
+#endif
+constexpr int kPolyPairs = POLY;          // of every four pairs of weights, on the FMA pipe
 constexpr int kSoftRegs = 200, kRoleRegs = 96;
+#ifndef SEGC
+#define SEGC 4
+#endif
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0, kColO = 256; // + 128 for B
 
@@ -123,14 +130,14 @@ template <int N> __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, 
     else
         asm volatile(KIVI_SS_HEAD KIVI_SS_STEP "}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc), "r"(1u));
 }
-// O += P V over 128 tokens: 8 steps, P 8 columns and V 2048 bytes a step.
+// O += P V over 64 tokens: 4 steps, P 8 columns and V 2048 bytes a step.
 #define KIVI_TS_STEP                                                                                     \
     "add.u32 a, a, 8;\n\tadd.u64 b, b, 128;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
 __device__ __forceinline__ void mma_pv(uint32_t d, uint32_t a, uint64_t b, uint32_t id) {
     asm volatile("{\n\t.reg .pred e, t;\n\t.reg .b32 a;\n\t.reg .b64 b;\n\telect.sync _|e, 0xffffffff;\n\t"
                  "setp.ne.b32 t, %4, 0;\n\tmov.b32 a, %1;\n\tmov.b64 b, %2;\n\t"
                  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t" KIVI_TS_STEP KIVI_TS_STEP KIVI_TS_STEP
-                     KIVI_TS_STEP KIVI_TS_STEP KIVI_TS_STEP KIVI_TS_STEP "}" ::"r"(d),
+                 "}" ::"r"(d),
                  "r"(a), "l"(b), "r"(id), "r"(1u));
 }
 #undef KIVI_SS_HEAD
@@ -226,9 +233,10 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// NaN if any is
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 // (a0, a1) * m + c, one instruction
@@ -243,6 +251,36 @@ __device__ __forceinline__ void add2(float &a0, float &a1, float b0, float b1) {
         "mov.b64 {%0, %1}, ra;\n\t}"
         : "+f"(a0), "+f"(a1)
         : "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void fma2c(float &a0, float &a1, float x0, float x1, float c) { // a = a * x + c
+    asm("{\n\t.reg .b64 ra, rx, rc;\n\tmov.b64 ra, {%0, %1};\n\tmov.b64 rx, {%2, %3};\n\tmov.b64 rc, {%4, %4};\n\t"
+        "fma.rn.f32x2 ra, ra, rx, rc;\n\tmov.b64 {%0, %1}, ra;\n\t}"
+        : "+f"(a0), "+f"(a1)
+        : "f"(x0), "f"(x1), "f"(c));
+}
+// 2^x of a pair on the FMA pipe, for x <= 8: x = n + f with n an integer and
+// |f| <= 1/2, 2^f by a polynomial of degree 4 (fitted by Remez exchange: relative
+// error 2.6e-6), n added to its exponent.  Below -126: 2^-126.  The special
+// function unit's 16 results a cycle would take as long for a tile as the tensor
+// pipe does, so some of the tile's weights come from here.
+__device__ __forceinline__ void ex2_pair(float &x0, float &x1) {
+    constexpr float magic = 12582912.0f; // 1.5 * 2^23: adding it leaves round(x) in the low bits
+    x0 = fmaxf(x0, -126.0f), x1 = fmaxf(x1, -126.0f);
+    float t0 = x0, t1 = x1;
+    add2(t0, t1, magic, magic);
+    float r0 = t0, r1 = t1;
+    add2(r0, r1, -magic, -magic);
+    asm("{\n\t.reg .b64 rx, rr, rm;\n\tmov.b64 rx, {%0, %1};\n\tmov.b64 rr, {%2, %3};\n\tmov.b64 rm, {%4, %4};\n\t"
+        "fma.rn.f32x2 rx, rr, rm, rx;\n\tmov.b64 {%0, %1}, rx;\n\t}" // f = x - n
+        : "+f"(x0), "+f"(x1)
+        : "f"(r0), "f"(r1), "f"(-1.0f));
+    float p0 = 0.009570102207362652f, p1 = p0;
+    fma2c(p0, p1, x0, x1, 0.05591785907745361f);
+    fma2c(p0, p1, x0, x1, 0.240247443318367f);
+    fma2c(p0, p1, x0, x1, 0.6931217908859253f);
+    fma2c(p0, p1, x0, x1, 0.9999992847442627f);
+    x0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+    x1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 template <bool F16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if constexpr (F16) {
@@ -283,9 +321,15 @@ __device__ __forceinline__ Block make_block(const PagesAttn &a, int TB, int b, c
 }
 __device__ __forceinline__ int blocks_of(int n, int TB) { return (n + TB - 1) / TB; }
 
+// Each (block, head) takes kSegCost entries of the list before its tiles: what
+// starting and ending it costs, in tiles' time, so that runs of short blocks are no
+// longer than others.
+constexpr int kSegCost = SEGC;
+__device__ __forceinline__ int entries(const Block &k) { return k.nt + kSegCost; }
+
 // A CTA's run of the list, walked by its copy warp.
 struct Walk {
-    long long f, end, row0; // tiles of the flat list; first tile of the current (block, head)
+    long long f, end, row0; // entries of the flat list; first entry of the current (block, head)
     int i, h;               // block of the sequence, head
     Block k;
 };
@@ -299,10 +343,13 @@ struct Seg {
     int whole, c0, c1;  // no other CTA has a part; else the CTAs that do
     int part;           // this CTA's part among the parts of all
 };
-__device__ __forceinline__ void make_seg(const PagesAttn &a, const Walk &w, long long begin, long long per, Seg &s) {
+// False where the run holds none of the (block, head)'s tiles.
+__device__ __forceinline__ bool make_seg(const PagesAttn &a, const Walk &w, long long begin, long long per, Seg &s) {
+    const long long tile0 = w.row0 + kSegCost; // entry of its first tile
     s.k = w.k;
-    s.t0 = (int)(w.f - w.row0);
-    s.n = (int)min((long long)w.k.nt, w.end - w.row0) - s.t0;
+    s.t0 = (int)max(0ll, w.f - tile0);
+    s.n = (int)max(0ll, min((long long)w.k.nt, w.end - tile0)) - s.t0;
+    if (s.n <= 0) return false;
     s.h = w.h;
     s.rows = w.k.ntok * a.G;
     s.dual = s.rows <= kRows;
@@ -314,16 +361,17 @@ __device__ __forceinline__ void make_seg(const PagesAttn &a, const Walk &w, long
         const int tA = max(1, w.k.ns + max(0, (pA >= 0 ? pA / kTok + 1 : 0) - w.k.ws));
         s.nA = max(0, min(tA - s.t0, s.n)), s.nB = s.n;
     }
-    const bool first = w.row0 >= begin; // the (block, head) starts in this CTA
-    s.whole = first && w.row0 + w.k.nt <= begin + per;
+    const bool first = tile0 >= begin; // its first tile is in this CTA
+    s.whole = first && tile0 + w.k.nt <= begin + per;
     s.c0 = s.c1 = s.part = 0;
     if (!s.whole) {
-        s.c0 = (int)(w.row0 / per), s.c1 = (int)((w.row0 + w.k.nt - 1) / per);
+        s.c0 = (int)(tile0 / per), s.c1 = (int)((tile0 + w.k.nt - 1) / per);
         s.part = 2 * blockIdx.x + (first ? 1 : 0);
     }
+    return true;
 }
 __device__ __forceinline__ bool walk_next(const PagesAttn &a, int TB, Walk &w) {
-    w.f = w.row0 + w.k.nt;
+    w.f = w.row0 + entries(w.k);
     if (w.f >= w.end) return false;
     w.row0 = w.f;
     if (++w.h < a.st.H) return true;
@@ -364,7 +412,7 @@ constexpr int kReaders = 11; // warps that read them: all but the copy warp
 struct Shared {
     uint64_t full[kStages], empty[kStages];
     uint64_t seg_full[kSegs], seg_empty[kSegs];
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+    uint64_t q_full[2], s_full[2], h_full[2], p_full[2], o_full[2]; // h: the first half of P
     uint64_t edge[4], half[4]; // an edge tile's V has landed, is half through
     uint64_t meet;             // the softmax warps
     uint64_t drain;
@@ -430,6 +478,7 @@ template <int ND, bool F16> __device__ __noinline__ void join_parts(const PagesA
             c4[u] = g % ND * 8 + i % 8;
             acc[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), mm[u] = -INFINITY, ll[u] = 0.0f;
         }
+#pragma unroll 2
         for (int x = s.c0; x <= s.c1; ++x) {
             const float *px = a.part + ((int64_t)x * 2 + (x == s.c0 ? 1 : 0)) * kPartFloats(D);
             float4 y[N];
@@ -607,6 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int x = 0; x < 2; ++x) {
             bar_init(&sh.q_full[x], 4);
             bar_init(&sh.s_full[x], 1);
+            bar_init(&sh.h_full[x], 4);
             bar_init(&sh.p_full[x], 4);
             bar_init(&sh.o_full[x], 1);
         }
@@ -675,7 +725,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int bi;
     for (int k0 = 0; k0 < items; k0 += kThreads) {
         const int k = k0 + tid;
-        scan(k < items ? block_at(k, bi).nt : 0, sum);
+        scan(k < items ? entries(block_at(k, bi)) : 0, sum);
         tiles += sum;
     }
     tiles *= H;
@@ -687,13 +737,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int k = k0 + tid;
             Block blk{};
             if (k < items) blk = block_at(k, bi);
-            const long long nt = k < items ? (long long)blk.nt * H : 0;
+            const long long nt = k < items ? (long long)entries(blk) * H : 0;
             const long long first = run + scan(nt, sum);
             if (nt > 0 && begin >= first && begin < first + nt) {
                 Walk w;
                 w.f = begin, w.end = end;
-                w.h = (int)((begin - first) / blk.nt);
-                w.row0 = first + (long long)w.h * blk.nt;
+                w.h = (int)((begin - first) / entries(blk));
+                w.row0 = first + (long long)w.h * entries(blk);
                 w.i = bi;
                 w.k = blk;
                 sh.walk = w;
@@ -806,8 +856,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         m4[2] = max3(m4[2], x[i + 4], x[i + 5]);
                         m4[3] = max3(m4[3], x[i + 6], x[i + 7]);
                     }
-                    const float mx = fmaxf(max3(max3(m4[0], x[124], x[125]), max3(m4[1], x[126], x[127]), m4[2]), m4[3]) * crow;
-                    const bool need = mx > m + kLazy, move = need && m != -INFINITY;
+                    const float mx = max3(max3(max3(m4[0], x[124], x[125]), max3(m4[1], x[126], x[127]), m4[2]), m4[3], m4[3]) * crow;
+                    // a NaN score makes the reference, and with it the row, NaN
+                    const bool need = !(mx <= m + kLazy), move = need && m != -INFINITY;
                     const float f = move ? ex2(m - mx) : 1.0f;
                     if (need) m = mx;
                     if (__any_sync(0xffffffffu, move)) {
@@ -828,18 +879,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int hlf = 0; hlf < 2; ++hlf) {
                         uint32_t pk[32];
 #pragma unroll
-                        for (int i = 0; i < 64; i += 4) {
+                        for (int i = 0; i < 64; i += 8) {
                             float *y = x + 64 * hlf + i;
-                            fma2s(y[0], y[1], crow, off);
-                            fma2s(y[2], y[3], crow, off);
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) y[q] = ex2(y[q]);
-                            add2(a0, a1, y[0], y[1]);
-                            add2(a2, a3, y[2], y[3]);
-                            pk[i / 2] = pack2<F16>(y[0], y[1]);
-                            pk[i / 2 + 1] = pack2<F16>(y[2], y[3]);
+                            for (int q = 0; q < 8; q += 2) {
+                                fma2s(y[q], y[q + 1], crow, off);
+                                if (q < 2 * kPolyPairs) ex2_pair(y[q], y[q + 1]);
+                                else y[q] = ex2(y[q]), y[q + 1] = ex2(y[q + 1]);
+                                if (q & 2) add2(a2, a3, y[q], y[q + 1]);
+                                else add2(a0, a1, y[q], y[q + 1]);
+                                pk[(i + q) / 2] = pack2<F16>(y[q], y[q + 1]);
+                            }
                         }
                         tmem_st32(cS + 32 * hlf, pk);
+                        if (hlf == 0) { // the tensor pipe starts on the first 64 tokens
+                            st_wait();
+                            tc_before();
+                            __syncwarp();
+                            // (an edge tile's V may still change, and its O)
+                            if (lane == 0 && !edge) bar_arrive(&sh.h_full[X]);
+                        }
                     }
                     l += (a0 + a1) + (a2 + a3);
                 }
@@ -852,7 +911,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 st_wait();
                 tc_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive(&sh.p_full[X]);
+                if (lane == 0) {
+                    if (edge || !any) bar_arrive(&sh.h_full[X]);
+                    bar_arrive(&sh.p_full[X]);
+                }
             }
             for (int j = nX; !dual && j < s.n; ++j) ne += tile_edge(a, s.k, tile_token(s.k, s.t0 + j));
             item += 2 * s.n;
@@ -929,9 +991,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             auto pv = [&](int X, int i) {
                 const uint32_t it = item + 2 * tile(X, i) + 1, slot = it % kStages;
                 if (!warp_wait(&sh.full[slot], (it / kStages) & 1, status)) return false;
+                const uint32_t o = tm + kColO + 128 * X, p = tm + kColS + 128 * X;
+                const uint64_t v = dv + (uint64_t)slot * (NP * kPanel / 16);
+                if (!warp_wait(&sh.h_full[X], np[X] & 1, status)) return false;
+                tc_after();
+                mma_pv(o, p, v, id_pv);
                 if (!warp_wait(&sh.p_full[X], np[X]++ & 1, status)) return false;
                 tc_after();
-                mma_pv(tm + kColO + 128 * X, tm + kColS + 128 * X, dv + (uint64_t)slot * (NP * kPanel / 16), id_pv);
+                mma_pv(o, p + 32, v + 4 * 128, id_pv);
                 if (frees(X)) mma_commit(&sh.empty[slot]);
                 if (i + 1 == (X ? nB : nA)) mma_commit(&sh.o_full[X]);
                 return true;
@@ -958,8 +1025,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t slot = nseg % kSegs;
             if (nseg >= kSegs && !(ok = warp_wait(&sh.seg_empty[slot], (nseg / kSegs - 1) & 1, status))) break;
             Seg s;
-            s.n = 0;
-            if (more) make_seg(a, w, begin, per, s);
+            while (more && !make_seg(a, w, begin, per, s)) more = walk_next(a, TB, w);
+            if (!more) s.n = 0;
             if (lane == 0) {
                 sh.seg[slot] = s;
                 bar_arrive(&sh.seg_full[slot]);
