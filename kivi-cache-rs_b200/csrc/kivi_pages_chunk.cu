@@ -51,14 +51,8 @@ constexpr int kStages = 5;                // K and V tiles in flight
 constexpr int kPanel = 16384;             // 128 rows x 64 channels
 constexpr long long kWait = 2000000000LL; // ~1 s
 constexpr float kLazy = 8.0f;
-#ifndef POLY
-#define POLY 1
-#endif
-constexpr int kPolyPairs = POLY;          // of every four pairs of weights, on the FMA pipe
+constexpr int kPolyPairs = 1;             // of every four pairs of weights, on the FMA pipe
 constexpr int kSoftRegs = 200, kRoleRegs = 96;
-#ifndef SEGC
-#define SEGC 4
-#endif
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0, kColO = 256; // + 128 for B
 
@@ -114,41 +108,48 @@ __device__ __forceinline__ uint32_t idesc(int bf16, int N, int b_mn_major) {
            ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
 }
 
-// MMAs over up to one 64-channel panel (both operands in shared memory, 32 bytes
-// a step), N of them, by one elected lane; the first accumulates iff acc.
-#define KIVI_SS_HEAD                                                                                     \
-    "{\n\t.reg .pred p, e, t;\n\t.reg .b64 a, b;\n\telect.sync _|e, 0xffffffff;\n\t"                      \
-    "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 t, %5, 0;\n\tmov.b64 a, %1;\n\tmov.b64 b, %2;\n\t"              \
-    "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
-#define KIVI_SS_STEP                                                                                     \
-    "add.u64 a, a, 2;\n\tadd.u64 b, b, 2;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
-template <int N> __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    static_assert(N == 2 || N == 4, "steps");
-    if constexpr (N == 4)
-        asm volatile(KIVI_SS_HEAD KIVI_SS_STEP KIVI_SS_STEP KIVI_SS_STEP "}" ::"r"(d), "l"(a), "l"(b), "r"(id),
-                     "r"(acc), "r"(1u));
-    else
-        asm volatile(KIVI_SS_HEAD KIVI_SS_STEP "}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc), "r"(1u));
+// One asm block per step of the issuing warp: one elect.sync, the MMAs by the
+// elected lane, and the commits that publish them (a commit arrives on its barrier
+// when every MMA issued before it has completed).
+#define KIVI_SS(off) \
+    "add.u64 a, %1, " #off ";\n\tadd.u64 b, %2, " #off ";\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+#define KIVI_COMMIT(bar) "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [" bar "];\n\t"
+// S = Q K^T over D channels: 32 bytes a step within a 64-channel panel, panels
+// kPanel bytes apart; publishes S on `done` and, if release, K's stage on `freed`.
+template <int D>
+__device__ __forceinline__ void mma_qk(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint64_t *done, uint64_t *freed,
+                                       bool release) {
+#define KIVI_QK(steps)                                                                                   \
+    asm volatile("{\n\t.reg .pred p, e, t, r;\n\t.reg .b64 a, b;\n\telect.sync _|e, 0xffffffff;\n\t"      \
+                 "setp.ne.b32 p, %4, %4;\n\tsetp.eq.b32 t, %4, %4;\n\tsetp.ne.and.b32 r, %6, 0, e;\n\t"    \
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t" steps                  \
+                 "@e " KIVI_COMMIT("%4") "@r " KIVI_COMMIT("%5") "}" ::"r"(d),                            \
+                 "l"(a), "l"(b), "r"(id), "r"(su32(done)), "r"(su32(freed)), "r"((uint32_t)release)       \
+                 : "memory")
+    static_assert(kPanel / 16 == 1024, "panel offset below");
+    if constexpr (D == 32) KIVI_QK(KIVI_SS(2));
+    else if constexpr (D == 64) KIVI_QK(KIVI_SS(2) KIVI_SS(4) KIVI_SS(6));
+    else if constexpr (D == 96) KIVI_QK(KIVI_SS(2) KIVI_SS(4) KIVI_SS(6) KIVI_SS(1024) KIVI_SS(1026));
+    else KIVI_QK(KIVI_SS(2) KIVI_SS(4) KIVI_SS(6) KIVI_SS(1024) KIVI_SS(1026) KIVI_SS(1028) KIVI_SS(1030));
+#undef KIVI_QK
 }
 // O += P V over 64 tokens: 4 steps, P 8 columns and V 2048 bytes a step.
-#define KIVI_TS_STEP                                                                                     \
-    "add.u32 a, a, 8;\n\tadd.u64 b, b, 128;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
-__device__ __forceinline__ void mma_pv(uint32_t d, uint32_t a, uint64_t b, uint32_t id) {
-    asm volatile("{\n\t.reg .pred e, t;\n\t.reg .b32 a;\n\t.reg .b64 b;\n\telect.sync _|e, 0xffffffff;\n\t"
-                 "setp.ne.b32 t, %4, 0;\n\tmov.b32 a, %1;\n\tmov.b64 b, %2;\n\t"
-                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t" KIVI_TS_STEP KIVI_TS_STEP KIVI_TS_STEP
-                 "}" ::"r"(d),
-                 "r"(a), "l"(b), "r"(id), "r"(1u));
-}
-#undef KIVI_SS_HEAD
-#undef KIVI_SS_STEP
-#undef KIVI_TS_STEP
-// Arrives on b when every MMA issued so far has completed.
-__device__ __forceinline__ void mma_commit(uint64_t *b) {
-    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(su32(b))
+#define KIVI_TS(i) \
+    "add.u32 a, %1, 8 * " #i ";\n\tadd.u64 b, %2, 128 * " #i ";\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+__device__ __forceinline__ void mma_pv(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint64_t *freed, bool release) {
+    asm volatile("{\n\t.reg .pred e, t, r;\n\t.reg .b32 a;\n\t.reg .b64 b;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "setp.eq.b32 t, %4, %4;\n\tsetp.ne.and.b32 r, %5, 0, e;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, t;\n\t" KIVI_TS(1) KIVI_TS(2) KIVI_TS(3)
+                 "@r " KIVI_COMMIT("%4") "}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(id), "r"(su32(freed)), "r"((uint32_t)release)
                  : "memory");
 }
+__device__ __forceinline__ void mma_commit(uint64_t *b) {
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e " KIVI_COMMIT("%0") "}" ::"r"(su32(b)) : "memory");
+}
+#undef KIVI_SS
+#undef KIVI_TS
+#undef KIVI_COMMIT
 __device__ __forceinline__ void copy_box(void *dst, const CUtensorMap *map, int x, int y, uint64_t *b) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
                  "[%4];" ::"r"(su32(dst)),
@@ -324,7 +325,7 @@ __device__ __forceinline__ int blocks_of(int n, int TB) { return (n + TB - 1) / 
 // Each (block, head) takes kSegCost entries of the list before its tiles: what
 // starting and ending it costs, in tiles' time, so that runs of short blocks are no
 // longer than others.
-constexpr int kSegCost = SEGC;
+constexpr int kSegCost = 4;
 __device__ __forceinline__ int entries(const Block &k) { return k.nt + kSegCost; }
 
 // A CTA's run of the list, walked by its copy warp.
@@ -342,6 +343,7 @@ struct Seg {
     int nA, nB;         // tiles of each
     int whole, c0, c1;  // no other CTA has a part; else the CTAs that do
     int part;           // this CTA's part among the parts of all
+    uint32_t item, edges; // copies and edge tiles of the run before it
 };
 // False where the run holds none of the (block, head)'s tiles.
 __device__ __forceinline__ bool make_seg(const PagesAttn &a, const Walk &w, long long begin, long long per, Seg &s) {
@@ -464,7 +466,7 @@ __host__ __device__ constexpr int64_t kPartFloats(int D) { return (int64_t)2 * k
 // (row, four channels) four at a time, one step's loads independent of one
 // another; eight lanes share a row, so outputs leave in runs of 64 bytes.
 template <int ND, bool F16> __device__ __noinline__ void join_parts(const PagesAttn &a, const Seg &s) {
-    constexpr int D = 32 * ND, N = 4;
+    constexpr int D = 32 * ND, N = 8;
     const int G = a.G, n = (s.rows + 3) / 4 * 4 * (D / 4), tid = threadIdx.x;
     // item i: groups of 8 channels-of-four x 4 rows
     for (int i0 = tid; i0 < n; i0 += 256 * N) {
@@ -786,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t lanes = tm + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t cS = lanes + kColS + 128 * X, cO = lanes + kColO + 128 * X;
         const float crow = a.scale * 1.4426950408889634f;
-        uint32_t ns = 0, no = 0, ne = 0, item = 0, met = 0; // tiles, blocks, edge tiles, copies, meetings so far
+        uint32_t ns = 0, no = 0, met = 0; // tiles, blocks, meetings so far
         auto meet = [&]() { // of the softmax warps
             tc_before();
             __syncwarp();
@@ -825,11 +827,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const int n = dual ? s.n : nX;
             Tiles tl(a, s);
+            uint32_t edges = s.edges; // edge tiles of the run up to this one
             for (int j = 0; j < n; ++j) {
                 const int T = tl.token(j);
                 const bool edge = tl.edge(T);
-                const uint32_t e = ne;
-                if (edge) ++ne;
+                if (edge) ++edges;
                 if (dual && (j & 1) != X) continue;
                 if (!(ok = warp_wait(&sh.s_full[X], ns & 1, status))) break;
                 ++ns;
@@ -903,9 +905,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     l += (a0 + a1) + (a2 + a3);
                 }
                 if (edge) { // the tile's V has been through the fixing warps
-                    const uint32_t it = item + 2 * j + 1;
+                    const uint32_t it = s.item + 2 * j + 1;
                     if (!(ok = warp_wait(&sh.full[it % kStages], (it / kStages) & 1, status))) break;
-                    const uint32_t *fl = sh.flags[e & 3];
+                    const uint32_t *fl = sh.flags[(edges - 1) & 3];
                     if (fl[0] | fl[1] | fl[2] | fl[3]) add_unfinite<ND, F16>(sh.args, fl, s.k.b, s.h, T, p, lo, cO);
                 }
                 st_wait();
@@ -916,8 +918,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     bar_arrive(&sh.p_full[X]);
                 }
             }
-            for (int j = nX; !dual && j < s.n; ++j) ne += tile_edge(a, s.k, tile_token(s.k, s.t0 + j));
-            item += 2 * s.n;
             // ---- the rows out
             if (ok && nX > 0) ok = warp_wait(&sh.o_full[X], no++ & 1, status);
             tc_after();
@@ -961,56 +961,76 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t id_qk = idesc(!F16, kTok, 0), id_pv = idesc(!F16, D, 1);
         const uint64_t dq = sdesc(su32(sq), 16, 1024), dr = sdesc(su32(ring), 16, 1024),
                        dv = sdesc(su32(ring), kPanel, 1024);
-        uint32_t np[2] = {0, 0}, nq[2] = {0, 0}, item = 0;
+        uint32_t np[2] = {0, 0}, nq = 0; // tiles and blocks so far, modulo 2
+        auto wait = [&](uint64_t *b, uint32_t par) { return warp_wait(b, par, status); };
+        // a stage of the ring and the parity of its present phase
+        struct Pos {
+            uint32_t slot, par;
+            __device__ __forceinline__ Pos on(uint32_t n) const { // n <= kStages items on
+                const bool wrap = slot + n >= kStages;
+                return Pos{wrap ? slot + n - kStages : slot + n, wrap ? par ^ 1u : par};
+            }
+        };
+        auto qk = [&](int X, int q, uint32_t slot, bool release) {
+            mma_qk<D>(tm + kColS + 128 * X, dq + q * (NP * kPanel / 16), dr + slot * (NP * kPanel / 16), id_qk, &sh.s_full[X],
+                      &sh.empty[slot], release);
+        };
+        auto pv = [&](int X, uint32_t slot, bool release) { // by halves, as the weights come
+            const uint32_t o = tm + kColO + 128 * X, p = tm + kColS + 128 * X;
+            const uint64_t v = dv + slot * (NP * kPanel / 16);
+            if (!wait(&sh.h_full[X], np[X])) return false;
+            tc_after();
+            mma_pv(o, p, v, id_pv, &sh.empty[slot], false);
+            if (!wait(&sh.p_full[X], np[X])) return false;
+            np[X] ^= 1;
+            tc_after();
+            mma_pv(o, p + 32, v + 4 * 128, id_pv, &sh.empty[slot], release);
+            return true;
+        };
         while (ok && next_seg()) {
             const Seg &s = *sp;
-            const int dual = s.dual, nA = s.nA, nB = s.nB;
-            // tile (of the segment) that X takes as its i-th
-            auto tile = [&](int X, int i) { return dual ? 2 * i + X : i; };
-            // this use of a tile is its last
-            auto frees = [&](int X) { return dual || X == 1; };
-            auto qk = [&](int X, int i) {
-                const uint32_t it = item + 2 * tile(X, i), slot = it % kStages;
-                if (i == 0 && !warp_wait(&sh.q_full[X], nq[X]++ & 1, status)) return false;
-                if (!warp_wait(&sh.full[slot], (it / kStages) & 1, status)) return false;
-                tc_after();
-                const uint32_t d = tm + kColS + 128 * X;
-                const uint64_t q = dq + (uint64_t)(dual ? 0 : X) * (NP * kPanel / 16);
-                const uint64_t b = dr + (uint64_t)slot * (NP * kPanel / 16);
-                if constexpr (D == 32) {
-                    mma_ss<2>(d, q, b, id_qk, 0u);
-                } else {
-                    mma_ss<4>(d, q, b, id_qk, 0u);
-                    if constexpr (D == 96) mma_ss<2>(d, q + kPanel / 16, b + kPanel / 16, id_qk, 1u);
-                    if constexpr (D == 128) mma_ss<4>(d, q + kPanel / 16, b + kPanel / 16, id_qk, 1u);
+            const int n = s.n, nA = s.nA;
+            Pos K{s.item % kStages, s.item / kStages & 1u}; // of the tile whose O += P V is next
+            ok = wait(&sh.q_full[0], nq) && wait(&sh.q_full[1], nq) && wait(&sh.full[K.slot], K.par);
+            nq ^= 1;
+            if (!ok) break;
+            tc_after();
+            if (!s.dual) {
+                if (nA > 0) qk(0, 0, K.slot, false);
+                qk(1, 1, K.slot, true);
+                for (int i = 0; ok && i < n; ++i) {
+                    const Pos V = K.on(1), N = K.on(2);
+                    const bool next = i + 1 < n;
+                    if (!(ok = wait(&sh.full[V.slot], V.par))) break;
+                    if (i < nA && !(ok = pv(0, V.slot, false))) break;
+                    if (i + 1 == nA) mma_commit(&sh.o_full[0]);
+                    if (next && !(ok = wait(&sh.full[N.slot], N.par))) break;
+                    if (i + 1 < nA) qk(0, 0, N.slot, false);
+                    if (!(ok = pv(1, V.slot, true))) break;
+                    if (next) qk(1, 1, N.slot, true);
+                    K = N;
                 }
-                mma_commit(&sh.s_full[X]);
-                if (frees(X)) mma_commit(&sh.empty[slot]);
-                return true;
-            };
-            auto pv = [&](int X, int i) {
-                const uint32_t it = item + 2 * tile(X, i) + 1, slot = it % kStages;
-                if (!warp_wait(&sh.full[slot], (it / kStages) & 1, status)) return false;
-                const uint32_t o = tm + kColO + 128 * X, p = tm + kColS + 128 * X;
-                const uint64_t v = dv + (uint64_t)slot * (NP * kPanel / 16);
-                if (!warp_wait(&sh.h_full[X], np[X] & 1, status)) return false;
-                tc_after();
-                mma_pv(o, p, v, id_pv);
-                if (!warp_wait(&sh.p_full[X], np[X]++ & 1, status)) return false;
-                tc_after();
-                mma_pv(o, p + 32, v + 4 * 128, id_pv);
-                if (frees(X)) mma_commit(&sh.empty[slot]);
-                if (i + 1 == (X ? nB : nA)) mma_commit(&sh.o_full[X]);
-                return true;
-            };
-            // row tiles without a cached tile in this run report their queries all the same
-            ok = nA > 0 ? qk(0, 0) : warp_wait(&sh.q_full[0], nq[0]++ & 1, status);
-            if (ok) ok = nB > 0 ? qk(1, 0) : warp_wait(&sh.q_full[1], nq[1]++ & 1, status);
-            for (int i = 0; ok && i < max(nA, nB); ++i) {
-                if (i < nA) ok = pv(0, i) && (i + 1 >= nA || qk(0, i + 1));
-                if (ok && i < nB) ok = pv(1, i) && (i + 1 >= nB || qk(1, i + 1));
+                if (ok) mma_commit(&sh.o_full[1]);
+            } else { // tile t is A's or B's in turn, over the one query tile
+                qk(0, 0, K.slot, true);
+                if (n > 1) {
+                    const Pos N = K.on(2);
+                    if (!(ok = wait(&sh.full[N.slot], N.par))) break;
+                    qk(1, 0, N.slot, true);
+                }
+                for (int t = 0; ok && t < n; ++t) {
+                    const int X = t & 1;
+                    const Pos V = K.on(1), N = K.on(4);
+                    if (!(ok = wait(&sh.full[V.slot], V.par) && pv(X, V.slot, true))) break;
+                    if (t + 2 < n) {
+                        if (!(ok = wait(&sh.full[N.slot], N.par))) break;
+                        qk(X, 0, N.slot, true);
+                    } else {
+                        mma_commit(&sh.o_full[X]);
+                    }
+                    K = K.on(2);
+                }
             }
-            item += 2 * s.n;
         }
         mma_commit(&sh.drain); // tensor memory outlives every MMA
         warp_wait(&sh.drain, 0, status);
@@ -1027,6 +1047,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             Seg s;
             while (more && !make_seg(a, w, begin, per, s)) more = walk_next(a, TB, w);
             if (!more) s.n = 0;
+            s.item = item, s.edges = ne;
             if (lane == 0) {
                 sh.seg[slot] = s;
                 bar_arrive(&sh.seg_full[slot]);
@@ -1069,13 +1090,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         // ------------------------------------------------------------ V rows of edge tiles
-        uint32_t item = 0, ne = 0;
         while (ok && next_seg()) {
             const Seg &s = *sp;
-            for (int j = 0; ok && j < s.n; ++j, item += 2) {
+            uint32_t ne = s.edges;
+            for (int j = 0; ok && j < s.n; ++j) {
                 const int T = tile_token(s.k, s.t0 + j);
                 if (!tile_edge(a, s.k, T)) continue;
-                const uint32_t slot = (item + 1) % kStages;
+                const uint32_t slot = (s.item + 2 * j + 1) % kStages;
                 if (!(ok = warp_wait(&sh.edge[ne & 3], (ne >> 2) & 1, status))) break;
                 unsigned char *v = ring + slot * (NP * kPanel);
 #pragma unroll 1
