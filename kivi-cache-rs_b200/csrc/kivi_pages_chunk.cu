@@ -46,13 +46,17 @@ constexpr int kTok = 128;                 // cached tokens per tile
 constexpr int kRows = 128;                // rows of one row tile
 constexpr int kSoft = 8;                  // softmax warps
 constexpr int kMmaWarp = 8, kCopyWarp = 9, kFixWarp = 10; // and 11
-constexpr int kThreads = 384;
-constexpr int kStages = 5;                // K and V tiles in flight
+constexpr int kConvWarp = 12;             // codes: 12-15 convert
+__host__ __device__ constexpr int threads_of(int bits) { return bits == 16 ? 384 : 512; }
+// K and V tiles in flight
+__host__ __device__ constexpr int stages_of(int bits) { return bits == 16 ? 5 : 4; }
 constexpr int kPanel = 16384;             // 128 rows x 64 channels
 constexpr long long kWait = 2000000000LL; // ~1 s
 constexpr float kLazy = 8.0f;
 constexpr int kPolyPairs = 1;             // of every four pairs of weights, on the FMA pipe
-constexpr int kSoftRegs = 200, kRoleRegs = 96;
+// registers of a softmax thread and of the others
+__host__ __device__ constexpr int soft_regs(int bits) { return bits == 16 ? 200 : 176; }
+__host__ __device__ constexpr int role_regs(int bits) { return bits == 16 ? 96 : 80; }
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0, kColO = 256; // + 128 for B
 
@@ -292,6 +296,7 @@ template <bool F16> __device__ __forceinline__ uint32_t pack2(float a, float b) 
         return *reinterpret_cast<const uint32_t *>(&h);
     }
 }
+__device__ __forceinline__ uint32_t pack_out(bool f16, float a, float b) { return f16 ? pack2<true>(a, b) : pack2<false>(a, b); }
 __device__ __forceinline__ float unpack(bool f16, uint16_t x) {
     return f16 ? __half2float(__ushort_as_half(x)) : __uint_as_float((uint32_t)x << 16);
 }
@@ -410,29 +415,46 @@ __device__ __forceinline__ bool token_seen(const PagesAttn &a, const Block &k, i
 }
 
 constexpr int kSegs = 4;     // segments published ahead
-constexpr int kReaders = 11; // warps that read them: all but the copy warp
+// warps that read them: softmax, MMA, and those that touch the operand tiles
+__host__ __device__ constexpr int readers_of(int bits) { return kSoft + 1 + (bits == 16 ? 2 : 4); }
 struct Shared {
-    uint64_t full[kStages], empty[kStages];
+    uint64_t full[5], empty[5]; // stages_of(bits) in use
     uint64_t seg_full[kSegs], seg_empty[kSegs];
     uint64_t q_full[2], s_full[2], h_full[2], p_full[2], o_full[2]; // h: the first half of P
     uint64_t edge[4], half[4]; // an edge tile's V has landed, is half through
     uint64_t meet;             // the softmax warps
+    uint64_t range[4], conv;   // codes: a tile's exponents are known; the converting warps
     uint64_t drain;
     uint32_t flags[4][4]; // tokens of an edge tile whose value row is not finite
     uint32_t tmem;
     int last;
-    long long scan[kThreads / 32];
+    long long scan[16];
     Walk walk;
     Seg seg[kSegs];
     PagesAttn args; // for the functions out of line: the parameters' own place is slow to read by address
 };
 
-static_assert(sizeof(Shared) + 1024 + 7 * 2 * kPanel <= 232448, "shared memory per block");
-constexpr int smem_bytes(int np) { return 2 * np * kPanel + kStages * np * kPanel + (int)sizeof(Shared) + 1024; }
+// Codes: the operands are f16, a tile's keys and values times 2^-exponent (largest
+// finite one below 2^14), a row's query likewise, and a token's (scale, centre).
+struct SharedCodes {
+    int kexp[4], vexp[4];  // of tile counter & 3
+    float most[2][4][2];   // a tile's largest key and value per warp, by tile parity
+    float4 token[2][kTok]; // key scale, key centre, value scale, value centre
+    int qexp[2 * kRows];
+};
+constexpr int smem_bytes(int bits, int np) {
+    return (2 + stages_of(bits)) * np * kPanel + (int)sizeof(Shared) + (bits == 16 ? 0 : (int)sizeof(SharedCodes)) + 1024;
+}
+static_assert(smem_bytes(16, 2) <= 232448 && smem_bytes(8, 2) <= 232448, "shared memory per block");
+
+__device__ __forceinline__ float exp2i(int k) { return __uint_as_float((uint32_t)(max(-126, min(127, k)) + 127) << 23); }
+// e with x 2^-e < 2^14 for x >= 0 (the upper end of f16, so that what is far smaller
+// than x keeps its bits too); -126 at least
+__device__ __forceinline__ int f16_exponent(float x) { return max(-126, (int)(__float_as_uint(x) >> 23) - 140); }
 
 // Rows of V that are not finite were taken out of an edge tile (flags, one bit
 // per token); they are added here to the rows that see them: p > 0, so p v is v.
-template <int ND, bool F16>
+template <int BITS, int ND, bool F16>
 __device__ __noinline__ void add_unfinite(const PagesAttn &a, const uint32_t *flags, int b, int h, int T, int p, int lo,
                                           uint32_t cO) {
     for (int f = 0; f < 4; ++f) {
@@ -442,14 +464,18 @@ __device__ __noinline__ void add_unfinite(const PagesAttn &a, const uint32_t *fl
             bits &= bits - 1;
             const bool see = t <= p && (t >= lo || t < a.sinks);
             const int64_t r = pages_row(a.st, max(pages_page(a.b, a.st, b, t), 0), h, t);
-            const uint16_t *v = reinterpret_cast<const uint16_t *>(a.st.v + r * a.st.row_bytes);
+            const unsigned char *v = a.st.v + r * a.st.row_bytes;
+            const float2 q = BITS == 16 ? make_float2(0.0f, 0.0f) : __ldg(a.st.vp + r);
 #pragma unroll 1
             for (int c = 0; c < 32 * ND; c += 32) {
                 float o[32];
                 tmem_ld32(cO + c, o);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    const float y = unpack(F16, v[c + i]);
+                    float y;
+                    if constexpr (BITS == 16) y = unpack(F16, reinterpret_cast<const uint16_t *>(v)[c + i]);
+                    else if constexpr (BITS == 8) y = fmaf((float)v[c + i], q.x, q.y);
+                    else y = fmaf((float)(v[(c + i) / 2] >> (4 * (i & 1)) & 15), q.x, q.y);
                     if (see && !isfinite(y)) o[i] += y;
                 }
                 tmem_st32(cO + c, reinterpret_cast<const uint32_t *>(o));
@@ -465,9 +491,10 @@ __host__ __device__ constexpr int64_t kPartFloats(int D) { return (int64_t)2 * k
 // The last CTA of a (block, head) joins its parts, in CTA order.  A thread takes
 // (row, four channels) four at a time, one step's loads independent of one
 // another; eight lanes share a row, so outputs leave in runs of 64 bytes.
-template <int ND, bool F16> __device__ __noinline__ void join_parts(const PagesAttn &a, const Seg &s) {
+template <int ND> __device__ __noinline__ void join_parts(const PagesAttn &a, const Seg &s) {
     constexpr int D = 32 * ND, N = 8;
     const int G = a.G, n = (s.rows + 3) / 4 * 4 * (D / 4), tid = threadIdx.x;
+    const bool f16 = a.dtype == kF16;
     // item i: groups of 8 channels-of-four x 4 rows
     for (int i0 = tid; i0 < n; i0 += 256 * N) {
         float4 acc[N];
@@ -508,7 +535,7 @@ template <int ND, bool F16> __device__ __noinline__ void join_parts(const PagesA
             const bool sees = s.k.p0 + tk >= 0;
             const float inv = 1.0f / ll[u];
             uint2 y = make_uint2(0, 0);
-            if (sees) y = make_uint2(pack2<F16>(acc[u].x * inv, acc[u].y * inv), pack2<F16>(acc[u].z * inv, acc[u].w * inv));
+            if (sees) y = make_uint2(pack_out(f16, acc[u].x * inv, acc[u].y * inv), pack_out(f16, acc[u].z * inv, acc[u].w * inv));
             const int64_t otok = s.k.start + s.k.i0 + tk;
             uint16_t *d = static_cast<uint16_t *>(a.out) + otok * a.o_token + (int64_t)(s.h * G + hd) * a.o_head + 4 * c;
             if (a.o_vec) {
@@ -536,14 +563,14 @@ __device__ __noinline__ void store_unaligned(uint16_t *x, uint4 y) {
 // of its query tile, which is free by now, so that whole rows are stored a step),
 // or as a part ([channels / 4][row] float4: a step's stores are contiguous).  A's
 // threads add B's O where B shared their rows.  `off`: the row's output, as load_query's.
-template <int ND, bool F16>
+template <int ND>
 __device__ __noinline__ void store_rows(const PagesAttn &a, const Seg &s, unsigned char *tile, uint32_t cO, int row0,
                                         int r0, int64_t off, bool sees, float m, float l, float fa, float fb) {
     constexpr int D = 32 * ND;
     const int lane = threadIdx.x & 31, row = row0 + lane;
     const float inv = sees ? 1.0f / l : 0.0f;
     float4 *part = reinterpret_cast<float4 *>(a.part + (int64_t)s.part * kPartFloats(D)) + r0 + row;
-    const bool whole = s.whole, dual = s.dual;
+    const bool whole = s.whole, dual = s.dual, f16 = a.dtype == kF16;
     if (whole) fa *= inv, fb *= inv;
 #pragma unroll 1
     for (int c = 0; c < D; c += 16) {
@@ -567,8 +594,8 @@ __device__ __noinline__ void store_rows(const PagesAttn &a, const Seg &s, unsign
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint4 y =
-                    make_uint4(pack2<F16>(o[8 * i], o[8 * i + 1]), pack2<F16>(o[8 * i + 2], o[8 * i + 3]),
-                               pack2<F16>(o[8 * i + 4], o[8 * i + 5]), pack2<F16>(o[8 * i + 6], o[8 * i + 7]));
+                    make_uint4(pack_out(f16, o[8 * i], o[8 * i + 1]), pack_out(f16, o[8 * i + 2], o[8 * i + 3]),
+                               pack_out(f16, o[8 * i + 4], o[8 * i + 5]), pack_out(f16, o[8 * i + 6], o[8 * i + 7]));
                 const int cc = c / 8 + i;
                 *reinterpret_cast<uint4 *>(tile + (cc >> 3) * kPanel + row * 128 + (((cc & 7) ^ (row & 7)) << 4)) =
                     sees ? y : make_uint4(0, 0, 0, 0);
@@ -636,25 +663,102 @@ __device__ __noinline__ void load_query(const PagesAttn &a, unsigned char *tile,
     }
 }
 
+// The same for codes: rows in f16 times 2^-exponent (exact, unless an element lies
+// 2^-28 below the row's largest), exponents to `exps`.
+template <int ND>
+__device__ __noinline__ void load_query_scaled(const PagesAttn &a, unsigned char *tile, int *exps, int row0, int64_t off) {
+    constexpr int D = 32 * ND, C = D / 8, L = C > 8 ? 16 : C > 4 ? 8 : 4, R = 32 / L;
+    constexpr int U = 32 / R < 4 ? 32 / R : 4;
+    const int lane = threadIdx.x & 31, c = lane % L, sub = lane / L;
+    const uint16_t *q = static_cast<const uint16_t *>(a.q) + 8 * c;
+    const bool f16 = a.dtype == kF16;
+    unsigned char *dst = tile + (c >> 3) * kPanel;
+#pragma unroll 1
+    for (int i0 = 0; i0 < 32; i0 += R * U) {
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t o = __shfl_sync(0xffffffffu, (long long)off, i0 + R * u + sub);
+            v[u] = make_uint4(0, 0, 0, 0);
+            if (o >= 0 && c < C) {
+                if (a.q_vec) v[u] = __ldg(reinterpret_cast<const uint4 *>(q + o));
+                else v[u] = load_unaligned(q + o);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = row0 + i0 + R * u + sub;
+            const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+            float x[8], m = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                x[k] = unpack(f16, (uint16_t)(w[k / 2] >> (16 * (k & 1))));
+                m = fmaxf(m, fabsf(x[k]));
+            }
+#pragma unroll
+            for (int k = 1; k < L; k <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+            const int e = f16_exponent(m); // an infinite row stays infinite
+            const float f = exp2i(-e) * a.qsign;
+            if (c < C)
+                *reinterpret_cast<uint4 *>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+                    make_uint4(pack2<true>(x[0] * f, x[1] * f), pack2<true>(x[2] * f, x[3] * f),
+                               pack2<true>(x[4] * f, x[5] * f), pack2<true>(x[6] * f, x[7] * f));
+            if (c == 0) exps[r] = e;
+        }
+    }
+}
+
+// 16 codes (4 or 2 words) -> f16 values fma(c, scale, zero), with centre = zero +
+// 2^(BITS-1) scale and c - 2^(BITS-1) exact in fp32 (the code in the mantissa of
+// 2^23, less 2^23 + 2^(BITS-1)); one rounding to f16.
+template <int BITS> __device__ __forceinline__ void dequant16(const uint32_t *w, float scale, float centre, uint32_t (&o)[8]) {
+    constexpr float bias = -8388608.0f - (float)(1 << (BITS - 1));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { // four codes
+        float x[4];
+        uint32_t b;
+        if constexpr (BITS == 8) {
+            b = w[i];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = __uint_as_float(__byte_perm(b, 0x4B000000u, 0x7440u | k));
+        } else {
+            b = w[i / 2] >> (16 * (i & 1));
+            const uint32_t ev = b & 0x0f0fu, od = b >> 4 & 0x0f0fu; // codes 0, 2 and 1, 3 in bytes 0, 1
+            x[0] = __uint_as_float(__byte_perm(ev, 0x4B000000u, 0x7440u)), x[1] = __uint_as_float(__byte_perm(od, 0x4B000000u, 0x7440u));
+            x[2] = __uint_as_float(__byte_perm(ev, 0x4B000000u, 0x7441u)), x[3] = __uint_as_float(__byte_perm(od, 0x4B000000u, 0x7441u));
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+            add2(x[k], x[k + 1], bias, bias);
+            fma2s(x[k], x[k + 1], scale, centre);
+            o[2 * i + k / 2] = pack2<true>(x[k], x[k + 1]);
+        }
+    }
+}
+
 // n low bits set (n may lie outside 0 .. 32)
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 
-template <int ND, bool F16>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int BITS, int ND, bool F16>
+__global__ void __launch_bounds__(threads_of(BITS), 1)
     pages_chunk_kernel(const __grid_constant__ PagesAttn a, int TB, int min_per, int *counters, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
     constexpr int D = 32 * ND, NP = (ND + 1) / 2; // channels, 64-channel panels
+    constexpr int kThreads = threads_of(BITS), kStages = stages_of(BITS);
+    constexpr bool kCodes = BITS < 16;
+    static_assert(!kCodes || F16, "codes become f16 operands");
     extern __shared__ unsigned char raw[];
     unsigned char *sm = raw + ((1024 - (su32(raw) & 1023)) & 1023);
     unsigned char *sq = sm, *ring = sm + 2 * NP * kPanel;
     Shared &sh = *reinterpret_cast<Shared *>(ring + kStages * NP * kPanel);
+    SharedCodes &sc = *reinterpret_cast<SharedCodes *>(ring + kStages * NP * kPanel + sizeof(Shared)); // codes alone
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PagesStore &st = a.st;
     const int H = st.H, G = a.G;
     unsigned int *status = st.status;
     if (tid == 0) {
         sh.args = a;
-        for (int i = 0; i < kStages; ++i) bar_init(&sh.full[i], 1), bar_init(&sh.empty[i], 1);
+        for (int i = 0; i < kStages; ++i) bar_init(&sh.full[i], kCodes ? 4 : 1), bar_init(&sh.empty[i], 1);
         for (int x = 0; x < 2; ++x) {
             bar_init(&sh.q_full[x], 4);
             bar_init(&sh.s_full[x], 1);
@@ -662,9 +766,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             bar_init(&sh.p_full[x], 4);
             bar_init(&sh.o_full[x], 1);
         }
-        for (int i = 0; i < kSegs; ++i) bar_init(&sh.seg_full[i], 1), bar_init(&sh.seg_empty[i], kReaders);
+        for (int i = 0; i < kSegs; ++i) bar_init(&sh.seg_full[i], 1), bar_init(&sh.seg_empty[i], readers_of(BITS));
         for (int i = 0; i < 4; ++i) bar_init(&sh.edge[i], 1), bar_init(&sh.half[i], 1);
         bar_init(&sh.meet, kSoft);
+        for (int i = 0; i < 4; ++i) bar_init(&sh.range[i], 4);
+        bar_init(&sh.conv, 4);
         bar_init(&sh.drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -674,7 +780,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (warp == kCopyWarp && lane == 0) {
+    if (!kCodes && warp == kCopyWarp && lane == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
     }
@@ -774,20 +880,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
 
     // A softmax thread holds a row's 128 scores.  Its spills would go to L2 (shared
-    // memory leaves almost no L1), so the registers move to where they are needed:
-    // 256 kSoftRegs + 128 kRoleRegs of the block's 384 x 168.
-    static_assert(256 * kSoftRegs + 128 * kRoleRegs <= kThreads * 168, "register split");
+    // memory leaves almost no L1), so the registers move to where they are needed.
+    static_assert(256 * soft_regs(BITS) + (kThreads - 256) * role_regs(BITS) <= 65536 / kThreads / 8 * 8 * kThreads, "register split");
     if (warp < kSoft)
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(soft_regs(BITS)));
     else
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(role_regs(BITS)));
     if (warp < kSoft) {
         // ------------------------------------------------------------ softmax
         const int X = warp >> 2;   // A or B
         const int row = tid & 127; // tensor-memory lane
         const uint32_t lanes = tm + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t cS = lanes + kColS + 128 * X, cO = lanes + kColO + 128 * X;
-        const float crow = a.scale * 1.4426950408889634f;
+        const float c2 = a.scale * 1.4426950408889634f;
         uint32_t ns = 0, no = 0, met = 0; // tiles, blocks, meetings so far
         auto meet = [&]() { // of the softmax warps
             tc_before();
@@ -810,10 +915,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             float m = -INFINITY, l = 0.0f;
             if (r0 < s.rows) {
                 // ---- the row's query, and an empty O
-                if (!(X && dual))
-                    load_query<ND>(sh.args, sq + X * NP * kPanel, row & ~31,
-                                   live ? (int64_t)(s.k.start + s.k.i0 + tok) * a.q_token + (int64_t)(s.h * G + head) * a.q_head
-                                        : -1);
+                const int64_t off = live ? (int64_t)(s.k.start + s.k.i0 + tok) * a.q_token + (int64_t)(s.h * G + head) * a.q_head : -1;
+                if (X && dual) {
+                } else if constexpr (kCodes) {
+                    load_query_scaled<ND>(sh.args, sq + X * NP * kPanel, sc.qexp + X * kRows, row & ~31, off);
+                } else {
+                    load_query<ND>(sh.args, sq + X * NP * kPanel, row & ~31, off);
+                }
                 {
                     const uint32_t z[16] = {};
 #pragma unroll 1
@@ -828,6 +936,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int n = dual ? s.n : nX;
             Tiles tl(a, s);
             uint32_t edges = s.edges; // edge tiles of the run up to this one
+            float crow = c2;          // a score's exp2 units
+            int eref = 0;             // O's exponent
+            bool began = false;
             for (int j = 0; j < n; ++j) {
                 const int T = tl.token(j);
                 const bool edge = tl.edge(T);
@@ -836,6 +947,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = warp_wait(&sh.s_full[X], ns & 1, status))) break;
                 ++ns;
                 tc_after();
+                int shift = 0; // of this tile's values against O's
+                bool raise = false;
+                float fo = 1.0f;
+                if constexpr (kCodes) {
+                    const uint32_t tile = s.item / 2 + j;
+                    if (!(ok = warp_wait(&sh.range[tile & 3], tile >> 2 & 1, status))) break;
+                    // B has A's queries where it shares its rows, loaded before the first S
+                    crow = c2 * exp2i(sc.qexp[(dual ? 0 : X * kRows) + row]) * exp2i(sc.kexp[tile & 3]);
+                    const int e = sc.vexp[tile & 3];
+                    if (!began || e > eref) {
+                        if (began) raise = true, fo = exp2i(eref - e);
+                        eref = e;
+                    }
+                    began = true;
+                    shift = e - eref;
+                }
                 if (any) {
                     float x[128];
                     tmem_ld64(cS, x);
@@ -861,10 +988,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float mx = max3(max3(max3(m4[0], x[124], x[125]), max3(m4[1], x[126], x[127]), m4[2]), m4[3], m4[3]) * crow;
                     // a NaN score makes the reference, and with it the row, NaN
                     const bool need = !(mx <= m + kLazy), move = need && m != -INFINITY;
-                    const float f = move ? ex2(m - mx) : 1.0f;
+                    float f = move ? ex2(m - mx) : 1.0f;
                     if (need) m = mx;
-                    if (__any_sync(0xffffffffu, move)) {
+                    if (raise || __any_sync(0xffffffffu, move)) {
                         l *= f;
+                        f *= fo;
                         // every O += P V of earlier tiles is complete: S of this one was issued after them
 #pragma unroll 1
                         for (int c = 0; c < D; c += 16) {
@@ -875,7 +1003,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             tmem_st16(cO + c, reinterpret_cast<const uint32_t *>(o));
                         }
                     }
-                    const float off = m == -INFINITY ? 0.0f : -m;
+                    const float off = (m == -INFINITY ? 0.0f : -m) + (kCodes ? (float)shift : 0.0f);
                     float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
 #pragma unroll
                     for (int hlf = 0; hlf < 2; ++hlf) {
@@ -902,13 +1030,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                             if (lane == 0 && !edge) bar_arrive(&sh.h_full[X]);
                         }
                     }
-                    l += (a0 + a1) + (a2 + a3);
+                    const float sum = (a0 + a1) + (a2 + a3);
+                    l += kCodes ? sum * exp2i(-shift) : sum;
                 }
                 if (edge) { // the tile's V has been through the fixing warps
                     const uint32_t it = s.item + 2 * j + 1;
                     if (!(ok = warp_wait(&sh.full[it % kStages], (it / kStages) & 1, status))) break;
                     const uint32_t *fl = sh.flags[(edges - 1) & 3];
-                    if (fl[0] | fl[1] | fl[2] | fl[3]) add_unfinite<ND, F16>(sh.args, fl, s.k.b, s.h, T, p, lo, cO);
+                    if (fl[0] | fl[1] | fl[2] | fl[3]) add_unfinite<BITS, ND, F16>(sh.args, fl, s.k.b, s.h, T, p, lo, cO);
                 }
                 st_wait();
                 tc_before();
@@ -921,22 +1050,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ---- the rows out
             if (ok && nX > 0) ok = warp_wait(&sh.o_full[X], no++ & 1, status);
             tc_after();
-            float fa = 1.0f, fb = 0.0f;
+            float fa = kCodes ? exp2i(eref) : 1.0f, fb = 0.0f;
             if (dual) {
                 float2 *ml = reinterpret_cast<float2 *>(sq + NP * kPanel); // B's query tile is not in use
-                if (X) ml[row] = make_float2(m, l);
+                float *fx = reinterpret_cast<float *>(ml + kRows);
+                if (X) ml[row] = make_float2(m, l), fx[row] = fa;
                 if (!(ok = ok && meet())) break;
                 if (!X) {
                     const float2 y = ml[row];
                     const float nm = fmaxf(m, y.x), ref = nm == -INFINITY ? 0.0f : nm;
-                    fa = ex2(m - ref), fb = ex2(y.x - ref);
+                    const float wa = ex2(m - ref), wb = ex2(y.x - ref);
+                    fa *= wa, fb = fx[row] * wb;
                     m = nm;
-                    l = l * fa + y.y * fb;
+                    l = l * wa + y.y * wb;
                 }
             }
             if (!ok) break;
             if (any && !(X && dual))
-                store_rows<ND, F16>(sh.args, s, sq + X * NP * kPanel, cO, row & ~31, r0,
+                store_rows<ND>(sh.args, s, sq + X * NP * kPanel, cO, row & ~31, r0,
                                     live ? (int64_t)(s.k.start + s.k.i0 + tok) * a.o_token + (int64_t)(s.h * G + head) * a.o_head
                                          : -1,
                                     p >= 0, m, l, fa, fb);
@@ -951,7 +1082,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = meet())) break;
                 if (sh.last) {
                     __threadfence();
-                    join_parts<ND, F16>(sh.args, s);
+                    join_parts<ND>(sh.args, s);
                 }
             }
             if (dual && !(ok = meet())) break; // B's O and (m, l) are read
@@ -1061,6 +1192,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 asm volatile("prefetch.global.L2 [%0];" ::"l"(q) : "memory");
                 if constexpr (D > 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + 64) : "memory");
             }
+            if constexpr (kCodes) { // the converting warps fetch their own
+                for (int j = 0; j < s.n; ++j) ne += tile_edge(a, k, tile_token(k, s.t0 + j));
+                item += 2 * s.n;
+                more = walk_next(a, TB, w);
+                continue;
+            }
             for (int j = 0; ok && j < s.n; ++j) {
                 const int T = tile_token(k, s.t0 + j), t = T + piece * box;
                 // a box is needed if some row sees one of its tokens
@@ -1084,10 +1221,123 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (ok) more = walk_next(a, TB, w);
         }
         // no copy outlives the CTA
-        for (int i = 0; i < kStages && (uint32_t)i < item; ++i) {
+        for (int i = 0; !kCodes && i < kStages && (uint32_t)i < item; ++i) {
             const uint32_t it = item - 1 - i;
             warp_wait(&sh.full[it % kStages], (it / kStages) & 1, status);
         }
+    } else if (kCodes && warp >= kConvWarp) {
+        // ------------------------------------------------------------ codes to operand tiles
+        // Thread ct owns token ct's parameters; of the codes it takes 16 channels of every
+        // (128 / LP)-th token, and fetches its next ones as it converts these.
+        constexpr int LP = ND > 2 ? 8 : ND == 2 ? 4 : 2, RPI = kTok / LP, W = BITS == 8 ? 4 : 2;
+        const int ct = tid - 32 * kConvWarp, cw = warp - kConvWarp, piece = ct % LP, sub = ct / LP;
+        const bool mine = piece < 2 * ND;
+        uint32_t code[LP][W];
+        int pages = -1;                       // lane i: of tokens 16 i .. of the tile, i < 8
+        float2 kp, vp;                        // parameters of token ct
+        uint32_t met = 0;
+        auto lookup = [&](const Seg &s, int T) {
+            const int t = T + 16 * lane;
+            const bool any = lane < 8 && t <= s.k.p1 && (t + 16 > s.k.lo || t < a.sinks);
+            return any ? max(pages_page(a.b, st, s.k.b, t), 0) : -1;
+        };
+        auto fetch = [&](const Seg &s, bool v, int T, int pgs, int i) {
+            const int r = sub + RPI * i, pg = __shfl_sync(0xffffffffu, pgs, r >> 4);
+#pragma unroll
+            for (int k = 0; k < W; ++k) code[i][k] = 0;
+            if (pg >= 0 && mine) {
+                const unsigned char *q = (v ? st.v : st.k) + pages_row(st, pg, s.h, T + r) * (D * BITS / 8) + piece * (2 * BITS);
+                if constexpr (BITS == 8) {
+                    const uint4 x = __ldg(reinterpret_cast<const uint4 *>(q));
+                    code[i][0] = x.x, code[i][1] = x.y, code[i][2] = x.z, code[i][3] = x.w;
+                } else {
+                    const uint2 x = __ldg(reinterpret_cast<const uint2 *>(q));
+                    code[i][0] = x.x, code[i][1] = x.y;
+                }
+            }
+        };
+        auto params = [&](const Seg &s, int T, int pgs) {
+            const int pg = __shfl_sync(0xffffffffu, pgs, ct >> 4);
+            kp = vp = make_float2(0.0f, 0.0f);
+            if (pg >= 0 && token_seen(a, s.k, T + ct)) {
+                const int64_t r = pages_row(st, pg, s.h, T + ct);
+                kp = __ldg(st.kp + r), vp = __ldg(st.vp + r);
+            }
+        };
+        while (ok && next_seg()) {
+            const Seg &s = *sp;
+            uint32_t ne = s.edges;
+            int T = tile_token(s.k, s.t0);
+            pages = lookup(s, T);
+            params(s, T, pages);
+#pragma unroll
+            for (int i = 0; i < LP; ++i) fetch(s, false, T, pages, i);
+            for (int j = 0; ok && j < s.n; ++j) {
+                const uint32_t tile = s.item / 2 + j, it = s.item + 2 * j;
+                const bool edge = tile_edge(a, s.k, T);
+                // ---- the tile's range: |value| <= max(|zero|, |zero + levels scale|)
+                constexpr float levels = (float)((1 << BITS) - 1), half = (float)(1 << (BITS - 1));
+                const float kb = fmaxf(fabsf(kp.y), fabsf(fmaf(levels, kp.x, kp.y)));
+                const float vb = fmaxf(fabsf(vp.y), fabsf(fmaf(levels, vp.x, vp.y)));
+                const bool kf = isfinite(kb) && isfinite(kp.x), vf = isfinite(vb) && isfinite(vp.x);
+                const uint32_t km = __reduce_max_sync(0xffffffffu, kf ? __float_as_uint(kb) : 0u);
+                const uint32_t vm = __reduce_max_sync(0xffffffffu, vf ? __float_as_uint(vb) : 0u);
+                const uint32_t bad = __ballot_sync(0xffffffffu, !vf);
+                if (lane == 0) {
+                    sc.most[tile & 1][cw][0] = __uint_as_float(km), sc.most[tile & 1][cw][1] = __uint_as_float(vm);
+                    if (edge) sh.flags[ne & 3][cw] = bad;
+                }
+                sc.token[tile & 1][ct] = make_float4(kp.x, fmaf(half, kp.x, kp.y), edge && !vf ? 0.0f : vp.x,
+                                                     edge && !vf ? 0.0f : fmaf(half, vp.x, vp.y));
+                __syncwarp();
+                if (lane == 0) bar_arrive(&sh.conv);
+                if (!(ok = warp_wait(&sh.conv, met++ & 1, status))) break;
+                float kmost = 0.0f, vmost = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) kmost = fmaxf(kmost, sc.most[tile & 1][i][0]), vmost = fmaxf(vmost, sc.most[tile & 1][i][1]);
+                const int ke = f16_exponent(kmost), ve = f16_exponent(vmost);
+                if (ct == 0) sc.kexp[tile & 3] = ke, sc.vexp[tile & 3] = ve;
+                __syncwarp();
+                if (lane == 0) bar_arrive(&sh.range[tile & 3]);
+                const float kf2 = exp2i(-ke), vf2 = exp2i(-ve);
+                const bool more = j + 1 < s.n;
+                const int Tn = more ? tile_token(s.k, s.t0 + j + 1) : T;
+                const int pn = more ? lookup(s, Tn) : -1;
+#pragma unroll 1
+                for (int v = 0; v < 2; ++v) {
+                    const uint32_t item = it + v, slot = item % kStages;
+                    if (v == 1 && more) params(s, Tn, pn);
+                    if (item >= kStages && !(ok = warp_wait(&sh.empty[slot], (item / kStages - 1) & 1, status))) break;
+                    unsigned char *dst = ring + slot * (NP * kPanel);
+                    const float f = v ? vf2 : kf2;
+#pragma unroll
+                    for (int i = 0; i < LP; ++i) {
+                        const int r = sub + RPI * i;
+                        const float4 q = sc.token[tile & 1][r];
+                        uint32_t o[8];
+                        dequant16<BITS>(code[i], (v ? q.z : q.x) * f, (v ? q.w : q.y) * f, o);
+                        if (v == 0) fetch(s, true, T, pages, i);
+                        else fetch(s, false, Tn, pn, i);
+                        if (mine) {
+                            // (the two panels' lanes store their halves in opposite order: no bank conflicts)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                const int e = u ^ (piece >> 2 & 1), c = 2 * piece + e;
+                                *reinterpret_cast<uint4 *>(dst + (c >> 3) * kPanel + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+                                    e ? make_uint4(o[4], o[5], o[6], o[7]) : make_uint4(o[0], o[1], o[2], o[3]);
+                            }
+                        }
+                    }
+                    proxy_fence();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&sh.full[slot]);
+                }
+                ne += edge;
+                T = Tn, pages = pn;
+            }
+        }
+    } else if (kCodes) {
+        // two warps of the group have no role
     } else {
         // ------------------------------------------------------------ V rows of edge tiles
         while (ok && next_seg()) {
@@ -1142,27 +1392,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-template <int ND, bool F16> cudaError_t launch_chunk(const PagesAttn &a, int sms, cudaStream_t s) {
+template <int BITS, int ND, bool F16> cudaError_t launch_chunk(const PagesAttn &a, int sms, cudaStream_t s) {
     static bool configured[64] = {false};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-        e = cudaFuncSetAttribute(pages_chunk_kernel<ND, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes((ND + 1) / 2));
+        e = cudaFuncSetAttribute(pages_chunk_kernel<BITS, ND, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(BITS, (ND + 1) / 2));
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
     int *counters = reinterpret_cast<int *>(a.part + a.part_floats) - kPagesCounters;
     const int TB = 2 * kRows / a.G;
-    return launch_pdl(pages_chunk_kernel<ND, F16>, dim3((unsigned)sms), dim3(kThreads), smem_bytes((ND + 1) / 2), s, true, a, TB, 2,
+    return launch_pdl(pages_chunk_kernel<BITS, ND, F16>, dim3((unsigned)sms), dim3(threads_of(BITS)), smem_bytes(BITS, (ND + 1) / 2), s, true, a, TB, 2,
                       counters, a.maps->k, a.maps->v);
+}
+
+template <int BITS, bool F16> cudaError_t by_dim(const PagesAttn &a, int sms, cudaStream_t s) {
+    switch (a.st.D) {
+    case 32: return launch_chunk<BITS, 1, F16>(a, sms, s);
+    case 64: return launch_chunk<BITS, 2, F16>(a, sms, s);
+    case 96: return launch_chunk<BITS, 3, F16>(a, sms, s);
+    default: return launch_chunk<BITS, 4, F16>(a, sms, s);
+    }
 }
 
 } // namespace
 
 // Blocks of at least one token: up to 256 query heads per kv head.  The batch's
 // prefix lies in shared memory while the list is built.
-bool pages_chunk_supported(const PagesAttn &a) { return a.st.bits == 16 && a.G <= 2 * kRows && a.b.batch <= 16384; }
+bool pages_chunk_supported(const PagesAttn &a) { return a.G <= 2 * kRows && a.b.batch <= 16384; }
 
 int64_t pages_chunk_scratch(int D, int sms) { return (int64_t)sms * 2 * kPartFloats(D); }
 
@@ -1176,12 +1435,8 @@ cudaError_t launch_pages_chunk(const PagesAttn &a, cudaStream_t s) {
     ProfScope prof("pages_chunk", s);
     count_launch();
     const bool f16 = a.dtype == kF16;
-    switch (a.st.D) {
-    case 32: return f16 ? launch_chunk<1, true>(a, sms, s) : launch_chunk<1, false>(a, sms, s);
-    case 64: return f16 ? launch_chunk<2, true>(a, sms, s) : launch_chunk<2, false>(a, sms, s);
-    case 96: return f16 ? launch_chunk<3, true>(a, sms, s) : launch_chunk<3, false>(a, sms, s);
-    default: return f16 ? launch_chunk<4, true>(a, sms, s) : launch_chunk<4, false>(a, sms, s);
-    }
+    if (a.st.bits == 16) return f16 ? by_dim<16, true>(a, sms, s) : by_dim<16, false>(a, sms, s);
+    return a.st.bits == 8 ? by_dim<8, true>(a, sms, s) : by_dim<4, true>(a, sms, s);
 }
 
 // Tensor maps over 16-bit pages: rows of D elements, boxes of one page's tokens
