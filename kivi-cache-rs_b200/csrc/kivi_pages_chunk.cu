@@ -46,7 +46,7 @@ constexpr int kTok = 128;                 // cached tokens per tile
 constexpr int kRows = 128;                // rows of one row tile
 constexpr int kSoft = 8;                  // softmax warps
 constexpr int kMmaWarp = 8, kCopyWarp = 9, kFixWarp = 10; // and 11
-constexpr int kConvWarp = 12;             // codes: 12-15 convert
+constexpr int kConvWarp = 10, kConv = 6; // codes: 10-15 convert
 __host__ __device__ constexpr int threads_of(int bits) { return bits == 16 ? 384 : 512; }
 // K and V tiles in flight
 __host__ __device__ constexpr int stages_of(int bits) { return bits == 16 ? 5 : 4; }
@@ -55,8 +55,8 @@ constexpr long long kWait = 2000000000LL; // ~1 s
 constexpr float kLazy = 8.0f;
 constexpr int kPolyPairs = 1;             // of every four pairs of weights, on the FMA pipe
 // registers of a softmax thread and of the others
-__host__ __device__ constexpr int soft_regs(int bits) { return bits == 16 ? 200 : 176; }
-__host__ __device__ constexpr int role_regs(int bits) { return bits == 16 ? 96 : 80; }
+__host__ __device__ constexpr int soft_regs(int bits) { return bits == 16 ? 200 : 144; }
+__host__ __device__ constexpr int role_regs(int bits) { return bits == 16 ? 96 : 112; }
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0, kColO = 256; // + 128 for B
 
@@ -416,7 +416,7 @@ __device__ __forceinline__ bool token_seen(const PagesAttn &a, const Block &k, i
 
 constexpr int kSegs = 4;     // segments published ahead
 // warps that read them: softmax, MMA, and those that touch the operand tiles
-__host__ __device__ constexpr int readers_of(int bits) { return kSoft + 1 + (bits == 16 ? 2 : 4); }
+__host__ __device__ constexpr int readers_of(int bits) { return kSoft + 1 + (bits == 16 ? 2 : kConv); }
 struct Shared {
     uint64_t full[5], empty[5]; // stages_of(bits) in use
     uint64_t seg_full[kSegs], seg_empty[kSegs];
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
     unsigned int *status = st.status;
     if (tid == 0) {
         sh.args = a;
-        for (int i = 0; i < kStages; ++i) bar_init(&sh.full[i], kCodes ? 4 : 1), bar_init(&sh.empty[i], 1);
+        for (int i = 0; i < kStages; ++i) bar_init(&sh.full[i], kCodes ? kConv : 1), bar_init(&sh.empty[i], 1);
         for (int x = 0; x < 2; ++x) {
             bar_init(&sh.q_full[x], 4);
             bar_init(&sh.s_full[x], 1);
@@ -769,8 +769,8 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
         for (int i = 0; i < kSegs; ++i) bar_init(&sh.seg_full[i], 1), bar_init(&sh.seg_empty[i], readers_of(BITS));
         for (int i = 0; i < 4; ++i) bar_init(&sh.edge[i], 1), bar_init(&sh.half[i], 1);
         bar_init(&sh.meet, kSoft);
-        for (int i = 0; i < 4; ++i) bar_init(&sh.range[i], 4);
-        bar_init(&sh.conv, 4);
+        for (int i = 0; i < 4; ++i) bar_init(&sh.range[i], 1);
+        bar_init(&sh.conv, kConv);
         bar_init(&sh.drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -964,28 +964,43 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                     shift = e - eref;
                 }
                 if (any) {
-                    float x[128];
-                    tmem_ld64(cS, x);
-                    tmem_ld64(cS + 64, x + 64);
-                    if (edge) {
+                    // The row's scores; with codes, whose converting warps take a share of the
+                    // registers, the second 64 are read again for their weights.
+                    float x[kCodes ? 64 : 128];
+                    auto hide = [&](float *z, int base) { // of 32 tokens from base, those out of sight
+                        const uint32_t see = low_bits(p + 1 - base) & (~low_bits(lo - base) | low_bits(a.sinks - base));
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const int base = T + 32 * q;
-                            const uint32_t see = low_bits(p + 1 - base) & (~low_bits(lo - base) | low_bits(a.sinks - base));
+                        for (int i = 0; i < 32; ++i) z[i] = see >> i & 1u ? z[i] : -INFINITY;
+                    };
+                    float m4[4];
+                    auto most = [&](const float *z) { // 32 more
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                x[32 * q + i] = see >> i & 1u ? x[32 * q + i] : -INFINITY;
+                        for (int i = 0; i < 32; i += 8) {
+                            m4[0] = max3(m4[0], z[i], z[i + 1]);
+                            m4[1] = max3(m4[1], z[i + 2], z[i + 3]);
+                            m4[2] = max3(m4[2], z[i + 4], z[i + 5]);
+                            m4[3] = max3(m4[3], z[i + 6], z[i + 7]);
                         }
-                    }
-                    float m4[4] = {x[0], x[1], x[2], x[3]};
+                    };
+                    tmem_ld64(cS, x);
+                    if (edge) hide(x, T), hide(x + 32, T + 32);
 #pragma unroll
-                    for (int i = 4; i < 124; i += 8) {
-                        m4[0] = max3(m4[0], x[i], x[i + 1]);
-                        m4[1] = max3(m4[1], x[i + 2], x[i + 3]);
-                        m4[2] = max3(m4[2], x[i + 4], x[i + 5]);
-                        m4[3] = max3(m4[3], x[i + 6], x[i + 7]);
+                    for (int i = 0; i < 4; ++i) m4[i] = x[i];
+                    most(x), most(x + 32);
+                    if constexpr (kCodes) {
+#pragma unroll
+                        for (int c = 64; c < 128; c += 32) {
+                            float z[32];
+                            tmem_ld32(cS + c, z);
+                            if (edge) hide(z, T + c);
+                            most(z);
+                        }
+                    } else {
+                        tmem_ld64(cS + 64, x + 64);
+                        if (edge) hide(x + 64, T + 64), hide(x + 96, T + 96);
+                        most(x + 64), most(x + 96);
                     }
-                    const float mx = max3(max3(max3(m4[0], x[124], x[125]), max3(m4[1], x[126], x[127]), m4[2]), m4[3], m4[3]) * crow;
+                    const float mx = max3(max3(m4[0], m4[1], m4[2]), m4[3], m4[3]) * crow;
                     // a NaN score makes the reference, and with it the row, NaN
                     const bool need = !(mx <= m + kLazy), move = need && m != -INFINITY;
                     float f = move ? ex2(m - mx) : 1.0f;
@@ -1008,9 +1023,13 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
 #pragma unroll
                     for (int hlf = 0; hlf < 2; ++hlf) {
                         uint32_t pk[32];
+                        if (kCodes && hlf) {
+                            tmem_ld64(cS + 64, x);
+                            if (edge) hide(x, T + 64), hide(x + 32, T + 96);
+                        }
 #pragma unroll
                         for (int i = 0; i < 64; i += 8) {
-                            float *y = x + 64 * hlf + i;
+                            float *y = x + (kCodes ? 0 : 64 * hlf) + i;
 #pragma unroll
                             for (int q = 0; q < 8; q += 2) {
                                 fma2s(y[q], y[q + 1], crow, off);
@@ -1227,26 +1246,29 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
         }
     } else if (kCodes && warp >= kConvWarp) {
         // ------------------------------------------------------------ codes to operand tiles
-        // Thread ct owns token ct's parameters; of the codes it takes 16 channels of every
-        // (128 / LP)-th token, and fetches its next ones as it converts these.
-        constexpr int LP = ND > 2 ? 8 : ND == 2 ? 4 : 2, RPI = kTok / LP, W = BITS == 8 ? 4 : 2;
+        // Of the 192 threads ct, the first 128 own a token's parameters; of the codes each
+        // takes 16 channels of every RPI-th token, and fetches its next ones as it converts
+        // these.
+        constexpr int LP = ND > 2 ? 8 : ND == 2 ? 4 : 2, RPI = 32 * kConv / LP, N = (kTok + RPI - 1) / RPI;
+        constexpr int W = BITS == 8 ? 4 : 2, ROW = D * BITS / 8;
         const int ct = tid - 32 * kConvWarp, cw = warp - kConvWarp, piece = ct % LP, sub = ct / LP;
         const bool mine = piece < 2 * ND;
-        uint32_t code[LP][W];
-        int pages = -1;                       // lane i: of tokens 16 i .. of the tile, i < 8
-        float2 kp, vp;                        // parameters of token ct
+        uint32_t code[N][W];
+        float2 kp, vp; // parameters of token ct
         uint32_t met = 0;
+        // lane i < 8: row number of token 16 i of the tile, -1 where nobody sees the 16
         auto lookup = [&](const Seg &s, int T) {
             const int t = T + 16 * lane;
             const bool any = lane < 8 && t <= s.k.p1 && (t + 16 > s.k.lo || t < a.sinks);
-            return any ? max(pages_page(a.b, st, s.k.b, t), 0) : -1;
+            return any ? (int)pages_row(st, max(pages_page(a.b, st, s.k.b, t), 0), s.h, t) : -1;
         };
-        auto fetch = [&](const Seg &s, bool v, int T, int pgs, int i) {
-            const int r = sub + RPI * i, pg = __shfl_sync(0xffffffffu, pgs, r >> 4);
+        const int shift = piece * (2 * BITS);
+        auto fetch = [&](bool v, int rows, int i) {
+            const int r = sub + RPI * i, base = __shfl_sync(0xffffffffu, rows, r >> 4 & 7);
 #pragma unroll
             for (int k = 0; k < W; ++k) code[i][k] = 0;
-            if (pg >= 0 && mine) {
-                const unsigned char *q = (v ? st.v : st.k) + pages_row(st, pg, s.h, T + r) * (D * BITS / 8) + piece * (2 * BITS);
+            if (base >= 0 && mine && r < kTok) {
+                const unsigned char *q = (v ? st.v : st.k) + (int64_t)(base + (r & 15)) * ROW + shift;
                 if constexpr (BITS == 8) {
                     const uint4 x = __ldg(reinterpret_cast<const uint4 *>(q));
                     code[i][0] = x.x, code[i][1] = x.y, code[i][2] = x.z, code[i][3] = x.w;
@@ -1256,22 +1278,21 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                 }
             }
         };
-        auto params = [&](const Seg &s, int T, int pgs) {
-            const int pg = __shfl_sync(0xffffffffu, pgs, ct >> 4);
+        auto params = [&](const Seg &s, int T, int rows) {
+            const int base = __shfl_sync(0xffffffffu, rows, ct >> 4 & 7);
             kp = vp = make_float2(0.0f, 0.0f);
-            if (pg >= 0 && token_seen(a, s.k, T + ct)) {
-                const int64_t r = pages_row(st, pg, s.h, T + ct);
-                kp = __ldg(st.kp + r), vp = __ldg(st.vp + r);
+            if (ct < kTok && base >= 0 && token_seen(a, s.k, T + ct)) {
+                kp = __ldg(st.kp + base + (ct & 15)), vp = __ldg(st.vp + base + (ct & 15));
             }
         };
         while (ok && next_seg()) {
             const Seg &s = *sp;
             uint32_t ne = s.edges;
             int T = tile_token(s.k, s.t0);
-            pages = lookup(s, T);
-            params(s, T, pages);
+            int rows = lookup(s, T);
+            params(s, T, rows);
 #pragma unroll
-            for (int i = 0; i < LP; ++i) fetch(s, false, T, pages, i);
+            for (int i = 0; i < N; ++i) fetch(false, rows, i);
             for (int j = 0; ok && j < s.n; ++j) {
                 const uint32_t tile = s.item / 2 + j, it = s.item + 2 * j;
                 const bool edge = tile_edge(a, s.k, T);
@@ -1283,12 +1304,13 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                 const uint32_t km = __reduce_max_sync(0xffffffffu, kf ? __float_as_uint(kb) : 0u);
                 const uint32_t vm = __reduce_max_sync(0xffffffffu, vf ? __float_as_uint(vb) : 0u);
                 const uint32_t bad = __ballot_sync(0xffffffffu, !vf);
-                if (lane == 0) {
+                if (lane == 0 && cw < 4) {
                     sc.most[tile & 1][cw][0] = __uint_as_float(km), sc.most[tile & 1][cw][1] = __uint_as_float(vm);
                     if (edge) sh.flags[ne & 3][cw] = bad;
                 }
-                sc.token[tile & 1][ct] = make_float4(kp.x, fmaf(half, kp.x, kp.y), edge && !vf ? 0.0f : vp.x,
-                                                     edge && !vf ? 0.0f : fmaf(half, vp.x, vp.y));
+                if (ct < kTok)
+                    sc.token[tile & 1][ct] = make_float4(kp.x, fmaf(half, kp.x, kp.y), edge && !vf ? 0.0f : vp.x,
+                                                         edge && !vf ? 0.0f : fmaf(half, vp.x, vp.y));
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.conv);
                 if (!(ok = warp_wait(&sh.conv, met++ & 1, status))) break;
@@ -1296,29 +1318,29 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) kmost = fmaxf(kmost, sc.most[tile & 1][i][0]), vmost = fmaxf(vmost, sc.most[tile & 1][i][1]);
                 const int ke = f16_exponent(kmost), ve = f16_exponent(vmost);
-                if (ct == 0) sc.kexp[tile & 3] = ke, sc.vexp[tile & 3] = ve;
-                __syncwarp();
-                if (lane == 0) bar_arrive(&sh.range[tile & 3]);
+                if (ct == 0) {
+                    sc.kexp[tile & 3] = ke, sc.vexp[tile & 3] = ve;
+                    bar_arrive(&sh.range[tile & 3]);
+                }
                 const float kf2 = exp2i(-ke), vf2 = exp2i(-ve);
                 const bool more = j + 1 < s.n;
                 const int Tn = more ? tile_token(s.k, s.t0 + j + 1) : T;
-                const int pn = more ? lookup(s, Tn) : -1;
+                const int rowsn = more ? lookup(s, Tn) : -1;
 #pragma unroll 1
                 for (int v = 0; v < 2; ++v) {
                     const uint32_t item = it + v, slot = item % kStages;
-                    if (v == 1 && more) params(s, Tn, pn);
+                    if (v == 1 && more) params(s, Tn, rowsn);
                     if (item >= kStages && !(ok = warp_wait(&sh.empty[slot], (item / kStages - 1) & 1, status))) break;
                     unsigned char *dst = ring + slot * (NP * kPanel);
                     const float f = v ? vf2 : kf2;
 #pragma unroll
-                    for (int i = 0; i < LP; ++i) {
+                    for (int i = 0; i < N; ++i) {
                         const int r = sub + RPI * i;
-                        const float4 q = sc.token[tile & 1][r];
+                        const float4 q = sc.token[tile & 1][r & (kTok - 1)];
                         uint32_t o[8];
                         dequant16<BITS>(code[i], (v ? q.z : q.x) * f, (v ? q.w : q.y) * f, o);
-                        if (v == 0) fetch(s, true, T, pages, i);
-                        else fetch(s, false, Tn, pn, i);
-                        if (mine) {
+                        fetch(v == 0, v ? rowsn : rows, i);
+                        if (mine && r < kTok) {
                             // (the two panels' lanes store their halves in opposite order: no bank conflicts)
 #pragma unroll
                             for (int u = 0; u < 2; ++u) {
@@ -1333,11 +1355,9 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                     if (lane == 0) bar_arrive(&sh.full[slot]);
                 }
                 ne += edge;
-                T = Tn, pages = pn;
+                T = Tn, rows = rowsn;
             }
         }
-    } else if (kCodes) {
-        // two warps of the group have no role
     } else {
         // ------------------------------------------------------------ V rows of edge tiles
         while (ok && next_seg()) {
