@@ -1256,27 +1256,34 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
         uint32_t code[N][W];
         float2 kp, vp; // parameters of token ct
         uint32_t met = 0;
-        // lane i < 8: row number of token 16 i of the tile, -1 where nobody sees the 16
+        // lane i < 8: page of tokens 16 i .. of the tile, -1 where nobody sees one of them;
+        // not looked at before rows_of, so that its load has time
         auto lookup = [&](const Seg &s, int T) {
             const int t = T + 16 * lane;
             const bool any = lane < 8 && t <= s.k.p1 && (t + 16 > s.k.lo || t < a.sinks);
-            return any ? (int)pages_row(st, max(pages_page(a.b, st, s.k.b, t), 0), s.h, t) : -1;
+            return any ? __ldg(a.b.table + (int64_t)s.k.b * a.b.table_stride + (t >> st.shift)) : -1;
         };
-        const int shift = piece * (2 * BITS);
+        auto rows_of = [&](const Seg &s, int T, int page) { // row number of token 16 i
+            const int t = T + 16 * lane;
+            const bool any = lane < 8 && t <= s.k.p1 && (t + 16 > s.k.lo || t < a.sinks);
+            if (any && (unsigned)page >= (unsigned)st.num_pages) {
+                atomicOr(status, kPagesBadPage);
+                page = 0;
+            }
+            return any ? (int)pages_row(st, page, s.h, t) : -1;
+        };
+        // Every lane loads, from some row of the store where there is nothing to load: a
+        // token that nobody sees has scale 0.
+        const int shift = min(piece, 2 * ND - 1) * (2 * BITS);
         auto fetch = [&](bool v, int rows, int i) {
             const int r = sub + RPI * i, base = __shfl_sync(0xffffffffu, rows, r >> 4 & 7);
-#pragma unroll
-            for (int k = 0; k < W; ++k) code[i][k] = 0;
-            if (base >= 0 && mine && r < kTok) {
-                const unsigned char *q = (v ? st.v : st.k) + (int64_t)(base + (r & 15)) * ROW + shift;
-                if constexpr (BITS == 8) {
-                    const uint4 x = __ldg(reinterpret_cast<const uint4 *>(q));
-                    code[i][0] = x.x, code[i][1] = x.y, code[i][2] = x.z, code[i][3] = x.w;
-                } else {
-                    const uint2 x = __ldg(reinterpret_cast<const uint2 *>(q));
-                    code[i][0] = x.x, code[i][1] = x.y;
-                }
-            }
+            const unsigned char *q = (v ? st.v : st.k) + (int64_t)(max(base, 0) + (r & 15)) * ROW + shift;
+            if constexpr (BITS == 8)
+                asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(code[i][0]), "=r"(code[i][1]), "=r"(code[i][2]), "=r"(code[i][W - 1])
+                             : "l"(q));
+            else
+                asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(code[i][0]), "=r"(code[i][1]) : "l"(q));
         };
         auto params = [&](const Seg &s, int T, int rows) {
             const int base = __shfl_sync(0xffffffffu, rows, ct >> 4 & 7);
@@ -1289,13 +1296,15 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
             const Seg &s = *sp;
             uint32_t ne = s.edges;
             int T = tile_token(s.k, s.t0);
-            int rows = lookup(s, T);
+            int rows = rows_of(s, T, lookup(s, T));
             params(s, T, rows);
 #pragma unroll
             for (int i = 0; i < N; ++i) fetch(false, rows, i);
             for (int j = 0; ok && j < s.n; ++j) {
                 const uint32_t tile = s.item / 2 + j, it = s.item + 2 * j;
-                const bool edge = tile_edge(a, s.k, T);
+                const bool edge = tile_edge(a, s.k, T), more = j + 1 < s.n;
+                const int Tn = more ? tile_token(s.k, s.t0 + j + 1) : T;
+                const int pagen = lookup(s, Tn);
                 // ---- the tile's range: |value| <= max(|zero|, |zero + levels scale|)
                 constexpr float levels = (float)((1 << BITS) - 1), half = (float)(1 << (BITS - 1));
                 const float kb = fmaxf(fabsf(kp.y), fabsf(fmaf(levels, kp.x, kp.y)));
@@ -1323,13 +1332,14 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                     bar_arrive(&sh.range[tile & 3]);
                 }
                 const float kf2 = exp2i(-ke), vf2 = exp2i(-ve);
-                const bool more = j + 1 < s.n;
-                const int Tn = more ? tile_token(s.k, s.t0 + j + 1) : T;
-                const int rowsn = more ? lookup(s, Tn) : -1;
+                int rowsn = -1;
 #pragma unroll 1
                 for (int v = 0; v < 2; ++v) {
                     const uint32_t item = it + v, slot = item % kStages;
-                    if (v == 1 && more) params(s, Tn, rowsn);
+                    if (v == 1) {
+                        rowsn = rows_of(s, Tn, pagen);
+                        params(s, Tn, rowsn);
+                    }
                     if (item >= kStages && !(ok = warp_wait(&sh.empty[slot], (item / kStages - 1) & 1, status))) break;
                     unsigned char *dst = ring + slot * (NP * kPanel);
                     const float f = v ? vf2 : kf2;
