@@ -39,21 +39,7 @@ __device__ __forceinline__ int find_sequence(const PagesBatch &b, int tok) {
     return lo;
 }
 
-// Eight consecutive elements at p, as floats.
-template <class E> __device__ __forceinline__ void load8(const E *p, bool vec, float (&x)[8]) {
-    if (vec) {
-        constexpr int W = sizeof(E) / 2; // 16-byte words
-        uint4 w[W];
-#pragma unroll
-        for (int i = 0; i < W; ++i) w[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
-        const E *e = reinterpret_cast<const E *>(w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f(e[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f(p[i]);
-    }
-}
+// Eight consecutive elements to p.
 template <class E> __device__ __forceinline__ void store8(E *p, bool vec, const float (&x)[8]) {
     if (vec) {
         constexpr int W = sizeof(E) / 2;
@@ -69,126 +55,281 @@ template <class E> __device__ __forceinline__ void store8(E *p, bool vec, const 
     }
 }
 
-// One row of D elements belongs to L = D / 8 rounded up to a power of two lanes,
-// eight elements each; a warp takes 32 / L of a token's 2 H rows (keys' heads,
-// then values').
-template <int BITS, int T>
-__global__ void __launch_bounds__(256) pages_write_kernel(PagesStore st, PagesBatch b, PagesDense x, int L,
-                                                          int wpt) {
-    using E = typename Elem<T>::type;
-    const int lane = threadIdx.x & 31;
-    const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int tok = (int)(w / wpt);
-    if (tok >= b.total) return;
-    const int r = (int)(w % wpt) * (32 / L) + lane / L; // row of the token
-    const int c = lane % L * 8;
-    const bool live = r < 2 * st.H && c < st.D;
-    const bool value = r >= st.H;
-    const int head = value ? r - st.H : r;
-    float e[8];
-    const float inf = INFINITY;
-    if (live)
-        load8(static_cast<const E *>(value ? x.v : x.k) + tok * x.token + head * x.head + c, x.vec, e);
+// 16 bytes of elements at p (8 of 16 bits, or one word of W for fp32), as loaded.
+template <class E> struct Raw {
+    static constexpr int W = sizeof(E) / 2;
+    uint4 w[W];
+    __device__ __forceinline__ void load(const E *p, bool vec) {
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) w[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+        } else {
+            E *e = reinterpret_cast<E *>(w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = p[i];
+        }
+    }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+        const E *e = reinterpret_cast<const E *>(w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f(e[i]);
+    }
+};
+
+// How a launch divides its work.  One row of D elements belongs to L = D / 8 rounded
+// up to a power of two lanes, eight elements each, so a warp step takes R = 32 / L of
+// a token's 2 H rows (keys' heads, then values').  A token is 2^log_parts warps',
+// which take its steps in turn: one warp where there are tokens enough, since finding
+// a token's sequence and page costs as much as a step; a warp for each step where
+// there are few and latency counts.
+struct Work {
+    int L, R, steps, log_parts;
+};
+constexpr int kAhead = 4; // steps whose loads are in flight at once
+
+// The token of this warp: its slot in the store, or false where it has none.
+struct Place {
+    int64_t row0; // row number of its slot in head 0's block
+    bool there;
+};
+__device__ __forceinline__ Place find_place(const PagesStore &st, const PagesBatch &b, int tok, bool &owned) {
     const int i = find_sequence(b, tok);
     const Span s = pages_span(b, st, i);
-    const int at = tok - s.start;
-    const int t = s.kv - s.n + at;
-    if (at < 0 || at >= s.n || t < 0) return; // warp-uniform
+    const int at = tok - s.start, t = s.kv - s.n + at;
+    owned = at >= 0 && at < s.n;
+    Place p{0, false};
+    if (!owned || t < 0) return p;
     const int page = pages_page(b, st, i, t);
-    if (page < 0) return;
-    const int64_t row = pages_row(st, page, head, t);
-    unsigned char *dst = (value ? st.v : st.k) + row * st.row_bytes;
-    if constexpr (BITS == 16) {
-        if (!live) return;
-        if (st.dtype == kBF16)
-            store8(reinterpret_cast<__nv_bfloat16 *>(dst) + c, true, e);
-        else
-            store8(reinterpret_cast<__half *>(dst) + c, true, e);
-    } else {
-        constexpr float levels = (float)((1 << BITS) - 1);
-        float mn = inf, mx = -inf;
-        if (live) {
-            mn = mx = e[0];
+    p.there = page >= 0;
+    p.row0 = pages_row(st, max(page, 0), 0, t);
+    return p;
+}
+
+__device__ __forceinline__ float min3f(float a, float b, float c) {
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// Eight codes of a row with (scale, zero), packed: code = clamp(rint((x - zero) /
+// scale), 0, levels) as an IEEE quotient gives it.  With d = x - zero, fma(d, 1 /
+// scale, 2^23) rounds the exact product d * rcp half to even into the low mantissa
+// bits, and e is that product's distance from the integer; product and quotient differ
+// by less than 2^(BITS-23), so where |e| <= 1/2 - 2^(BITS-22) for all eight, both round
+// to the same integer, which lies in 0 .. levels.  Otherwise (a near tie, NaN, a scale
+// without a normal reciprocal) the eight are divided.
+template <int BITS>
+__device__ __forceinline__ void pack8(const float (&x)[8], float zero, float scale, uint32_t &lo, uint32_t &hi) {
+    constexpr float levels = (float)((1 << BITS) - 1), magic = 8388608.0f;
+    constexpr float margin = (float)(1u << BITS) * 0x1p-22f;
+    uint32_t c[8];
+    float dev = 1.0f;
+    if (scale >= 0x1p-125f && scale <= 0x1p125f) {
+        const float rcp = __frcp_rn(scale);
+        dev = 0.0f;
 #pragma unroll
-            for (int j = 1; j < 8; ++j) {
-                mn = fminf(mn, e[j]);
-                mx = fmaxf(mx, e[j]);
-            }
+        for (int j = 0; j < 8; j += 2) {
+            const float2 d = __fadd2_rn(make_float2(x[j], x[j + 1]), make_float2(-zero, -zero));
+            const float2 r2 = make_float2(rcp, rcp), m2 = make_float2(magic, magic);
+            const float2 rm = __ffma2_rn(d, r2, m2);
+            const float2 nr = __ffma2_rn(rm, make_float2(-1.0f, -1.0f), m2); // minus the integer
+            const float2 e = __ffma2_rn(d, r2, nr);
+            dev = max3_nan(dev, fabsf(e.x), fabsf(e.y));
+            c[j] = __float_as_uint(rm.x), c[j + 1] = __float_as_uint(rm.y);
         }
-        // lanes of another row never mix in: the butterfly stays within L lanes
-        for (int o = L / 2; o > 0; o >>= 1) {
-            const float a = __shfl_xor_sync(0xffffffffu, mn, o), z = __shfl_xor_sync(0xffffffffu, mx, o);
-            mn = fminf(mn, a);
-            mx = fmaxf(mx, z);
-        }
-        if (!live) return;
-        const float span = __fsub_rn(mx, mn);
-        const float scale = span == 0.0f ? 0.0f : __fdiv_rn(span, levels);
-        uint32_t code[8];
-#pragma unroll
+    }
+    if (!(dev <= 0.5f - margin)) {
+#pragma unroll 1
         for (int j = 0; j < 8; ++j) {
-            float q = scale == 0.0f ? 0.0f : rintf(__fdiv_rn(__fsub_rn(e[j], mn), scale));
-            q = fminf(fmaxf(q, 0.0f), levels);
-            code[j] = __float_as_uint(__fadd_rn(q, 8388608.0f)) & 0xFFu;
-        }
-        if constexpr (BITS == 8) {
-            uint2 o;
-            o.x = code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
-            o.y = code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24;
-            *reinterpret_cast<uint2 *>(dst + c) = o;
-        } else {
-            uint32_t o = 0;
+            float v = x[0];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o |= code[j] << (4 * j);
-            *reinterpret_cast<uint32_t *>(dst + c / 2) = o;
+            for (int k = 1; k < 8; ++k) v = j == k ? x[k] : v;
+            float q = scale == 0.0f ? 0.0f : rintf(__fdiv_rn(__fsub_rn(v, zero), scale));
+            q = fminf(fmaxf(q, 0.0f), levels);
+            const uint32_t u = __float_as_uint(__fadd_rn(q, magic));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) c[k] = j == k ? u : c[k];
         }
-        if (c == 0) (value ? st.vp : st.kp)[row] = make_float2(scale, mn);
+    }
+    if constexpr (BITS == 8) {
+        lo = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+        hi = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
+    } else {
+        // pairs into bytes, then four bytes into the word
+        uint32_t p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = (c[2 * j] & 15u) | (c[2 * j + 1] & 15u) << 4;
+        lo = __byte_perm(__byte_perm(p[0], p[1], 0x0040), __byte_perm(p[2], p[3], 0x0040), 0x5410);
+        hi = 0;
     }
 }
 
 template <int BITS, int T>
-__global__ void __launch_bounds__(256) pages_read_kernel(PagesStore st, PagesBatch b, PagesDense x, int L,
-                                                         int wpt) {
+__global__ void __launch_bounds__(256) pages_write_kernel(PagesStore st, PagesBatch b, PagesDense x, Work w) {
     using E = typename Elem<T>::type;
+    pdl_wait();
+    pdl_trigger();
     const int lane = threadIdx.x & 31;
-    const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int tok = (int)(w / wpt);
+    const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int tok = (int)(id >> w.log_parts), part = (int)id & ((1 << w.log_parts) - 1);
     if (tok >= b.total) return;
-    const int r = (int)(w % wpt) * (32 / L) + lane / L;
-    const int c = lane % L * 8;
-    const int i = find_sequence(b, tok);
-    const Span s = pages_span(b, st, i);
-    const int at = tok - s.start;
-    const int t = s.kv - s.n + at;
-    if (r >= 2 * st.H || c >= st.D || at < 0 || at >= s.n) return;
-    const bool value = r >= st.H;
-    const int head = value ? r - st.H : r;
-    const int page = t < 0 ? -1 : pages_page(b, st, i, t);
-    float e[8] = {};
-    if (page >= 0) {
-        const int64_t row = pages_row(st, page, head, t);
-        const unsigned char *src = (value ? st.v : st.k) + row * st.row_bytes;
-        if constexpr (BITS == 16) {
-            if (st.dtype == kBF16)
-                load8(reinterpret_cast<const __nv_bfloat16 *>(src) + c, true, e);
-            else
-                load8(reinterpret_cast<const __half *>(src) + c, true, e);
-        } else {
-            const float2 p = (value ? st.vp : st.kp)[row];
-            if constexpr (BITS == 8) {
-                const uint2 o = *reinterpret_cast<const uint2 *>(src + c);
+    const int sub = lane / w.L, c = lane % w.L * 8;
+    const bool in = c < st.D;
+    bool owned = false;
+    Place at{0, false};
+    for (int s0 = part; s0 < w.steps; s0 += kAhead << w.log_parts) {
+        Raw<E> raw[kAhead];
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    e[j] = fmaf((float)(((j < 4 ? o.x : o.y) >> (8 * (j & 3))) & 0xFFu), p.x, p.y);
+        for (int u = 0; u < kAhead; ++u) {
+            const int r = (s0 + (u << w.log_parts)) * w.R + sub;
+            if (r < 2 * st.H && in) {
+                const bool value = r >= st.H;
+                raw[u].load(static_cast<const E *>(value ? x.v : x.k) + tok * x.token + (value ? r - st.H : r) * x.head + c, x.vec);
+            }
+        }
+        if (s0 == part) { // while the first loads are under way
+            at = find_place(st, b, tok, owned);
+            if (!at.there) return; // the whole warp
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int step = s0 + (u << w.log_parts);
+            if (step >= w.steps) break;
+            const int r = step * w.R + sub;
+            const bool live = r < 2 * st.H && in, value = r >= st.H;
+            const int64_t row = at.row0 + ((int64_t)(value ? r - st.H : r) << st.shift);
+            unsigned char *dst = (value ? st.v : st.k) + row * st.row_bytes;
+            if constexpr (BITS == 16) {
+                if (!live) continue;
+                if constexpr (T != kF32) {
+                    if (T == st.dtype) { // as it came
+                        *reinterpret_cast<uint4 *>(dst + 2 * c) = raw[u].w[0];
+                        continue;
+                    }
+                }
+                float e[8];
+                raw[u].floats(e);
+                if (st.dtype == kBF16)
+                    store8(reinterpret_cast<__nv_bfloat16 *>(dst) + c, true, e);
+                else
+                    store8(reinterpret_cast<__half *>(dst) + c, true, e);
             } else {
-                const uint32_t o = *reinterpret_cast<const uint32_t *>(src + c / 2);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) e[j] = fmaf((float)((o >> (4 * j)) & 15u), p.x, p.y);
+                float e[8], mn = INFINITY, mx = -INFINITY;
+                if (live) {
+                    raw[u].floats(e);
+                    mn = min3f(min3f(e[0], e[1], e[2]), min3f(e[3], e[4], e[5]), fminf(e[6], e[7]));
+                    mx = max3f(max3f(e[0], e[1], e[2]), max3f(e[3], e[4], e[5]), fmaxf(e[6], e[7]));
+                }
+                // lanes of another row never mix in: the butterfly stays within L lanes
+                for (int o = w.L / 2; o > 0; o >>= 1) {
+                    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                }
+                if (live) {
+                    const float span = __fsub_rn(mx, mn);
+                    const float scale = span == 0.0f ? 0.0f : __fdiv_rn(span, (float)((1 << BITS) - 1));
+                    uint32_t lo, hi;
+                    pack8<BITS>(e, mn, scale, lo, hi);
+                    if constexpr (BITS == 8)
+                        *reinterpret_cast<uint2 *>(dst + c) = make_uint2(lo, hi);
+                    else
+                        *reinterpret_cast<uint32_t *>(dst + c / 2) = lo;
+                    if (c == 0) (value ? st.vp : st.kp)[row] = make_float2(scale, mn);
+                }
+                __syncwarp();
             }
         }
     }
-    E *dst = static_cast<E *>(const_cast<void *>(value ? x.v : x.k)) + tok * x.token + head * x.head + c;
-    store8(dst, x.vec, e);
+}
+
+template <int BITS, int T>
+__global__ void __launch_bounds__(256) pages_read_kernel(PagesStore st, PagesBatch b, PagesDense x, Work w) {
+    using E = typename Elem<T>::type;
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int tok = (int)(id >> w.log_parts), part = (int)id & ((1 << w.log_parts) - 1);
+    if (tok >= b.total) return;
+    const int sub = lane / w.L, c = lane % w.L * 8;
+    const bool in = c < st.D;
+    bool owned;
+    const Place at = find_place(st, b, tok, owned);
+    if (!owned) return;
+    for (int s0 = part; s0 < w.steps; s0 += kAhead << w.log_parts) {
+        uint4 raw[kAhead];
+        float2 par[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int r = (s0 + (u << w.log_parts)) * w.R + sub;
+            raw[u] = make_uint4(0, 0, 0, 0);
+            par[u] = make_float2(0.0f, 0.0f);
+            if (r < 2 * st.H && in && at.there) {
+                const bool value = r >= st.H;
+                const int64_t row = at.row0 + ((int64_t)(value ? r - st.H : r) << st.shift);
+                const unsigned char *src = (value ? st.v : st.k) + row * st.row_bytes;
+                if constexpr (BITS == 16) {
+                    raw[u] = __ldcs(reinterpret_cast<const uint4 *>(src + 2 * c));
+                } else {
+                    if constexpr (BITS == 8) {
+                        const uint2 y = __ldcs(reinterpret_cast<const uint2 *>(src + c));
+                        raw[u].x = y.x, raw[u].y = y.y;
+                    } else {
+                        raw[u].x = __ldcs(reinterpret_cast<const uint32_t *>(src + c / 2));
+                    }
+                    par[u] = __ldg((value ? st.vp : st.kp) + row);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int r = (s0 + (u << w.log_parts)) * w.R + sub;
+            if (r >= 2 * st.H || !in) continue;
+            const bool value = r >= st.H;
+            E *dst = static_cast<E *>(const_cast<void *>(value ? x.v : x.k)) + tok * x.token + (value ? r - st.H : r) * x.head + c;
+            float e[8];
+            if constexpr (BITS == 16) {
+                if constexpr (T != kF32) {
+                    if (T == st.dtype && x.vec) {
+                        __stcs(reinterpret_cast<uint4 *>(dst), raw[u]);
+                        continue;
+                    }
+                }
+                const uint32_t v[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint16_t h = (uint16_t)(v[j / 2] >> (16 * (j & 1)));
+                    e[j] = st.dtype == kBF16 ? __uint_as_float((uint32_t)h << 16) : __half2float(__ushort_as_half(h));
+                }
+            } else {
+                // the code in the mantissa of 2^23, less 2^23: exact
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    uint32_t a, z;
+                    if constexpr (BITS == 8) {
+                        a = __byte_perm(j < 4 ? raw[u].x : raw[u].y, 0x4B000000u, 0x7440u | (j & 3));
+                        z = __byte_perm(j < 4 ? raw[u].x : raw[u].y, 0x4B000000u, 0x7441u + (j & 3));
+                    } else {
+                        a = (raw[u].x >> (4 * j) & 15u) | 0x4B000000u, z = (raw[u].x >> (4 * j + 4) & 15u) | 0x4B000000u;
+                    }
+                    const float2 q = __fadd2_rn(make_float2(__uint_as_float(a), __uint_as_float(z)), make_float2(-8388608.0f, -8388608.0f));
+                    const float2 y = __ffma2_rn(q, make_float2(par[u].x, par[u].x), make_float2(par[u].y, par[u].y));
+                    e[j] = y.x, e[j + 1] = y.y;
+                }
+            }
+            store8(dst, x.vec, e);
+        }
+    }
 }
 
 template <template <int, int> class F, class... A>
@@ -200,32 +341,35 @@ cudaError_t by_type(int bits, int dtype, A &&...a) {
     return dtype == kF32 ? F<4, kF32>::go(a...) : dtype == kF16 ? F<4, kF16>::go(a...) : F<4, kBF16>::go(a...);
 }
 
-// lanes per row and warps per token
-struct RowSplit {
-    int L, wpt;
-    int64_t ctas;
-    RowSplit(const PagesStore &st, const PagesBatch &b) {
-        L = 4;
-        while (L * 8 < st.D) L *= 2;
-        wpt = (2 * st.H + 32 / L - 1) / (32 / L);
-        ctas = ((int64_t)b.total * wpt + 7) / 8;
-    }
-};
+// The division of a launch; false if the grid would be too large.
+bool divide(const PagesStore &st, const PagesBatch &b, Work *w, unsigned *ctas) {
+    w->L = 4;
+    while (w->L * 8 < st.D) w->L *= 2;
+    w->R = 32 / w->L;
+    w->steps = (2 * st.H + w->R - 1) / w->R;
+    // measured for 16 x 1 tokens of 8 x 128: 3.4 us with a warp a step, 5 us with one a
+    // token; for 16 x 2048 tokens 66 us with one a token, 150 us with a warp a step
+    w->log_parts = 0;
+    while ((1 << w->log_parts) < w->steps && ((int64_t)b.total << w->log_parts) < 148 * 16) ++w->log_parts;
+    const int64_t n = (((int64_t)b.total << w->log_parts) + 7) / 8;
+    *ctas = (unsigned)n;
+    return n <= 0x7fffffff;
+}
 
 template <int BITS, int T> struct Write {
     static cudaError_t go(const PagesStore &st, const PagesBatch &b, const PagesDense &x, cudaStream_t s) {
-        const RowSplit r(st, b);
-        if (r.ctas > 0x7fffffff) return cudaErrorInvalidValue;
-        return launch_pdl(pages_write_kernel<BITS, T>, dim3((unsigned)r.ctas), dim3(256), 0, s, false, st, b, x,
-                          r.L, r.wpt);
+        Work w;
+        unsigned ctas;
+        if (!divide(st, b, &w, &ctas)) return cudaErrorInvalidValue;
+        return launch_pdl(pages_write_kernel<BITS, T>, dim3(ctas), dim3(256), 0, s, true, st, b, x, w);
     }
 };
 template <int BITS, int T> struct Read {
     static cudaError_t go(const PagesStore &st, const PagesBatch &b, const PagesDense &x, cudaStream_t s) {
-        const RowSplit r(st, b);
-        if (r.ctas > 0x7fffffff) return cudaErrorInvalidValue;
-        return launch_pdl(pages_read_kernel<BITS, T>, dim3((unsigned)r.ctas), dim3(256), 0, s, false, st, b, x,
-                          r.L, r.wpt);
+        Work w;
+        unsigned ctas;
+        if (!divide(st, b, &w, &ctas)) return cudaErrorInvalidValue;
+        return launch_pdl(pages_read_kernel<BITS, T>, dim3(ctas), dim3(256), 0, s, true, st, b, x, w);
     }
 };
 
