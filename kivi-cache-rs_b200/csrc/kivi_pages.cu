@@ -174,6 +174,57 @@ __device__ __forceinline__ void pack8(const float (&x)[8], float zero, float sca
     }
 }
 
+// Minimum and maximum of a row, NaN left out, over its L lanes: as (min, -max), so that
+// one minimum does for both; 16-bit elements stay packed in a word, which halves the
+// shuffles as well.
+template <int T> struct Range {
+    float mn, nx;
+    __device__ __forceinline__ void of(const Raw<float> &r, bool live) {
+        float e[8];
+        r.floats(e);
+        mn = live ? min3f(min3f(e[0], e[1], e[2]), min3f(e[3], e[4], e[5]), fminf(e[6], e[7])) : INFINITY;
+        nx = live ? -max3f(max3f(e[0], e[1], e[2]), max3f(e[3], e[4], e[5]), fmaxf(e[6], e[7])) : INFINITY;
+    }
+    __device__ __forceinline__ void join(int o, bool in) {
+        const float a = __shfl_xor_sync(0xffffffffu, mn, o), b = __shfl_xor_sync(0xffffffffu, nx, o);
+        if (in) mn = fminf(mn, a), nx = fminf(nx, b);
+    }
+    __device__ __forceinline__ float least() const { return mn; }
+    __device__ __forceinline__ float most() const { return -nx; }
+};
+template <int T> struct Range16 {
+    uint32_t v; // (min, -max)
+    __device__ __forceinline__ static uint32_t min2(uint32_t a, uint32_t b) {
+        uint32_t d;
+        if constexpr (T == kBF16) asm("min.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        else asm("min.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
+    __device__ __forceinline__ static uint32_t max2(uint32_t a, uint32_t b) {
+        uint32_t d;
+        if constexpr (T == kBF16) asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        else asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
+    template <class E> __device__ __forceinline__ void of(const Raw<E> &r, bool live) {
+        const uint4 w = r.w[0];
+        const uint32_t a = min2(min2(w.x, w.y), min2(w.z, w.w)), b = max2(max2(w.x, w.y), max2(w.z, w.w)) ^ 0x80008000u;
+        v = min2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+        if (!live) v = T == kBF16 ? 0x7f807f80u : 0x7c007c00u; // infinities
+    }
+    __device__ __forceinline__ void join(int o, bool in) {
+        const uint32_t a = __shfl_xor_sync(0xffffffffu, v, o);
+        if (in) v = min2(v, a);
+    }
+    __device__ __forceinline__ static float f(uint16_t h) {
+        return T == kBF16 ? __uint_as_float((uint32_t)h << 16) : __half2float(__ushort_as_half(h));
+    }
+    __device__ __forceinline__ float least() const { return f((uint16_t)v); }
+    __device__ __forceinline__ float most() const { return -f((uint16_t)(v >> 16)); }
+};
+template <> struct Range<kBF16> : Range16<kBF16> {};
+template <> struct Range<kF16> : Range16<kF16> {};
+
 template <int BITS, int T>
 __global__ void __launch_bounds__(256) pages_write_kernel(PagesStore st, PagesBatch b, PagesDense x, Work w) {
     using E = typename Elem<T>::type;
@@ -201,16 +252,24 @@ __global__ void __launch_bounds__(256) pages_write_kernel(PagesStore st, PagesBa
             at = find_place(st, b, tok, owned);
             if (!at.there) return; // the whole warp
         }
+        Range<T> range[kAhead];
+        if constexpr (BITS < 16) { // the steps' reductions side by side
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) range[u].of(raw[u], in && (s0 + (u << w.log_parts)) * w.R + sub < 2 * st.H);
+            // lanes of another row never mix in: the butterfly stays within L lanes
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) range[u].join(o, o < w.L);
+        }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            const int step = s0 + (u << w.log_parts);
-            if (step >= w.steps) break;
-            const int r = step * w.R + sub;
-            const bool live = r < 2 * st.H && in, value = r >= st.H;
+            const int r = (s0 + (u << w.log_parts)) * w.R + sub;
+            if (r >= 2 * st.H || !in) continue;
+            const bool value = r >= st.H;
             const int64_t row = at.row0 + ((int64_t)(value ? r - st.H : r) << st.shift);
             unsigned char *dst = (value ? st.v : st.k) + row * st.row_bytes;
             if constexpr (BITS == 16) {
-                if (!live) continue;
                 if constexpr (T != kF32) {
                     if (T == st.dtype) { // as it came
                         *reinterpret_cast<uint4 *>(dst + 2 * c) = raw[u].w[0];
@@ -224,31 +283,20 @@ __global__ void __launch_bounds__(256) pages_write_kernel(PagesStore st, PagesBa
                 else
                     store8(reinterpret_cast<__half *>(dst) + c, true, e);
             } else {
-                float e[8], mn = INFINITY, mx = -INFINITY;
-                if (live) {
-                    raw[u].floats(e);
-                    mn = min3f(min3f(e[0], e[1], e[2]), min3f(e[3], e[4], e[5]), fminf(e[6], e[7]));
-                    mx = max3f(max3f(e[0], e[1], e[2]), max3f(e[3], e[4], e[5]), fmaxf(e[6], e[7]));
-                }
-                // lanes of another row never mix in: the butterfly stays within L lanes
-                for (int o = w.L / 2; o > 0; o >>= 1) {
-                    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                }
-                if (live) {
-                    const float span = __fsub_rn(mx, mn);
-                    const float scale = span == 0.0f ? 0.0f : __fdiv_rn(span, (float)((1 << BITS) - 1));
-                    uint32_t lo, hi;
-                    pack8<BITS>(e, mn, scale, lo, hi);
-                    if constexpr (BITS == 8)
-                        *reinterpret_cast<uint2 *>(dst + c) = make_uint2(lo, hi);
-                    else
-                        *reinterpret_cast<uint32_t *>(dst + c / 2) = lo;
-                    if (c == 0) (value ? st.vp : st.kp)[row] = make_float2(scale, mn);
-                }
-                __syncwarp();
+                float e[8];
+                raw[u].floats(e);
+                const float mn = range[u].least(), span = __fsub_rn(range[u].most(), mn);
+                const float scale = span == 0.0f ? 0.0f : __fdiv_rn(span, (float)((1 << BITS) - 1));
+                uint32_t lo, hi;
+                pack8<BITS>(e, mn, scale, lo, hi);
+                if constexpr (BITS == 8)
+                    *reinterpret_cast<uint2 *>(dst + c) = make_uint2(lo, hi);
+                else
+                    *reinterpret_cast<uint32_t *>(dst + c / 2) = lo;
+                if (c == 0) (value ? st.vp : st.kp)[row] = make_float2(scale, mn);
             }
         }
+        __syncwarp();
     }
 }
 
