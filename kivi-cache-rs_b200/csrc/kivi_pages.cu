@@ -121,45 +121,43 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     return d;
 }
 
-// Eight codes of a row with (scale, zero), packed: code = clamp(rint((x - zero) /
-// scale), 0, levels) as an IEEE quotient gives it.  With d = x - zero, fma(d, 1 /
-// scale, 2^23) rounds the exact product d * rcp half to even into the low mantissa
-// bits, and e is that product's distance from the integer; product and quotient differ
-// by less than 2^(BITS-23), so where |e| <= 1/2 - 2^(BITS-22) for all eight, both round
-// to the same integer, which lies in 0 .. levels.  Otherwise (a near tie, NaN, a scale
-// without a normal reciprocal) the eight are divided.
+// clamp(rint((x - zero) / scale), 0, levels) by an IEEE quotient, in the low bits
+__device__ __noinline__ uint32_t exact_code(float x, float zero, float scale, float levels) {
+    float q = scale == 0.0f ? 0.0f : rintf(__fdiv_rn(__fsub_rn(x, zero), scale));
+    q = fminf(fmaxf(q, 0.0f), levels);
+    return __float_as_uint(__fadd_rn(q, 8388608.0f));
+}
+
+// Eight codes of a row with (scale, zero), packed: exact_code of each.  With d = x -
+// zero, fma(d, 1 / scale, 2^23) rounds the exact product d * rcp half to even into the
+// low mantissa bits, and e is that product's distance from the integer; product and
+// quotient differ by less than 2^(BITS-23), so where |e| <= 1/2 - 2^(BITS-22) both round
+// to the same integer, which lies in 0 .. levels.  The others (near ties, which 0.4% of
+// bf16 values are: their differences and spans have few bits; NaN; a scale without a
+// normal reciprocal) are divided one by one.
 template <int BITS>
 __device__ __forceinline__ void pack8(const float (&x)[8], float zero, float scale, uint32_t &lo, uint32_t &hi) {
     constexpr float levels = (float)((1 << BITS) - 1), magic = 8388608.0f;
-    constexpr float margin = (float)(1u << BITS) * 0x1p-22f;
+    const bool fast = scale >= 0x1p-125f && scale <= 0x1p125f;
+    const float limit = fast ? 0.5f - (float)(1u << BITS) * 0x1p-22f : -1.0f, rcp = fast ? __frcp_rn(scale) : 0.0f;
     uint32_t c[8];
-    float dev = 1.0f;
-    if (scale >= 0x1p-125f && scale <= 0x1p125f) {
-        const float rcp = __frcp_rn(scale);
-        dev = 0.0f;
+    float e[8];
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            const float2 d = __fadd2_rn(make_float2(x[j], x[j + 1]), make_float2(-zero, -zero));
-            const float2 r2 = make_float2(rcp, rcp), m2 = make_float2(magic, magic);
-            const float2 rm = __ffma2_rn(d, r2, m2);
-            const float2 nr = __ffma2_rn(rm, make_float2(-1.0f, -1.0f), m2); // minus the integer
-            const float2 e = __ffma2_rn(d, r2, nr);
-            dev = max3_nan(dev, fabsf(e.x), fabsf(e.y));
-            c[j] = __float_as_uint(rm.x), c[j + 1] = __float_as_uint(rm.y);
-        }
+    for (int j = 0; j < 8; j += 2) {
+        const float2 d = __fadd2_rn(make_float2(x[j], x[j + 1]), make_float2(-zero, -zero));
+        const float2 r2 = make_float2(rcp, rcp), m2 = make_float2(magic, magic);
+        const float2 rm = __ffma2_rn(d, r2, m2);
+        const float2 nr = __ffma2_rn(rm, make_float2(-1.0f, -1.0f), m2); // minus the integer
+        const float2 f = __ffma2_rn(d, r2, nr);
+        c[j] = __float_as_uint(rm.x), c[j + 1] = __float_as_uint(rm.y);
+        e[j] = f.x, e[j + 1] = f.y;
     }
-    if (!(dev <= 0.5f - margin)) {
-#pragma unroll 1
-        for (int j = 0; j < 8; ++j) {
-            float v = x[0];
+    const float dev = max3_nan(max3_nan(fabsf(e[0]), fabsf(e[1]), fabsf(e[2])), max3_nan(fabsf(e[3]), fabsf(e[4]), fabsf(e[5])),
+                               max3_nan(fabsf(e[6]), fabsf(e[7]), fabsf(e[7])));
+    if (!(dev <= limit)) {
 #pragma unroll
-            for (int k = 1; k < 8; ++k) v = j == k ? x[k] : v;
-            float q = scale == 0.0f ? 0.0f : rintf(__fdiv_rn(__fsub_rn(v, zero), scale));
-            q = fminf(fmaxf(q, 0.0f), levels);
-            const uint32_t u = __float_as_uint(__fadd_rn(q, magic));
-#pragma unroll
-            for (int k = 0; k < 8; ++k) c[k] = j == k ? u : c[k];
-        }
+        for (int j = 0; j < 8; ++j)
+            if (!(fabsf(e[j]) <= limit)) c[j] = exact_code(x[j], zero, scale, levels);
     }
     if constexpr (BITS == 8) {
         lo = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
