@@ -85,7 +85,7 @@ template <class E> struct Raw {
 struct Work {
     int L, R, steps, log_parts;
 };
-constexpr int kAhead = 4; // steps whose loads are in flight at once
+constexpr int kAhead = 2; // steps whose loads are in flight at once
 
 // The token of this warp: its slot in the store, or false where it has none.
 struct Place {

@@ -15,7 +15,10 @@
 // (scale s, zero z) apply to the sums, with z' = z + 2^(b-1) s:
 //   q.k = s_k (q.c) + z'_k sum q,   o = sum (p s_v) c + sum p z'_v.
 // P (or p s_v) is split into two 16-bit parts, so no weight is rounded to 8 or
-// 11 bits: the tensor pipe has the room.
+// 11 bits: the tensor pipe has the room.  With codes the operands are f16, whose ten
+// bits hold a code as it lies in its word (bf16's seven do not: twice the
+// instructions); a row's query is scaled by a power of two into f16's upper end, and
+// the weights by one that follows the largest value scale met, both undone in fp32.
 //
 // What bounds it: HBM.  Per token and kv head 4 D bytes (16-bit), 2 D + 16
 // (8-bit), D + 16 (4-bit), each read once.
@@ -109,29 +112,26 @@ template <bool F16> __device__ __forceinline__ void split2(float a, float b, uin
     }
 }
 
-__device__ __forceinline__ uint32_t sub_bf2(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
 __device__ __forceinline__ uint32_t sub_h2(uint32_t a, uint32_t b) {
     uint32_t d;
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
-// Codes in the low bits of w's two halves (other bits ignored) as a pair of
-// c - 2^(BITS-1), exact.  bf16 carries 7 bits behind the point: 128 + (c & 127)
-// minus 128 or 256 by the code's top bit; f16 carries ten: 1024 + c minus 1152.
-template <int BITS, bool F16> __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
-    if constexpr (BITS == 8 && F16)
-        return sub_h2((w & 0x00ff00ffu) | 0x64006400u, 0x64806480u);
-    else if constexpr (BITS == 8)
-        return sub_bf2((w & 0x007f007fu) | 0x43004300u, (~w & 0x00800080u) | 0x43004300u);
-    else if constexpr (F16)
-        return sub_h2((w & 0x000f000fu) | 0x64006400u, 0x64086408u);
-    else
-        return sub_bf2((w & 0x000f000fu) | 0x43004300u, 0x43084308u);
+// Codes in the low bits of w's two halves (other bits ignored) as a pair of f16
+// c - 2^(BITS-1), exact: the code in the mantissa of 1024.
+template <int BITS> __device__ __forceinline__ uint32_t low_pair(uint32_t w) {
+    if constexpr (BITS == 8) return sub_h2((w & 0x00ff00ffu) | 0x64006400u, 0x64806480u);
+    return sub_h2((w & 0x000f000fu) | 0x64006400u, 0x64086408u);
 }
+// The next codes of the two halves.  8 bits: shifted down.  4 bits: left in place, so
+// 16 (c - 8), the 16 taken out of the queries or of the output.
+template <int BITS> __device__ __forceinline__ uint32_t next_pair(uint32_t w) {
+    if constexpr (BITS == 8) return low_pair<8>(w >> 8);
+    return sub_h2((w & 0x00f000f0u) | 0x64006400u, 0x64806480u);
+}
+// x in its upper end of f16: e with |x| 2^-e < 2^14 (-126 at least)
+__device__ __forceinline__ int f16_exponent(uint32_t magnitude_bits) { return max(-126, (int)(magnitude_bits >> 23) - 140); }
+__device__ __forceinline__ float exp2i(int k) { return __uint_as_float((uint32_t)(max(-126, min(127, k)) + 127) << 23); }
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -214,6 +214,7 @@ __device__ __forceinline__ void store_out(const PagesAttn &a, int tok, int hq, i
 template <int BITS, int ND, bool F16>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(BITS, ND))
     pages_decode_kernel(const PagesAttn a, int min_per, int *counters) {
+    static_assert(BITS == 16 || F16, "codes become f16 operands");
     using L = Lay<BITS, ND>;
     constexpr int D = L::D, TT = L::TT, TK = L::TK, STEPS = 2 * ND;
     __shared__ long long s_sum[kWarps + 1];
@@ -299,6 +300,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(BITS, ND))
             // ---- this row's queries, in the order of the key registers
             uint32_t qf[STEPS][2];
             float qs0 = 0.0f, qs1 = 0.0f; // sums of rows 2j, 2j + 1
+            float c20 = c2, c21 = c2;     // their scores' exp2 units
             {
                 const uint16_t *q = static_cast<const uint16_t *>(a.q) + sp.start * a.q_token +
                                     (int64_t)(h * G + g) * a.q_head;
@@ -311,16 +313,36 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(BITS, ND))
                         if (g < G) x = q[L::kch(s, r, 0, j)] | (uint32_t)q[L::kch(s, r, 1, j)] << 16;
                         if (a.qsign < 0.0f) x ^= 0x80008000u;
                         qf[s][r] = x;
-                        if constexpr (BITS < 16) {
-                            if constexpr (F16) {
-                                const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&x));
-                                sum += y.x + y.y;
-                            } else {
-                                sum += __uint_as_float(x << 16) + __uint_as_float(x & 0xffff0000u);
-                            }
-                        }
                     }
                 if constexpr (BITS < 16) {
+                    auto pair = [&](uint32_t x) {
+                        if (a.dtype == kF16) return __half22float2(*reinterpret_cast<const __half2 *>(&x));
+                        return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+                    };
+                    float most = 0.0f;
+#pragma unroll
+                    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const float2 y = pair(qf[s][r]);
+                            most = fmaxf(most, fmaxf(fabsf(y.x), fabsf(y.y)));
+                            sum += y.x + y.y;
+                        }
+                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                    const int e = f16_exponent(__float_as_uint(most));
+                    const float f = exp2i(-e);
+#pragma unroll
+                    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const float2 y = pair(qf[s][r]);
+                            const float fr = BITS == 4 && r ? f * 0.0625f : f; // next_pair's 16
+                            const __half2 h = __floats2half2_rn(y.x * fr, y.y * fr);
+                            qf[s][r] = *reinterpret_cast<const uint32_t *>(&h);
+                        }
+                    c20 = c2 * exp2i(__shfl_sync(0xffffffffu, e, 8 * j));
+                    c21 = c2 * exp2i(__shfl_sync(0xffffffffu, e, 8 * j + 4));
                     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
                     qs0 = __shfl_sync(0xffffffffu, sum, 8 * j);
@@ -332,6 +354,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(BITS, ND))
 #pragma unroll
             for (int i = 0; i < STEPS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
             float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, z0 = 0.0f, z1 = 0.0f;
+            int eref = -200; // exponent of O, with codes
             Tile<BITS, ND, F16> x;
 
             auto first_token = [&](int t) { return (t < tl.ns ? t : t - tl.ns + tl.ws) * TK; };
@@ -398,12 +421,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(BITS, ND))
                             a0 = x.k[s][0][2 * i], a2 = x.k[s][0][2 * i + 1];
                             a1 = x.k[s][1][2 * i], a3 = x.k[s][1][2 * i + 1];
                         } else if constexpr (BITS == 8) {
-                            a0 = code_pair<8, F16>(x.k[s][0][i]), a2 = code_pair<8, F16>(x.k[s][0][i] >> 8);
-                            a1 = code_pair<8, F16>(x.k[s][1][i]), a3 = code_pair<8, F16>(x.k[s][1][i] >> 8);
+                            a0 = low_pair<8>(x.k[s][0][i]), a2 = next_pair<8>(x.k[s][0][i]);
+                            a1 = low_pair<8>(x.k[s][1][i]), a3 = next_pair<8>(x.k[s][1][i]);
                         } else {
                             const uint32_t u = x.k[s][0][i / 2] >> (8 * (i & 1)), w = x.k[s][1][i / 2] >> (8 * (i & 1));
-                            a0 = code_pair<4, F16>(u), a2 = code_pair<4, F16>(u >> 4);
-                            a1 = code_pair<4, F16>(w), a3 = code_pair<4, F16>(w >> 4);
+                            a0 = low_pair<4>(u), a2 = next_pair<4>(u);
+                            a1 = low_pair<4>(w), a3 = next_pair<4>(w);
                         }
                         mma<F16>(c, a0, a1, a2, a3, qf[i][0], qf[i][1]);
                     }
@@ -414,9 +437,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(BITS, ND))
                         constexpr float half = (float)(1 << (BITS - 1));
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const float sc = x.kp[s][i].x * c2, z = fmaf(half, x.kp[s][i].x, x.kp[s][i].y) * c2;
-                            sx[s][2 * i] = fmaf(sc, c[2 * i], z * qs0);
-                            sx[s][2 * i + 1] = fmaf(sc, c[2 * i + 1], z * qs1);
+                            const float z = fmaf(half, x.kp[s][i].x, x.kp[s][i].y) * c2;
+                            sx[s][2 * i] = fmaf(x.kp[s][i].x * c20, c[2 * i], z * qs0);
+                            sx[s][2 * i + 1] = fmaf(x.kp[s][i].x * c21, c[2 * i + 1], z * qs1);
                         }
                     }
                 }
@@ -456,6 +479,26 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(BITS, ND))
 #pragma unroll
                     for (int i = 0; i < STEPS; ++i) o[i][0] *= f0, o[i][2] *= f0, o[i][1] *= f1, o[i][3] *= f1;
                 }
+                float fv = 1.0f; // of the value scales
+                if constexpr (BITS < 16) {
+                    uint32_t most = 0;
+#pragma unroll
+                    for (int s = 0; s < TT; ++s)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t b = __float_as_uint(fabsf(vp[s][i].x));
+                            if (b < 0x7f800000u) most = max(most, b);
+                        }
+                    // p <= 2^kLazy: weights below 2^14
+                    const int e = f16_exponent(__reduce_max_sync(0xffffffffu, most)) + (int)kLazy;
+                    if (e > eref) {
+                        const float f = exp2i(max(eref - e, -126));
+                        eref = e;
+#pragma unroll
+                        for (int i = 0; i < STEPS; ++i) o[i][0] *= f, o[i][1] *= f, o[i][2] *= f, o[i][3] *= f;
+                    }
+                    fv = exp2i(-eref);
+                }
                 const float r0 = m0 == -INFINITY ? 0.0f : m0, r1 = m1 == -INFINITY ? 0.0f : m1;
                 // ---- weights, and O^T += V^T P^T
 #pragma unroll
@@ -463,7 +506,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(BITS, ND))
                     float p[4] = {ex2(sx[s][0] - r0), ex2(sx[s][1] - r1), ex2(sx[s][2] - r0), ex2(sx[s][3] - r1)};
                     l0 += p[0] + p[2];
                     l1 += p[1] + p[3];
-                    constexpr bool PF = BITS == 16 && F16; // weights of codes are bf16: p s_v has its range
                     if constexpr (BITS < 16) {
                         constexpr float half = (float)(1 << (BITS - 1));
 #pragma unroll
@@ -471,13 +513,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(BITS, ND))
                             const float z = fmaf(half, vp[s][i].x, vp[s][i].y);
                             z0 = fmaf(p[2 * i], z, z0);
                             z1 = fmaf(p[2 * i + 1], z, z1);
-                            p[2 * i] *= vp[s][i].x;
-                            p[2 * i + 1] *= vp[s][i].x;
+                            p[2 * i] *= vp[s][i].x * fv;
+                            p[2 * i + 1] *= vp[s][i].x * fv;
                         }
                     }
                     uint32_t h0, e0, h1, e1;
-                    split2<PF>(p[0], p[1], h0, e0);
-                    split2<PF>(p[2], p[3], h1, e1);
+                    split2<F16>(p[0], p[1], h0, e0);
+                    split2<F16>(p[2], p[3], h1, e1);
                     h0 = transpose8(h0), h1 = transpose8(h1), e0 = transpose8(e0), e1 = transpose8(e1);
                     if (BITS == 16 && edge) { // 0 times what an unseen row holds is not 0 where that is not finite
 #pragma unroll
@@ -496,19 +538,19 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(BITS, ND))
                             const uint32_t sel = i & 1 ? 0x7632 : 0x5410;
                             const uint32_t u = prmt(x.v[s][0][i / 2], x.v[s][1][i / 2], sel);
                             const uint32_t w = prmt(x.v[s][2][i / 2], x.v[s][3][i / 2], sel);
-                            a0 = code_pair<8, false>(u), a1 = code_pair<8, false>(u >> 8);
-                            a2 = code_pair<8, false>(w), a3 = code_pair<8, false>(w >> 8);
+                            a0 = low_pair<8>(u), a1 = next_pair<8>(u);
+                            a2 = low_pair<8>(w), a3 = next_pair<8>(w);
                         } else {
                             constexpr bool two = L::VU > 2; // two half words of four channels per word
                             const int wi = two ? i / 4 : i / 2;
                             const uint32_t sel = two && (i & 2) ? 0x7632 : 0x5410;
                             const uint32_t u = prmt(x.v[s][0][wi], x.v[s][1][wi], sel) >> (8 * (i & 1));
                             const uint32_t w = prmt(x.v[s][2][wi], x.v[s][3][wi], sel) >> (8 * (i & 1));
-                            a0 = code_pair<4, false>(u), a1 = code_pair<4, false>(u >> 4);
-                            a2 = code_pair<4, false>(w), a3 = code_pair<4, false>(w >> 4);
+                            a0 = low_pair<4>(u), a1 = next_pair<4>(u);
+                            a2 = low_pair<4>(w), a3 = next_pair<4>(w);
                         }
-                        mma<PF>(o[i], a0, a1, a2, a3, e0, e1);
-                        mma<PF>(o[i], a0, a1, a2, a3, h0, h1);
+                        mma<F16>(o[i], a0, a1, a2, a3, e0, e1);
+                        mma<F16>(o[i], a0, a1, a2, a3, h0, h1);
                     }
                 }
                 if (more) {
@@ -531,14 +573,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(BITS, ND))
                 s_l[warp][2 * j] = l0, s_l[warp][2 * j + 1] = l1;
             }
             {
+                const float fo[2] = {BITS < 16 ? exp2i(eref) : 1.0f, BITS < 16 ? exp2i(eref) * (BITS == 4 ? 0.0625f : 1.0f) : 1.0f};
                 float *r0p = reinterpret_cast<float *>(s_o4[warp][2 * j]), *r1p = reinterpret_cast<float *>(s_o4[warp][2 * j + 1]);
 #pragma unroll
                 for (int i = 0; i < STEPS; ++i)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int c = L::vch(i, e, g);
-                        r0p[c] = o[i][2 * e] + z0;
-                        r1p[c] = o[i][2 * e + 1] + z1;
+                        r0p[c] = fmaf(o[i][2 * e], fo[e], z0);
+                        r1p[c] = fmaf(o[i][2 * e + 1], fo[e], z1);
                     }
             }
             __syncthreads();
@@ -656,8 +699,8 @@ cudaError_t launch_pages_decode(const PagesAttn &a, cudaStream_t s) {
     const bool f16 = a.dtype == kF16;
     switch (a.st.bits) {
     case 16: return f16 ? by_dim<16, true>(a, s) : by_dim<16, false>(a, s);
-    case 8: return f16 ? by_dim<8, true>(a, s) : by_dim<8, false>(a, s);
-    default: return f16 ? by_dim<4, true>(a, s) : by_dim<4, false>(a, s);
+    case 8: return by_dim<8, true>(a, s);
+    default: return by_dim<4, true>(a, s);
     }
 }
 

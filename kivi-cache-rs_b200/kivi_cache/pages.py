@@ -19,6 +19,7 @@ from dataclasses import dataclass
 
 DTYPES = {"f32": 0, "f16": 1, "bf16": 2}
 _TENSOR_TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+_types = {}  # the same by dtype object, filled as they are met
 
 
 class _PagesConfig(C.Structure):
@@ -66,17 +67,19 @@ def _rows(x, dtype, strides, heads, dim, total, what):
     """(pointer, type code, token stride, head stride) of dense rows
     [total, heads, dim]: a tensor's own, or a pointer's as given (contiguous
     where no strides are)."""
-    if isinstance(x, int) or x is None:
+    if x is None or isinstance(x, int):
         if dtype is None:
             raise _bad(f"{what}: a pointer needs dtype=")
         token, head = strides if strides is not None else (heads * dim, dim)
         return x, _code(dtype), token, head
-    shape = tuple(x.shape)
-    if shape != (total, heads, dim):
-        raise _bad(f"{what}: expected shape {(total, heads, dim)}, got {shape}")
-    code = _TENSOR_TYPES.get(str(x.dtype))
+    if x.shape != (total, heads, dim):
+        raise _bad(f"{what}: expected shape {(total, heads, dim)}, got {tuple(x.shape)}")
+    code = _types.get(x.dtype)
     if code is None:
-        raise _bad(f"{what}: unsupported element type {x.dtype}")
+        code = _TENSOR_TYPES.get(str(x.dtype))
+        if code is None:
+            raise _bad(f"{what}: unsupported element type {x.dtype}")
+        _types[x.dtype] = code
     token, head, inner = x.stride()
     if inner != 1:
         raise _bad(f"{what}: the elements of a row must be contiguous, their stride is {inner}")
@@ -172,6 +175,9 @@ class KvPages:
                                     _ptr(d_value_params), self.device, C.byref(h), C.byref(err)), err)
         self._h = h.value
         self.config = config
+        self._heads, self._dim = config.num_kv_heads, config.head_dim
+        self._write, self._read = lib().kivi_pages_write_dev, lib().kivi_pages_read_dev
+        self._attention = lib().kivi_pages_attention_dev
 
     def close(self):
         if getattr(self, "_h", None):
@@ -185,28 +191,30 @@ class KvPages:
             pass
 
     def _sides(self, batch, d_keys, d_values, dtype, strides):
-        heads, dim = self.config.num_kv_heads, self.config.head_dim
-        k = _rows(d_keys, dtype, strides, heads, dim, batch.total_tokens, "keys")
-        v = _rows(d_values, dtype, strides, heads, dim, batch.total_tokens, "values")
-        if k[1:] != v[1:]:
+        total = batch.total_tokens
+        k, code, token, head = _rows(d_keys, dtype, strides, self._heads, self._dim, total, "keys")
+        v, *other = _rows(d_values, dtype, strides, self._heads, self._dim, total, "values")
+        if other != [code, token, head]:
             raise _bad("keys and values must have the same type and strides")
-        return k[0], v[0], k[1], k[2], k[3]
+        return k, v, code, token, head
 
     def write_dev(self, batch, d_keys, d_values, dtype=None, strides=None, stream=None):
         """Writes the batch's newest tokens, [total_tokens, num_kv_heads,
         head_dim] in f32, bf16 or f16, into their pages."""
         k, v, code, token, head = self._sides(batch, d_keys, d_values, dtype, strides)
         err = _Err()
-        _check(lib().kivi_pages_write_dev(self._h, batch._ref, code, k, v, token, head,
-                                          _stream(stream), C.byref(err)), err)
+        rc = self._write(self._h, batch._ref, code, k, v, token, head, _stream(stream), C.byref(err))
+        if rc:
+            _check(rc, err)
 
     def read_dev(self, batch, d_keys, d_values, dtype=None, strides=None, stream=None):
         """Reads the batch's newest tokens back (whole sequences where cu_tokens
         counts them whole)."""
         k, v, code, token, head = self._sides(batch, d_keys, d_values, dtype, strides)
         err = _Err()
-        _check(lib().kivi_pages_read_dev(self._h, batch._ref, code, k, v, token, head,
-                                         _stream(stream), C.byref(err)), err)
+        rc = self._read(self._h, batch._ref, code, k, v, token, head, _stream(stream), C.byref(err))
+        if rc:
+            _check(rc, err)
 
     def attention_dev(self, batch, d_query, num_q_heads, scale, d_out, window=0, sinks=0, d_lse=None,
                       dtype=None, query_strides=None, out_strides=None, stream=None):
@@ -214,7 +222,7 @@ class KvPages:
         query and out [total_tokens, num_q_heads, head_dim].  With ``window`` a
         token sees its ``window`` last tokens (itself among them) and the first
         ``sinks``.  ``d_lse``: fp32 [total_tokens, num_q_heads] or None."""
-        dim, total = self.config.head_dim, batch.total_tokens
+        dim, total = self._dim, batch.total_tokens
         q, code, qt, qh = _rows(d_query, dtype, query_strides, num_q_heads, dim, total, "query")
         o, ocode, ot, oh = _rows(d_out, dtype, out_strides, num_q_heads, dim, total, "out")
         if ocode != code:
@@ -226,9 +234,10 @@ class KvPages:
                 or tuple(d_lse.shape) != (total, num_q_heads)):
             raise _bad("lse must be contiguous fp32 [total_tokens, num_q_heads]")
         err = _Err()
-        _check(lib().kivi_pages_attention_dev(self._h, batch._ref, code, q, num_q_heads, qt, qh, scale,
-                                              window, sinks, o, ot, oh, _ptr(d_lse),
-                                              _stream(stream), C.byref(err)), err)
+        rc = self._attention(self._h, batch._ref, code, q, num_q_heads, qt, qh, scale, window, sinks, o,
+                             ot, oh, _ptr(d_lse), _stream(stream), C.byref(err))
+        if rc:
+            _check(rc, err)
 
     def status(self):
         """Waits for the device; raises KiviError if a call since the last
