@@ -513,11 +513,12 @@ uint64_t kivi_guard_sequence_length(const kivi_guard *guard);
  * standing for fma(code, scale, zero).
  *
  * The memory is the caller's (a serving engine reserves its pool itself); the
- * handle keeps pointers to it and the scratch of the attention.  Every call is
- * stream-ordered.  Calls on one handle may use several streams: an attention
- * call waits on the device for the handle's previous one, whose scratch it
- * shares (inside a stream capture it does not: order captured calls on one
- * handle yourself).  Writing and attending are ordered by the caller's streams.
+ * handle keeps pointers to it.  Every call is stream-ordered, and calls may use
+ * several streams: all handles of a device share one scratch (40 MB, there while
+ * any handle is) for the attention's partial states, and an attention call on
+ * another stream than the device's previous one waits for that one on the
+ * device.  Inside a stream capture it does not: order captured attention calls of
+ * one device yourself.  Writing and attending are ordered by the caller's streams.
  */
 #define KIVI_DTYPE_F32 0
 #define KIVI_DTYPE_F16 1
@@ -583,7 +584,9 @@ int32_t kivi_pages_read_dev(const kivi_pages *pages, const kivi_pages_batch *bat
  * dtype (F16 or BF16) is the type of d_query and d_out and, for 16-bit pages,
  * the store's.  Strides in elements; d_lse, when not null, gets the rows'
  * natural log-sum-exp [total_tokens][num_q_heads] (-inf where nothing is seen),
- * with which outputs over disjoint tokens can be joined. */
+ * with which outputs over disjoint tokens can be joined.  Up to 256 query heads
+ * per kv head and, unless max_tokens is 1 with at most 8 of them, 16384
+ * sequences; more is KIVI_ERR_UNSUPPORTED. */
 int32_t kivi_pages_attention_dev(kivi_pages *pages, const kivi_pages_batch *batch, int32_t dtype,
                                  const void *d_query, uint64_t num_q_heads,
                                  uint64_t query_token_stride, uint64_t query_head_stride,

@@ -2824,16 +2824,69 @@ int32_t kivi_guard_append(kivi_guard *g, const float *keys, uint64_t keys_len, c
 
 // ---------------------------------------------------------------- paged store
 
-struct kivi_pages {
-    kivi::PagesStore st{};
+namespace {
+
+// The attention's scratch, one per device for all its handles (a model has one handle a
+// layer): 40 MB of partial states.  A call on another stream than the last one's first
+// waits for that one on the device.
+struct PagesScratch {
     int device = 0;
-    float *scratch = nullptr;   // the attention's partial states
-    int64_t scratch_floats = 0;
-    kivi::PagesMaps maps{};
-    cudaEvent_t done = nullptr; // after the last attention call outside a capture
+    uint64_t refs = 0;
+    float *p = nullptr;
+    int64_t floats = 0;
+    cudaEvent_t done = nullptr;  // after the last attention call outside a capture
     cudaStream_t last = nullptr; // its stream
     bool used = false;
     std::mutex mu;
+};
+std::mutex g_pages_mu;
+PagesScratch *g_pages_scratch[kMaxHintDevices] = {nullptr};
+
+void free_scratch(PagesScratch *x) {
+    dfree(x->p);
+    if (x->done) cudaEventDestroy(x->done);
+    delete x;
+}
+
+// The current device's scratch, with one more reference.
+cudaError_t acquire_scratch(int device, PagesScratch **out) {
+    *out = nullptr;
+    if (device < 0 || device >= kMaxHintDevices) return cudaErrorInvalidDevice;
+    std::lock_guard<std::mutex> lk(g_pages_mu);
+    PagesScratch *x = g_pages_scratch[device];
+    if (!x) {
+        x = new (std::nothrow) PagesScratch();
+        if (!x) return cudaErrorMemoryAllocation;
+        x->device = device;
+        cudaError_t e;
+        if ((e = kivi::pages_scratch_floats(&x->floats)) != cudaSuccess ||
+            (e = dalloc(&x->p, (size_t)x->floats)) != cudaSuccess ||
+            (e = cudaMemset(x->p + x->floats - kivi::kPagesCounters, 0, kivi::kPagesCounters * sizeof(float))) != cudaSuccess ||
+            (e = cudaEventCreateWithFlags(&x->done, cudaEventDisableTiming)) != cudaSuccess) {
+            free_scratch(x);
+            return e;
+        }
+        g_pages_scratch[device] = x;
+    }
+    ++x->refs;
+    *out = x;
+    return cudaSuccess;
+}
+
+void release_scratch(PagesScratch *x) {
+    std::lock_guard<std::mutex> lk(g_pages_mu);
+    if (--x->refs) return;
+    g_pages_scratch[x->device] = nullptr;
+    free_scratch(x); // cudaFree waits for queued calls
+}
+
+} // namespace
+
+struct kivi_pages {
+    kivi::PagesStore st{};
+    int device = 0;
+    kivi::PagesMaps maps{};
+    PagesScratch *scratch = nullptr;
 };
 
 namespace {
@@ -2963,14 +3016,10 @@ int32_t kivi_pages_new(const kivi_pages_config *config, void *d_keys, void *d_va
     st.vp = config->bits == 16 ? nullptr : reinterpret_cast<float2 *>(d_value_params);
     h->device = device;
     cudaError_t e;
-    if ((e = kivi::pages_scratch_floats(st, &h->scratch_floats)) != cudaSuccess ||
+    if ((e = acquire_scratch(device, &h->scratch)) != cudaSuccess ||
         (e = dalloc(&st.status, 1)) != cudaSuccess ||
         (e = cudaMemset(st.status, 0, sizeof(unsigned int))) != cudaSuccess ||
-        (e = dalloc(&h->scratch, (size_t)h->scratch_floats)) != cudaSuccess ||
-        (e = cudaMemset(h->scratch + h->scratch_floats - kivi::kPagesCounters, 0,
-                        kivi::kPagesCounters * sizeof(float))) != cudaSuccess ||
-        (st.bits == 16 && (e = kivi::pages_tensor_maps(st, &h->maps)) != cudaSuccess) ||
-        (e = cudaEventCreateWithFlags(&h->done, cudaEventDisableTiming)) != cudaSuccess) {
+        (st.bits == 16 && (e = kivi::pages_tensor_maps(st, &h->maps)) != cudaSuccess)) {
         rc = cuda_fail(err, e, "kivi_pages_new");
         kivi_pages_free(h);
         return rc;
@@ -2982,10 +3031,8 @@ int32_t kivi_pages_new(const kivi_pages_config *config, void *d_keys, void *d_va
 void kivi_pages_free(kivi_pages *h) {
     if (!h) return;
     DeviceGuard dg(h->device);
-    // queued calls still use the status word and the scratch: cudaFree waits for them
-    dfree(h->st.status);
-    dfree(h->scratch);
-    if (h->done) cudaEventDestroy(h->done);
+    dfree(h->st.status); // cudaFree waits for queued calls, which still use it
+    if (h->scratch) release_scratch(h->scratch);
     delete h;
 }
 
@@ -3060,21 +3107,25 @@ int32_t kivi_pages_attention_dev(kivi_pages *h, const kivi_pages_batch *batch, i
     a.qsign = std::signbit(scale) ? -1.0f : 1.0f;
     a.window = (int)std::min<uint64_t>(window, 0x7fffffffull);
     a.sinks = window ? (int)std::min<uint64_t>(sinks, 0x7fffffffull) : 0;
-    a.part = h->scratch;
-    a.part_floats = h->scratch_floats;
+    a.part = h->scratch->p;
+    a.part_floats = h->scratch->floats;
     a.maps = &h->maps;
+    if (!kivi::pages_attention_supported(a))
+        return set_msg(err, KIVI_ERR_UNSUPPORTED, "%d query heads per kv head and %d sequences: up to 256 and 16384",
+                       a.G, a.b.batch);
     DeviceGuard dg(h->device);
     cudaStream_t st = (cudaStream_t)stream;
-    std::lock_guard<std::mutex> lk(h->mu);
+    PagesScratch *x = h->scratch;
+    std::lock_guard<std::mutex> lk(x->mu);
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     CUDA_TRY(cudaStreamIsCapturing(st, &cap), "pages_attention");
     const bool live = cap == cudaStreamCaptureStatusNone;
-    if (live && h->used && h->last != st) CUDA_TRY(cudaStreamWaitEvent(st, h->done, 0), "pages_attention");
+    if (live && x->used && x->last != st) CUDA_TRY(cudaStreamWaitEvent(st, x->done, 0), "pages_attention");
     CUDA_TRY(kivi::launch_pages_attention(a, st), "pages_attention");
     if (live) {
-        CUDA_TRY(cudaEventRecord(h->done, st), "pages_attention");
-        h->last = st;
-        h->used = true;
+        CUDA_TRY(cudaEventRecord(x->done, st), "pages_attention");
+        x->last = st;
+        x->used = true;
     }
     return set_err(err, KIVI_OK);
 }

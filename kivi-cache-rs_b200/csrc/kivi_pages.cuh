@@ -83,7 +83,7 @@ struct PagesAttn {
     float scale;        // >= 0; a negative scale is folded into qsign
     float qsign;
     int window, sinks;  // window 0: everything up to the row's own token
-    float *part;        // scratch of kivi_pages handles
+    float *part;        // the device's scratch
     int64_t part_floats;
     const PagesMaps *maps;
 };
@@ -124,16 +124,18 @@ cudaError_t launch_pages_write(const PagesStore &st, const PagesBatch &b, const 
 cudaError_t launch_pages_read(const PagesStore &st, const PagesBatch &b, const PagesDense &x,
                               cudaStream_t s);
 cudaError_t launch_pages_attention(const PagesAttn &a, cudaStream_t s);
-// Scratch that a handle keeps for launch_pages_attention on this device: partial
+// Scratch of launch_pages_attention on the current device, for any store: partial
 // states, then kPagesCounters counters, zeroed once and left zero by every call.
 constexpr int kPagesCounters = 2048;
-cudaError_t pages_scratch_floats(const PagesStore &st, int64_t *floats);
+cudaError_t pages_scratch_floats(int64_t *floats);
+bool pages_attention_supported(const PagesAttn &a);
 // One newest token per sequence, at most eight query heads per kv head
 // (kivi_pages_decode.cu).
 bool pages_decode_supported(const PagesAttn &a);
+int64_t pages_decode_scratch(int sms); // floats
 // Anything else (kivi_pages_chunk.cu).
 bool pages_chunk_supported(const PagesAttn &a);
-int64_t pages_chunk_scratch(int D, int sms); // floats
+int64_t pages_chunk_scratch(int sms); // floats
 cudaError_t pages_tensor_maps(const PagesStore &st, PagesMaps *maps);
 cudaError_t launch_pages_chunk(const PagesAttn &a, cudaStream_t s);
 cudaError_t launch_pages_decode(const PagesAttn &a, cudaStream_t s);

@@ -1453,14 +1453,14 @@ template <int BITS, bool F16> cudaError_t by_dim(const PagesAttn &a, int sms, cu
 // prefix lies in shared memory while the list is built.
 bool pages_chunk_supported(const PagesAttn &a) { return a.G <= 2 * kRows && a.b.batch <= 16384; }
 
-int64_t pages_chunk_scratch(int D, int sms) { return (int64_t)sms * 2 * kPartFloats(D); }
+int64_t pages_chunk_scratch(int sms) { return (int64_t)sms * 2 * kPartFloats(128); }
 
 cudaError_t launch_pages_chunk(const PagesAttn &a, cudaStream_t s) {
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return e;
-    if (sms > kPagesCounters || pages_chunk_scratch(a.st.D, sms) > a.part_floats - kPagesCounters)
+    if (sms > kPagesCounters || pages_chunk_scratch(sms) > a.part_floats - kPagesCounters)
         return cudaErrorInvalidConfiguration;
     ProfScope prof("pages_chunk", s);
     count_launch();

@@ -691,6 +691,8 @@ template <int BITS, bool F16> cudaError_t by_dim(const PagesAttn &a, cudaStream_
 
 } // namespace
 
+int64_t pages_decode_scratch(int sms) { return (int64_t)sms * 4 * 2 * kMaxG * (128 + 2); }
+
 bool pages_decode_supported(const PagesAttn &a) { return a.b.most == 1 && a.G <= kMaxG; }
 
 cudaError_t launch_pages_decode(const PagesAttn &a, cudaStream_t s) {

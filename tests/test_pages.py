@@ -488,3 +488,88 @@ def test_nothing_to_do(env):
     c.store.write_dev(c.step, x, x)
     c.store.read_dev(c.step, x, x)
     c.store.status()
+
+
+def test_refusals(env):
+    """Refused before anything is launched, output untouched."""
+    torch, K = env
+    c = Case(env, [1, 2], [30, 40], heads=2, group=2, dim=64)
+    q = c.queries()
+    out = torch.zeros_like(q)
+    before = K.kernel_launches()
+
+    def refused(variant, call):
+        with pytest.raises(K.KiviError) as e:
+            call()
+        assert e.value.variant == variant, e.value
+
+    attend = c.store.attention_dev
+    refused("QueryHeads", lambda: attend(c.step, q[:, :3], 3, 0.1, out[:, :3]))
+    refused("InvalidArgument", lambda: attend(c.step, q[:2], 4, 0.1, out))              # shape
+    refused("InvalidArgument", lambda: attend(c.step, q, 4, 0.1, out.half()))           # types differ
+    refused("InvalidArgument", lambda: attend(c.step, q.half(), 4, 0.1, out.half()))    # not the pages'
+    refused("Unsupported", lambda: attend(c.step, q.float(), 4, 0.1, out.float()))
+    refused("InvalidArgument", lambda: attend(c.step, q.mT.contiguous().mT, 4, 0.1, out))  # strided elements
+    refused("InvalidArgument", lambda: attend(c.step, q, 4, 0.1, out[:, :1].expand(3, 4, 64)))  # rows overlap
+    refused("InvalidArgument", lambda: attend(c.step, q, 4, 0.1, out, window=-1))
+    refused("InvalidArgument", lambda: attend(c.step, q, 4, 0.1, out, d_lse=torch.zeros(3, 4)[:, ::2]))
+    refused("InvalidArgument", lambda: attend(c.step, None, 4, 0.1, None, dtype="bf16"))
+    refused("InvalidArgument", lambda: c.store.write_dev(c.step, q[:, :2], q[:, :2].half()))
+    refused("InvalidArgument", lambda: c.store.write_dev(c.step, q, q))                 # four heads, not two
+    refused("InvalidArgument", lambda: c.store.read_dev(c.step, out[:, :1].expand(3, 2, 64), out[:, :1].expand(3, 2, 64)))
+    wide = torch.zeros(3, 2 * 257, 64, dtype=c.dtype, device="cuda")
+    refused("Unsupported", lambda: attend(c.step, wide, 2 * 257, 0.1, wide))
+    with pytest.raises(K.KiviError):
+        K.KvPages(c.config, c.data[0][:1], c.data[1])                                   # too little memory
+    assert K.kernel_launches() == before and bool((out == 0).all())
+
+
+def test_handles_share_a_device(env):
+    """Two stores attending in turn on two streams, and one freed between."""
+    torch, K = env
+    a, b = Case(env, seed=1, **CHUNK[3]), Case(env, bits=8, seed=2, **DECODE[6])
+    qa, qb = a.queries(), b.queries()
+    wa, wb = a.attend(qa, 0.1)[0], b.attend(qb, 0.1)[0]
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = [(torch.empty_like(qa), torch.empty_like(qb)) for _ in range(8)]
+    torch.cuda.synchronize()
+    for oa, ob in outs:
+        a.store.attention_dev(a.step, qa, a.heads * a.group, 0.1, oa, stream=s)
+        b.store.attention_dev(b.step, qb, b.heads * b.group, 0.1, ob, stream=t)
+    torch.cuda.synchronize()
+    assert all(torch.equal(oa, wa) and torch.equal(ob, wb) for oa, ob in outs)
+    a.store.close()
+    assert torch.equal(b.attend(qb, 0.1)[0], wb)
+
+
+def test_broadcast_inputs(env):
+    """One row written to every token and head (strides 0)."""
+    torch, K = env
+    c = Case(env, [5], [5], heads=3, dim=32, bits=8)
+    row = torch.randn(1, 1, 32, device="cuda").to(c.dtype)
+    c.store.write_dev(c.step, row.expand(5, 3, 32), row.expand(5, 3, 32))
+    k, v = torch.empty(5, 3, 32, dtype=c.dtype, device="cuda"), torch.empty(5, 3, 32, dtype=c.dtype, device="cuda")
+    c.store.read_dev(c.step, k, v)
+    assert bool((k == k[:1, :1]).all()) and torch.equal(k, v) and bool(((k - row).abs() <= 0.05).all())
+
+
+def test_many_short_sequences(env):
+    """More sequences than a CTA has threads, decode and chunks."""
+    torch, K = env
+    for new in ([1] * 700, [i % 4 for i in range(700)]):
+        c = Case(env, new, [max(n, i % 37) for i, n in enumerate(new)], heads=1, group=2, dim=32)
+        c.check(c.queries(), 0.2)
+
+
+def test_example_runs(env):
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "kivi-cache-rs_b200", "examples",
+                        "paged_serving.py")
+    spec = importlib.util.spec_from_file_location("paged_serving", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    for bits in (16, 8, 4):
+        worst = mod.serve(bits=bits, sequences=3, prompt=150, steps=4, window=64, sinks=4, page_size=16)
+        assert worst <= 0.05, (bits, worst)
