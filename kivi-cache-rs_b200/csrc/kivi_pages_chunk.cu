@@ -1383,22 +1383,36 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                 for (int h2 = 0; h2 < 2; ++h2) {
                     const int r = 64 * (warp - kFixWarp) + 32 * h2 + lane;
                     const bool seen = token_seen(a, s.k, T + r);
-                    bool bad = false;
-#pragma unroll 4
-                    for (int c = 0; c < D / 8; ++c) {
-                        uint4 *q = reinterpret_cast<uint4 *>(v + (c >> 3) * kPanel + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-                        uint4 x = *q;
-                        uint32_t *e = reinterpret_cast<uint32_t *>(&x);
-                        bool hit = !seen;
-                        if (!seen) x = make_uint4(0, 0, 0, 0);
+                    constexpr uint32_t ex = F16 ? 0x7c00u : 0x7f80u; // all exponent bits: not finite
+                    unsigned char *rowp = v + r * 128;
+                    auto chunk = [&](int c) { return reinterpret_cast<uint4 *>(rowp + (c >> 3) * kPanel + (((c & 7) ^ (r & 7)) << 4)); };
+                    // the row's largest magnitude pattern first; its elements one by one only
+                    // where that is not finite
+                    uint32_t most = 0;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            constexpr uint32_t ex = F16 ? 0x7c00u : 0x7f80u; // all exponent bits: not finite
-                            if ((e[i] & ex) == ex) e[i] &= 0xffff0000u, hit = bad = true;
-                            if ((e[i] >> 16 & ex) == ex) e[i] &= 0x0000ffffu, hit = bad = true;
-                        }
-                        if (hit) *q = x;
+                    for (int c = 0; c < D / 8; ++c) {
+                        const uint4 x = *chunk(c);
+                        most = __vmaxu2(most, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
+                                                       __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
                     }
+                    const bool bad = seen && ((most & 0xffffu) >= ex || (most >> 16) >= ex);
+                    if (!seen) {
+#pragma unroll
+                        for (int c = 0; c < D / 8; ++c) *chunk(c) = make_uint4(0, 0, 0, 0);
+                    } else if (bad) {
+#pragma unroll 1
+                        for (int c = 0; c < D / 8; ++c) {
+                            uint4 x = *chunk(c);
+                            uint32_t *e = reinterpret_cast<uint32_t *>(&x);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if ((e[i] & ex) == ex) e[i] &= 0xffff0000u;
+                                if ((e[i] >> 16 & ex) == ex) e[i] &= 0x0000ffffu;
+                            }
+                            *chunk(c) = x;
+                        }
+                    }
+                    __syncwarp();
                     const uint32_t bits = __ballot_sync(0xffffffffu, bad);
                     if (lane == 0) sh.flags[ne & 3][2 * (warp - kFixWarp) + h2] = bits;
                 }
