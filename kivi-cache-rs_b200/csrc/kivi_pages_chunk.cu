@@ -29,8 +29,26 @@
 // mix of lengths.  A (block, head) that spans CTAs leaves partial states in the
 // handle's scratch; the CTA that finishes last joins them in CTA order.
 //
-// Warps: 0-3 softmax of A, 4-7 of B, 8 MMA issue, 9 copies (TMA tensor maps over
-// the pages, a box per page and 64 channels), 10-11 the masked tiles' V rows.
+// Warps: 0-3 softmax of A, 4-7 of B, 8 MMA issue, 9 the run's segments and the copies
+// (TMA tensor maps over the pages, a box per page and 64 channels), 10-11 the masked
+// tiles' V rows.  8- and 4-bit pages: instead of copies, warps 10-15 turn the codes into
+// f16 operand tiles in shared memory, each tile's keys and values scaled by a power of
+// two into f16's upper end (undone in the softmax's factor and O's exponent).
+//
+// What bounds it: per cached tile and pair of row tiles the tensor pipe has 2048 cycles
+// of work and the special function unit as many exponentials (three quarters of them
+// stay there, one quarter are polynomials on the FMA pipe), but a row tile's chain S ->
+// softmax -> P V -> next S is about 3400: a 2048-token chunk over 10240 bf16 tokens, 32
+// heads over 8, takes 291 us in short bursts and 333 us back to back (1.06 and 0.93
+// PFLOP/s, tensor pipe 49% active), an 8192-token prompt under a window of 1024 245 us, of which a block's start and end (queries in, rows out,
+// about 20000 cycles for every 10 tiles) are half.  With 8-bit pages ragged 1024-token
+// chunks over 8000 take 709 us (0.54 PFLOP/s): the converting warps share the issue slots
+// with the softmax (529 us without the conversion's arithmetic, 457 us without its
+// loads as well).
+// Measured and left out: 16 softmax warps, two to a row (301-319 us for the chunk above);
+// S in halves of 64 tokens, double-buffered (310 us; 416 us with the next half's maximum
+// taken between the exponentials); half or none of the exponentials on the FMA pipe (314
+// us each).
 #include <cudaTypedefs.h>
 #include <math.h>
 

@@ -20,8 +20,12 @@
 // instructions); a row's query is scaled by a power of two into f16's upper end, and
 // the weights by one that follows the largest value scale met, both undone in fp32.
 //
-// What bounds it: HBM.  Per token and kv head 4 D bytes (16-bit), 2 D + 16
-// (8-bit), D + 16 (4-bit), each read once.
+// What bounds it: HBM for 16-bit pages (per token and kv head 4 D bytes, each read
+// once: 16 x 32768 tokens of 8 x 128 in 318 us, 6.7 TB/s; under a window of 4096 and 4
+// first tokens, 270 MB, 52 us).  For codes (2 D + 16 and D + 16 bytes) the work of taking
+// them apart: 433 warp instructions per 16 tokens at 4 bits, 223 of them on the half-rate
+// integer pipe, so 141 us for 396 MB (2.8 TB/s; issue slots and that pipe 54% busy).
+// More CTAs per SM (spills, or 16-token tiles) and larger tiles were no faster.
 //
 // Split: the visible tokens of all (sequence, kv head) rows form one flat list
 // of tiles, and CTA i takes tiles [i per, (i + 1) per): one wave, no tail, any
@@ -675,7 +679,8 @@ cudaError_t launch_decode(const PagesAttn &a, cudaStream_t s) {
     int *counters = reinterpret_cast<int *>(a.part + a.part_floats) - kPagesCounters;
     if (grid > kPagesCounters || (int64_t)grid * 2 * kMaxG * (32 * ND + 2) > a.part_floats - kPagesCounters)
         return cudaErrorInvalidConfiguration;
-    // a CTA takes at least two tiles per warp: fewer make more parts to join
+    // a CTA takes at least two tiles per warp: fewer make more parts to join (one sequence
+    // of 4096 8-bit tokens: 16.6 us with two, 16.1 us with one, 20.9 us with four)
     return launch_pdl(pages_decode_kernel<BITS, ND, F16>, dim3((unsigned)grid), dim3(kThreads), 0, s, true, a,
                       2 * kWarps, counters);
 }
