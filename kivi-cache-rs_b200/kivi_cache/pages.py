@@ -81,9 +81,10 @@ def _rows(x, dtype, strides, heads, dim, total, what):
             raise _bad(f"{what}: unsupported element type {x.dtype}")
         _types[x.dtype] = code
     token, head, inner = x.stride()
-    if inner != 1:
+    if inner != 1 and total:
         raise _bad(f"{what}: the elements of a row must be contiguous, their stride is {inner}")
-    return x.data_ptr(), code, token, head
+    # the stride of a dimension of one says nothing
+    return x.data_ptr(), code, token if total > 1 else heads * dim, head if heads > 1 and total else dim
 
 
 @dataclass(frozen=True)
