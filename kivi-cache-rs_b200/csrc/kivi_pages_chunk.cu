@@ -1089,7 +1089,10 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
             tc_after();
             float fa = kCodes ? exp2i(eref) : 1.0f, fb = 0.0f;
             if (dual) {
-                float2 *ml = reinterpret_cast<float2 *>(sq + NP * kPanel); // B's query tile is not in use
+                // through B's query tile, not in use here; the last segment's rows may still be
+                // on their way out through it until all warps are here
+                if (!(ok = ok && meet())) break;
+                float2 *ml = reinterpret_cast<float2 *>(sq + NP * kPanel);
                 float *fx = reinterpret_cast<float *>(ml + kRows);
                 if (X) ml[row] = make_float2(m, l), fx[row] = fa;
                 if (!(ok = ok && meet())) break;

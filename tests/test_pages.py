@@ -295,6 +295,7 @@ CHUNK = [
     dict(new=[400], kv=[3777], group=4, page=64),
     dict(new=[90, 260], kv=[2600, 1311], group=6, heads=3, dim=64, page=16),
     dict(new=[1100], kv=[1100], group=1, heads=1, page=256),
+    dict(new=[214, 61, 1], kv=[2601, 62, 1], group=33, heads=3, dim=96, page=32),  # short blocks after long ones
     dict(new=[2], kv=[0], group=33, heads=1, dim=64, page=256),
 ]
 MASKS = [(1, 0), (1, 3), (17, 0), (64, 4), (100, 21), (128, 200), (5000, 4)]
