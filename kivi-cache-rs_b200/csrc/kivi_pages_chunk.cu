@@ -951,6 +951,8 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.q_full[X]);
             }
+            // B's query tile is to take B's (m, l): the last segment's rows are out of it
+            if (dual && !(ok = meet())) break;
             const int n = dual ? s.n : nX;
             Tiles tl(a, s);
             uint32_t edges = s.edges; // edge tiles of the run up to this one
@@ -1089,9 +1091,7 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
             tc_after();
             float fa = kCodes ? exp2i(eref) : 1.0f, fb = 0.0f;
             if (dual) {
-                // through B's query tile, not in use here; the last segment's rows may still be
-                // on their way out through it until all warps are here
-                if (!(ok = ok && meet())) break;
+                // through B's query tile, not in use here
                 float2 *ml = reinterpret_cast<float2 *>(sq + NP * kPanel);
                 float *fx = reinterpret_cast<float *>(ml + kRows);
                 if (X) ml[row] = make_float2(m, l), fx[row] = fa;
