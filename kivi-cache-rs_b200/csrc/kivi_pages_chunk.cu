@@ -469,6 +469,16 @@ __device__ __forceinline__ float exp2i(int k) { return __uint_as_float((uint32_t
 // e with x 2^-e < 2^14 for x >= 0 (the upper end of f16, so that what is far smaller
 // than x keeps its bits too); -126 at least
 __device__ __forceinline__ int f16_exponent(float x) { return max(-126, (int)(__float_as_uint(x) >> 23) - 140); }
+// c 2^e, a score's exp2 units, for e between -252 and 230: positive and finite where c is
+// a number, since a hidden score is -inf and the scores of zero queries or keys (whose
+// exponents are the least there are) are 0, and neither may become NaN by it.
+__device__ __forceinline__ float score_units(float c, int e) {
+    const int h = e >> 1;
+    float y = c * __uint_as_float((uint32_t)(h + 127) << 23) * __uint_as_float((uint32_t)(e - h + 127) << 23);
+    asm("max.NaN.f32 %0, %0, 0f00800000;" : "+f"(y)); // 2^-126
+    asm("min.NaN.f32 %0, %0, 0f7f7fffff;" : "+f"(y));
+    return y;
+}
 
 // Rows of V that are not finite were taken out of an edge tile (flags, one bit
 // per token); they are added here to the rows that see them: p > 0, so p v is v.
@@ -958,6 +968,7 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
             uint32_t edges = s.edges; // edge tiles of the run up to this one
             float crow = c2;          // a score's exp2 units
             int eref = 0;             // O's exponent
+            int kref = 0;             // the keys' exponent in crow
             bool began = false;
             for (int j = 0; j < n; ++j) {
                 const int T = tl.token(j);
@@ -974,7 +985,10 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                     const uint32_t tile = s.item / 2 + j;
                     if (!(ok = warp_wait(&sh.range[tile & 3], tile >> 2 & 1, status))) break;
                     // B has A's queries where it shares its rows, loaded before the first S
-                    crow = c2 * exp2i(sc.qexp[(dual ? 0 : X * kRows) + row]) * exp2i(sc.kexp[tile & 3]);
+                    if (const int ke = sc.kexp[tile & 3]; !began || ke != kref) {
+                        kref = ke;
+                        crow = score_units(c2, sc.qexp[(dual ? 0 : X * kRows) + row] + ke);
+                    }
                     const int e = sc.vexp[tile & 3];
                     if (!began || e > eref) {
                         if (began) raise = true, fo = exp2i(eref - e);
