@@ -453,7 +453,9 @@ struct Shared {
 };
 
 // Codes: the operands are f16, a tile's keys and values times 2^-exponent (largest
-// finite one below 2^14), a row's query likewise, and a token's (scale, centre).
+// finite one below 2^14; of the values' kKeep more are left free rather than O moved),
+// a row's query likewise, and a token's (scale, centre).
+constexpr int kKeep = 6;
 struct SharedCodes {
     int kexp[4], vexp[4];  // of tile counter & 3
     float most[2][4][2];   // a tile's largest key and value per warp, by tile parity
@@ -478,6 +480,52 @@ __device__ __forceinline__ float score_units(float c, int e) {
     asm("max.NaN.f32 %0, %0, 0f00800000;" : "+f"(y)); // 2^-126
     asm("min.NaN.f32 %0, %0, 0f7f7fffff;" : "+f"(y));
     return y;
+}
+
+// A tile's weights times 2^k, where O could not go to its values' exponent.
+__device__ __noinline__ void scale_weights(uint32_t cS, int k) {
+    const __half2 f = __float2half2_rn(exp2i(k));
+    st_wait();
+#pragma unroll 1
+    for (int c = 0; c < kTok / 2; c += 16) {
+        float w[16];
+        tmem_ld16(cS + c, w);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            __half2 *h = reinterpret_cast<__half2 *>(w + i);
+            *h = __hmul2(*h, f);
+        }
+        tmem_st16(cS + c, reinterpret_cast<const uint32_t *>(w));
+    }
+}
+
+// O and its exponents (one a row) go to a tile's values' exponent e, or, where O would
+// leave fp32's range by that, as near as it can: the new exponents.
+template <int ND> __device__ __noinline__ int move_exponent(uint32_t cO, int eref, int e) {
+    uint32_t most = 0;
+    if (__any_sync(0xffffffffu, e < eref)) {
+#pragma unroll 1
+        for (int c = 0; c < 32 * ND; c += 16) {
+            float o[16];
+            tmem_ld16(cO + c, o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = max(most, __float_as_uint(fabsf(o[i])));
+        }
+    }
+    int n = e;
+    if (e < eref && most > 0 && most < 0x7f800000u) n = min(max(e, eref + (int)(most >> 23) - 227), eref); // below 2^101
+    const int d = eref - n, h = d >> 1;
+    const float f0 = exp2i(h), f1 = exp2i(d - h);
+#pragma unroll 1
+    for (int c = 0; c < 32 * ND; c += 16) {
+        float o[16];
+        tmem_ld16(cO + c, o);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] *= f0, o[i] *= f1;
+        tmem_st16(cO + c, reinterpret_cast<const uint32_t *>(o));
+    }
+    st_wait();
+    return n;
 }
 
 // Rows of V that are not finite were taken out of an edge tile (flags, one bit
@@ -969,7 +1017,6 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
             float crow = c2;          // a score's exp2 units
             int eref = 0;             // O's exponent
             int kref = 0;             // the keys' exponent in crow
-            bool began = false;
             for (int j = 0; j < n; ++j) {
                 const int T = tl.token(j);
                 const bool edge = tl.edge(T);
@@ -978,24 +1025,23 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                 if (!(ok = warp_wait(&sh.s_full[X], ns & 1, status))) break;
                 ++ns;
                 tc_after();
-                int shift = 0; // of this tile's values against O's
-                bool raise = false;
-                float fo = 1.0f;
+                bool late = edge; // the weights go out in one piece
                 if constexpr (kCodes) {
                     const uint32_t tile = s.item / 2 + j;
                     if (!(ok = warp_wait(&sh.range[tile & 3], tile >> 2 & 1, status))) break;
                     // B has A's queries where it shares its rows, loaded before the first S
-                    if (const int ke = sc.kexp[tile & 3]; !began || ke != kref) {
+                    const bool first = j < (dual ? 2 : 1);
+                    if (const int ke = sc.kexp[tile & 3]; first || ke != kref) {
                         kref = ke;
                         crow = score_units(c2, sc.qexp[(dual ? 0 : X * kRows) + row] + ke);
                     }
                     const int e = sc.vexp[tile & 3];
-                    if (!began || e > eref) {
-                        if (began) raise = true, fo = exp2i(eref - e);
+                    if (first) {
                         eref = e;
+                    } else if (any && __any_sync(0xffffffffu, e != eref)) {
+                        eref = move_exponent<ND>(cO, eref, e);
+                        late |= __any_sync(0xffffffffu, e != eref);
                     }
-                    began = true;
-                    shift = e - eref;
                 }
                 if (any) {
                     // The row's scores; with codes, whose converting warps take a share of the
@@ -1037,11 +1083,10 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                     const float mx = max3(max3(m4[0], m4[1], m4[2]), m4[3], m4[3]) * crow;
                     // a NaN score makes the reference, and with it the row, NaN
                     const bool need = !(mx <= m + kLazy), move = need && m != -INFINITY;
-                    float f = move ? ex2(m - mx) : 1.0f;
+                    const float f = move ? ex2(m - mx) : 1.0f;
                     if (need) m = mx;
-                    if (raise || __any_sync(0xffffffffu, move)) {
+                    if (__any_sync(0xffffffffu, move)) {
                         l *= f;
-                        f *= fo;
                         // every O += P V of earlier tiles is complete: S of this one was issued after them
 #pragma unroll 1
                         for (int c = 0; c < D; c += 16) {
@@ -1052,7 +1097,7 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                             tmem_st16(cO + c, reinterpret_cast<const uint32_t *>(o));
                         }
                     }
-                    const float off = (m == -INFINITY ? 0.0f : -m) + (kCodes ? (float)shift : 0.0f);
+                    const float off = m == -INFINITY ? 0.0f : -m;
                     float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
 #pragma unroll
                     for (int hlf = 0; hlf < 2; ++hlf) {
@@ -1080,11 +1125,14 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                             tc_before();
                             __syncwarp();
                             // (an edge tile's V may still change, and its O)
-                            if (lane == 0 && !edge) bar_arrive(&sh.h_full[X]);
+                            if (lane == 0 && !late) bar_arrive(&sh.h_full[X]);
                         }
                     }
-                    const float sum = (a0 + a1) + (a2 + a3);
-                    l += kCodes ? sum * exp2i(-shift) : sum;
+                    l += (a0 + a1) + (a2 + a3);
+                    if (kCodes && late) {
+                        const int e = sc.vexp[(s.item / 2 + j) & 3];
+                        if (__any_sync(0xffffffffu, e != eref)) scale_weights(cS, e - eref);
+                    }
                 }
                 if (edge) { // the tile's V has been through the fixing warps
                     const uint32_t it = s.item + 2 * j + 1;
@@ -1096,7 +1144,7 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                 tc_before();
                 __syncwarp();
                 if (lane == 0) {
-                    if (edge || !any) bar_arrive(&sh.h_full[X]);
+                    if (late || !any) bar_arrive(&sh.h_full[X]);
                     bar_arrive(&sh.p_full[X]);
                 }
             }
@@ -1330,6 +1378,7 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
         while (ok && next_seg()) {
             const Seg &s = *sp;
             uint32_t ne = s.edges;
+            int ve = 0; // the values' exponent
             int T = tile_token(s.k, s.t0);
             int rows = rows_of(s, T, lookup(s, T));
             params(s, T, rows);
@@ -1361,7 +1410,10 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                 float kmost = 0.0f, vmost = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) kmost = fmaxf(kmost, sc.most[tile & 1][i][0]), vmost = fmaxf(vmost, sc.most[tile & 1][i][1]);
-                const int ke = f16_exponent(kmost), ve = f16_exponent(vmost);
+                const int ke = f16_exponent(kmost), own = f16_exponent(vmost);
+                // O moves when this does, so it starts with room for values four times as
+                // large, and stays while they fit and lose nothing by it; zeros take any
+                if (j == 0 || own > ve || (own < ve - kKeep && vmost > 0.0f)) ve = min(own + 2, 127);
                 if (ct == 0) {
                     sc.kexp[tile & 3] = ke, sc.vexp[tile & 3] = ve;
                     bar_arrive(&sh.range[tile & 3]);

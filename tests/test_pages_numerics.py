@@ -37,3 +37,53 @@ def test_scale_zero(env, bits, size):
     c = Case(env, [70], [200], heads=1, bits=bits)
     rewrite(c, k=c.k * size)
     c.check(c.queries() * size, 0.0)
+
+
+# ------------------------------------------------------------------ values of unlike size
+
+
+@pytest.mark.parametrize("bits,kind", [(16, "bf16"), (8, "bf16"), (8, "f16"), (4, "bf16")])
+@pytest.mark.parametrize("new", [1, 70, 300])
+@pytest.mark.parametrize("sizes", [(1, 0), (100, 0), (1000, 0), (0, 1000), (1, 1000, 1e-3), (0, 0)])
+def test_runs_of_unlike_values(env, bits, kind, new, sizes):
+    """128 tokens of one size after 128 of another, zeros among them: outputs and
+    log-sum-exps, causal and under a window."""
+    torch, K = env
+    c = Case(env, [new], [800], heads=1, bits=bits, kind=kind)
+    t = torch.arange(800, device="cuda") // 128
+    size = torch.tensor(sizes, device="cuda")[t % len(sizes)].float()
+    rewrite(c, v=c.v * size[:, None, None])
+    q = c.queries()
+    c.check(q, 0.1)
+    c.check(q, 0.1, 200, 140)
+
+
+@pytest.mark.parametrize("bits,kind", [(16, "bf16"), (8, "bf16"), (4, "bf16")])
+@pytest.mark.parametrize("new", [70])
+@pytest.mark.parametrize("big", [1e6, 1e9, 1e12])
+def test_large_values_of_small_weight(env, bits, kind, new, big):
+    """Tokens whose values are far larger and whose weights are as much smaller: what
+    the others give stays exact to its own size."""
+    torch, K = env
+    c = Case(env, [new], [640], heads=1, bits=bits, kind=kind)
+    k, v = c.k.float() * 0.3, c.v.float()
+    large = (torch.arange(640, device="cuda") // 128) % 2 == 0
+    k[:, :, 0] = torch.where(large, -8.0, 0.0)[:, None]
+    v[large] *= big
+    rewrite(c, k=k, v=v)
+    q = c.queries() * 0.3
+    q[:, :, 0] = 1.0
+    c.check(q, math.log(big * 1e3) / 8)
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("sizes", [(1e30, 1e-8), (1e-30, 1e30), (1e30, 0, 1e-30, 1e30)])
+def test_runs_of_extreme_values(env, bits, sizes):
+    """Sums that no exponent of the small values holds."""
+    torch, K = env
+    c = Case(env, [130], [800], heads=1, bits=bits)
+    t = torch.arange(800, device="cuda") // 128
+    size = torch.tensor(sizes, device="cuda")[t % len(sizes)].float()
+    rewrite(c, v=c.v.float() * size[:, None, None])
+    c.check(c.queries(), 0.1)
+    c.check(c.queries(), 0.1, 200, 140)
