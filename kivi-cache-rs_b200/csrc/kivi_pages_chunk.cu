@@ -1081,10 +1081,11 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                         most(x + 64), most(x + 96);
                     }
                     const float mx = max3(max3(m4[0], m4[1], m4[2]), m4[3], m4[3]) * crow;
-                    // a NaN score makes the reference, and with it the row, NaN
+                    // a NaN score makes the reference, and with it the row, NaN; so does an
+                    // infinite one (times 0), whose own weight is infinity less infinity
                     const bool need = !(mx <= m + kLazy), move = need && m != -INFINITY;
                     const float f = move ? ex2(m - mx) : 1.0f;
-                    if (need) m = mx;
+                    if (need) m = fmaf(mx, 0.0f, mx);
                     if (__any_sync(0xffffffffu, move)) {
                         l *= f;
                         // every O += P V of earlier tiles is complete: S of this one was issued after them

@@ -87,3 +87,48 @@ def test_runs_of_extreme_values(env, bits, sizes):
     rewrite(c, v=c.v.float() * size[:, None, None])
     c.check(c.queries(), 0.1)
     c.check(c.queries(), 0.1, 200, 140)
+
+
+# ------------------------------------------------------------------ infinities and NaN
+
+
+@pytest.mark.parametrize("bits,kind,bad", [(16, "bf16", math.inf), (16, "bf16", math.nan), (16, "f16", math.inf),
+                                           (8, "bf16", math.inf), (4, "f16", math.inf)])
+@pytest.mark.parametrize("at", range(8))
+def test_a_score_that_is_not_finite(env, bits, kind, at, bad):
+    """NaN in every channel of the rows that see it, nothing in the others', at each of
+    eight neighbouring tokens (the codec leaves a NaN out of its row's range, so for codes
+    an infinity, whose row's parameters are not finite)."""
+    torch, K = env
+    new, kv, row = 70, 200, 24 + at
+    c = Case(env, [new], [kv], heads=1, bits=bits, kind=kind)
+    q = c.queries()
+    q[:, :, 3] = q[:, :, 3].abs() + 0.5
+    want, wlse = c.attend(q, 0.1)
+    k = c.k.clone()
+    k[kv - new + row, 0, 3] = bad
+    rewrite(c, k=k)
+    got, lse = c.attend(q, 0.1)
+    assert torch.equal(got[:row], want[:row]) and torch.equal(lse[:row], wlse[:row])
+    assert bool(torch.isnan(got[row:]).all()) and bool(torch.isnan(lse[row:]).all())
+    # out of the window again for the last rows
+    got, _ = c.attend(q, 0.1, 16, 2)
+    assert bool(torch.isnan(got[row:row + 16]).all())
+    assert bool(torch.isfinite(got[row + 16:]).all()) and bool(torch.isfinite(got[:row]).all())
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+def test_scores_that_overflow(env, bits):
+    """Finite keys and queries whose product does not fit fp32."""
+    torch, K = env
+    for at in range(8):
+        c = Case(env, [70], [200], heads=1, bits=bits)
+        q = c.queries()
+        q[:, :, 3] = 1e30
+        k = c.k.clone()
+        k[:, :, 3] = 0
+        k[130 + 24 + at, 0, 3] = 1e30
+        rewrite(c, k=k)
+        got, _ = c.attend(q, 1.0)
+        assert bool(torch.isnan(got[24 + at:]).all())
+        assert not bool(torch.isnan(got[:24 + at]).any())
