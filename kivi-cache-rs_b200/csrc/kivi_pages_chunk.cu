@@ -71,6 +71,7 @@ __host__ __device__ constexpr int stages_of(int bits) { return bits == 16 ? 5 : 
 constexpr int kPanel = 16384;             // 128 rows x 64 channels
 constexpr long long kWait = 2000000000LL; // ~1 s
 constexpr float kLazy = 8.0f;
+constexpr float kFar = 16777216.0f;      // 2^24: no bits below 1
 constexpr int kPolyPairs = 1;             // of every four pairs of weights, on the FMA pipe
 // registers of a softmax thread and of the others
 __host__ __device__ constexpr int soft_regs(int bits) { return bits == 16 ? 200 : 144; }
@@ -480,6 +481,24 @@ __device__ __forceinline__ float score_units(float c, int e) {
     asm("max.NaN.f32 %0, %0, 0f00800000;" : "+f"(y)); // 2^-126
     asm("min.NaN.f32 %0, %0, 0f7f7fffff;" : "+f"(y));
     return y;
+}
+
+// A tile's scores, in tensor memory: hidden ones to -inf, in rows whose reference -off is
+// not 0 the others to what times `crow` is their distance from it.  p, lo and sinks count
+// from the tile's first token.
+__device__ __forceinline__ void spread_scores(uint32_t cS, float crow, float off, int p, int lo, int sinks) {
+#pragma unroll 1
+    for (int c = 0; c < kTok; c += 16) {
+        float x[16];
+        tmem_ld16(cS + c, x);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (off != 0.0f) x[i] = __fadd_rn(__fmul_rn(x[i], crow), off) / crow;
+            if (c + i > p || (c + i < lo && c + i >= sinks)) x[i] = -INFINITY;
+        }
+        tmem_st16(cS + c, reinterpret_cast<const uint32_t *>(x));
+    }
+    st_wait();
 }
 
 // A tile's weights times 2^k, where O could not go to its values' exponent.
@@ -1098,7 +1117,22 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                             tmem_st16(cO + c, reinterpret_cast<const uint32_t *>(o));
                         }
                     }
-                    const float off = m == -INFINITY ? 0.0f : -m;
+                    float off = m == -INFINITY ? 0.0f : -m;
+                    // A product is not rounded before m, which is, is taken from it: where m has
+                    // no bits below 1 the row's own largest score would be far from 0, so the
+                    // scores become what times crow is their rounded distance from m.
+                    if (__any_sync(0xffffffffu, fabsf(off) >= kFar)) {
+                        const float ref = fabsf(off) >= kFar ? off : 0.0f;
+                        off -= ref;
+                        if constexpr (kCodes) {
+                            spread_scores(cS, crow, ref, p - T, lo - T, a.sinks - T);
+                            tmem_ld64(cS, x);
+                        } else if (ref != 0.0f) {
+                            const float inv = 1.0f / crow;
+#pragma unroll
+                            for (int i = 0; i < 128; ++i) x[i] = __fmul_rn(__fadd_rn(__fmul_rn(x[i], crow), ref), inv);
+                        }
+                    }
                     float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
 #pragma unroll
                     for (int hlf = 0; hlf < 2; ++hlf) {

@@ -132,3 +132,32 @@ def test_scores_that_overflow(env, bits):
         got, _ = c.attend(q, 1.0)
         assert bool(torch.isnan(got[24 + at:]).all())
         assert not bool(torch.isnan(got[:24 + at]).any())
+
+
+@pytest.mark.parametrize("bits,kind", [(16, "bf16"), (16, "f16"), (8, "bf16"), (4, "bf16")])
+@pytest.mark.parametrize("new", [1, 70, 300])
+@pytest.mark.parametrize("scale", [1e6, -1e6, 1e12, 1e25])
+def test_scores_far_apart(env, bits, kind, new, scale):
+    """Scores past what fp32 holds to the unit: all of a row's weight on its largest one,
+    or shared by the tokens that tie."""
+    torch, K = env
+    c = Case(env, [new], [500], heads=1, bits=bits, kind=kind)
+    k = torch.zeros_like(c.k)
+    k[:, 0, 3] = (1 + torch.arange(500, device="cuda") * 37 % 61) / 61
+    rewrite(c, k=k)
+    q = torch.zeros_like(c.queries())
+    q[:, :, 3] = 1.0 + torch.arange(4, device="cuda") / 4
+    for window, sinks in ((0, 0), (150, 3)):
+        out, _ = c.attend(q, scale, window, sinks)
+        held = [x[0] for x in (c.held(0), c.held(1))]
+        for i in range(new):
+            p = 500 - new + i
+            t = torch.arange(500, device="cuda")
+            see = (t <= p) & ((t > p - window) | (t < sinks) if window else t >= 0)
+            x = held[0][:, 0, 3] * (1 if scale > 0 else -1)
+            x[~see] = -math.inf
+            ties = x >= x.max() - 1e-3
+            v = held[1][ties, 0]
+            u = 2.0**-8 if kind == "bf16" else 2.0**-11
+            tol = (2 * u + 2.0**-10) * v.abs().mean(0) + 2.0**-16
+            assert bool(((out[i].double() - v.mean(0)).abs() <= tol).all())
