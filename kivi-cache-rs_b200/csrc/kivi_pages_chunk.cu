@@ -282,14 +282,16 @@ __device__ __forceinline__ void fma2c(float &a0, float &a1, float x0, float x1, 
         : "+f"(a0), "+f"(a1)
         : "f"(x0), "f"(x1), "f"(c));
 }
-// 2^x of a pair on the FMA pipe, for x <= 8: x = n + f with n an integer and
-// |f| <= 1/2, 2^f by a polynomial of degree 4 (fitted by Remez exchange: relative
-// error 2.6e-6), n added to its exponent.  Below -126: 2^-126.  The special
+// 2^x of a pair on the FMA pipe, for x below 2^6: x = n + f with n an integer and
+// |f| <= 1/2, 2^f by a polynomial of degree 4 that is 1 at 0 (fitted for the least
+// relative error under that: 2.9e-6), n added to its exponent.  So 2^-127, where x ends,
+// comes out as 0: the weight of a hidden score is 0, and a large finite value meets no
+// row that does not see it.  Between -126 and -127 results lie below 2^-126.  The special
 // function unit's 16 results a cycle would take as long for a tile as the tensor
 // pipe does, so some of the tile's weights come from here.
 __device__ __forceinline__ void ex2_pair(float &x0, float &x1) {
     constexpr float magic = 12582912.0f; // 1.5 * 2^23: adding it leaves round(x) in the low bits
-    x0 = fmaxf(x0, -126.0f), x1 = fmaxf(x1, -126.0f);
+    x0 = fmaxf(x0, -127.0f), x1 = fmaxf(x1, -127.0f);
     float t0 = x0, t1 = x1;
     add2(t0, t1, magic, magic);
     float r0 = t0, r1 = t1;
@@ -298,11 +300,11 @@ __device__ __forceinline__ void ex2_pair(float &x0, float &x1) {
         "fma.rn.f32x2 rx, rr, rm, rx;\n\tmov.b64 {%0, %1}, rx;\n\t}" // f = x - n
         : "+f"(x0), "+f"(x1)
         : "f"(r0), "f"(r1), "f"(-1.0f));
-    float p0 = 0.009570102207362652f, p1 = p0;
-    fma2c(p0, p1, x0, x1, 0.05591785907745361f);
-    fma2c(p0, p1, x0, x1, 0.240247443318367f);
-    fma2c(p0, p1, x0, x1, 0.6931217908859253f);
-    fma2c(p0, p1, x0, x1, 0.9999992847442627f);
+    float p0 = 0.009582576341927052f, p1 = p0;
+    fma2c(p0, p1, x0, x1, 0.05590682849287987f);
+    fma2c(p0, p1, x0, x1, 0.24024106562137604f);
+    fma2c(p0, p1, x0, x1, 0.6931241154670715f);
+    fma2c(p0, p1, x0, x1, 1.0f);
     x0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
     x1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }

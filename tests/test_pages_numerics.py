@@ -161,3 +161,23 @@ def test_scores_far_apart(env, bits, kind, new, scale):
             u = 2.0**-8 if kind == "bf16" else 2.0**-11
             tol = (2 * u + 2.0**-10) * v.abs().mean(0) + 2.0**-16
             assert bool(((out[i].double() - v.mean(0)).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("at", range(8))
+@pytest.mark.parametrize("big", [1e38, -3e38])
+def test_a_token_out_of_sight_weighs_nothing(env, at, big):
+    """The largest bf16 values in a newest token, and behind the window: rows that do not
+    see them keep every bit."""
+    torch, K = env
+    new, kv, row = 70, 200, 24 + at
+    c = Case(env, [new], [kv], heads=1)
+    q = c.queries()
+    v = c.v.clone()
+    v[kv - new + row] = big
+    want, _ = c.attend(q, 0.1)
+    wide, _ = c.attend(q, 0.1, 16, 2)
+    rewrite(c, v=v)
+    got, _ = c.attend(q, 0.1)
+    assert torch.equal(got[:row], want[:row])
+    got, _ = c.attend(q, 0.1, 16, 2)
+    assert torch.equal(got[:row], wide[:row]) and torch.equal(got[row + 16:], wide[row + 16:])
