@@ -332,6 +332,10 @@ struct Block {
     int p0, p1;            // positions of the first and last token
     int lo, ns, ws, nt;
 };
+// The token at which the window that ends with position p starts, where there is a window
+// (negative: with the first token; p may lie that far before it that p - window + 1 does
+// not fit 32 bits).
+__device__ __forceinline__ int window_start(const PagesAttn &a, int p) { return max(p, -1) - a.window + 1; }
 __device__ __forceinline__ Block make_block(const PagesAttn &a, int TB, int b, const Span &s, int i) {
     Block k;
     k.b = b, k.start = s.start, k.n = s.n, k.kv = s.kv;
@@ -339,7 +343,7 @@ __device__ __forceinline__ Block make_block(const PagesAttn &a, int TB, int b, c
     k.ntok = min(TB, s.n - k.i0);
     k.p0 = s.kv - s.n + k.i0;
     k.p1 = k.p0 + k.ntok - 1;
-    k.lo = a.window ? max(0, k.p0 - a.window + 1) : 0;
+    k.lo = a.window ? max(0, window_start(a, k.p0)) : 0;
     k.ws = k.lo / kTok;
     k.ns = min((min(a.sinks, k.lo) + kTok - 1) / kTok, k.ws);
     // rows that see nothing still need a tile: it writes their zeros
@@ -419,13 +423,13 @@ __device__ __forceinline__ int tile_token(const Block &k, int t) { return (t < k
 // Some row of the block does not see some token of the tile.
 __device__ __forceinline__ bool tile_edge(const PagesAttn &a, const Block &k, int T) {
     if (T + kTok - 1 > k.p0) return true;
-    return a.window && T < k.p1 - a.window + 1 && T + kTok > a.sinks;
+    return a.window && T < window_start(a, k.p1) && T + kTok > a.sinks;
 }
 // The same of one segment's tiles, from registers.
 struct Tiles {
     int t0, ns, skip, p0, low, sinks;
     __device__ __forceinline__ Tiles(const PagesAttn &a, const Seg &s)
-        : t0(s.t0), ns(s.k.ns), skip((s.k.ws - s.k.ns) * kTok), p0(s.k.p0), low(a.window ? s.k.p1 - a.window + 1 : 0),
+        : t0(s.t0), ns(s.k.ns), skip((s.k.ws - s.k.ns) * kTok), p0(s.k.p0), low(a.window ? window_start(a, s.k.p1) : 0),
           sinks(a.sinks) {}
     __device__ __forceinline__ int token(int j) const { return (t0 + j) * kTok + (t0 + j < ns ? 0 : skip); }
     __device__ __forceinline__ bool edge(int T) const { return T + kTok - 1 > p0 || (T < low && T + kTok > sinks); }
@@ -1007,7 +1011,7 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
             const bool live = r0 + row < s.rows;
             const int tok = live ? (r0 + row) / G : 0, head = live ? r0 + row - tok * G : 0;
             const int p = live ? s.k.p0 + tok : -1;
-            const int lo = a.window ? max(0, p - a.window + 1) : 0;
+            const int lo = a.window ? max(0, window_start(a, p)) : 0;
             const bool any = __any_sync(0xffffffffu, live);
             float m = -INFINITY, l = 0.0f;
             if (r0 < s.rows) {

@@ -181,3 +181,19 @@ def test_a_token_out_of_sight_weighs_nothing(env, at, big):
     assert torch.equal(got[:row], want[:row])
     got, _ = c.attend(q, 0.1, 16, 2)
     assert torch.equal(got[:row], wide[:row]) and torch.equal(got[row + 16:], wide[row + 16:])
+
+
+# ------------------------------------------------------------------ windows
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("window,sinks", [(2**31 - 1, 0), (2**31 - 1, 3), (2**31 - 4, 0), (1 << 40, 2**31 - 1), (2**31 - 300, 5)])
+@pytest.mark.parametrize("new,kv", [([8], [5]), ([300, 1], [290, 40]), ([70], [200]), ([1], [200])])
+def test_windows_as_large_as_none(env, bits, window, sinks, new, kv):
+    """Also where more tokens are new than the cache counts, so that rows stand before it."""
+    torch, K = env
+    c = Case(env, new, kv, heads=1, bits=bits)
+    q = c.queries()
+    want, wlse = c.attend(q, 0.1)
+    got, lse = c.check(q, 0.1, window, sinks)
+    assert torch.equal(got, want) and torch.equal(lse, wlse)
