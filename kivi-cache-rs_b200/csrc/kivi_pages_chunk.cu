@@ -450,7 +450,7 @@ struct Shared {
     uint64_t meet;             // the softmax warps
     uint64_t range[4], conv;   // codes: a tile's exponents are known; the converting warps
     uint64_t drain;
-    uint32_t flags[4][4]; // tokens of an edge tile whose value row is not finite
+    uint32_t flags[4][4]; // 16-bit pages: tokens of an edge tile whose value row is not finite
     uint32_t tmem;
     int last;
     long long scan[16];
@@ -461,11 +461,17 @@ struct Shared {
 
 // Codes: the operands are f16, a tile's keys and values times 2^-exponent (largest
 // finite one below 2^14; of the values' kKeep more are left free rather than O moved),
-// a row's query likewise, and a token's (scale, centre).
-constexpr int kKeep = 6;
+// a row's query likewise, and a token's (scale, centre).  In an edge tile the largest one
+// may be a token that some rows do not see, so its exponent leaves out (flags) tokens
+// 2^kSpan above the smallest: their keys get exponents of their own, undone in their
+// columns of S, and their values are added apart.
+constexpr int kKeep = 6, kSpan = 20, kOdd = 1024;
 struct SharedCodes {
-    int kexp[4], vexp[4];  // of tile counter & 3
-    float most[2][4][2];   // a tile's largest key and value per warp, by tile parity
+    int kexp[4], vexp[4];  // of tile counter & 3, as far as lift; kOdd more where tokens stand apart
+    uint32_t apart[4][4];  // tokens of an edge tile whose values are added apart
+    uint32_t far[4][4];    // and those whose keys have exponents of their own
+    uint8_t lift[4][kTok]; // how far these lie above the tile's
+    float most[2][4][4];   // a tile's largest key and value per warp, an edge tile's smallest, by tile parity
     float4 token[2][kTok]; // key scale, key centre, value scale, value centre
     int qexp[2 * kRows];
 };
@@ -553,9 +559,9 @@ template <int ND> __device__ __noinline__ int move_exponent(uint32_t cO, int ere
     return n;
 }
 
-// Rows of V that are not finite were taken out of an edge tile (flags, one bit
-// per token); they are added here to the rows that see them: p > 0, so p v is v.
-template <int BITS, int ND, bool F16>
+// 16-bit pages: rows of V that are not finite were taken out of an edge tile (flags, one
+// bit per token); they are added here to the rows that see them: p > 0, so p v is v.
+template <int ND, bool F16>
 __device__ __noinline__ void add_unfinite(const PagesAttn &a, const uint32_t *flags, int b, int h, int T, int p, int lo,
                                           uint32_t cO) {
     for (int f = 0; f < 4; ++f) {
@@ -565,18 +571,14 @@ __device__ __noinline__ void add_unfinite(const PagesAttn &a, const uint32_t *fl
             bits &= bits - 1;
             const bool see = t <= p && (t >= lo || t < a.sinks);
             const int64_t r = pages_row(a.st, max(pages_page(a.b, a.st, b, t), 0), h, t);
-            const unsigned char *v = a.st.v + r * a.st.row_bytes;
-            const float2 q = BITS == 16 ? make_float2(0.0f, 0.0f) : __ldg(a.st.vp + r);
+            const uint16_t *v = reinterpret_cast<const uint16_t *>(a.st.v + r * a.st.row_bytes);
 #pragma unroll 1
             for (int c = 0; c < 32 * ND; c += 32) {
                 float o[32];
                 tmem_ld32(cO + c, o);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    float y;
-                    if constexpr (BITS == 16) y = unpack(F16, reinterpret_cast<const uint16_t *>(v)[c + i]);
-                    else if constexpr (BITS == 8) y = fmaf((float)v[c + i], q.x, q.y);
-                    else y = fmaf((float)(v[(c + i) / 2] >> (4 * (i & 1)) & 15), q.x, q.y);
+                    const float y = unpack(F16, v[c + i]);
                     if (see && !isfinite(y)) o[i] += y;
                 }
                 tmem_st32(cO + c, reinterpret_cast<const uint32_t *>(o));
@@ -584,6 +586,81 @@ __device__ __noinline__ void add_unfinite(const PagesAttn &a, const uint32_t *fl
             }
         }
     }
+}
+
+// Codes: a tile of which some tokens stand apart, before its softmax.  Scores of keys with
+// exponents of their own, in tensor memory, times 2^lift (finite ones stay it); then the
+// row's reference, sum and O; then the values that were left out, to the rows that see them,
+// with the weights of their scores (not finite ones as they are, since p > 0), O's exponent
+// raised where one would not fit.
+struct RowState {
+    float m, l;
+    int eref;
+};
+template <int BITS, int ND>
+__device__ __noinline__ RowState settle_apart(const PagesAttn &a, const SharedCodes &sc, const Seg &s, uint32_t tile, int T, int p,
+                                              int lo, uint32_t cS, float crow, RowState row) {
+    const uint32_t cO = cS + (kColO - kColS);
+    const uint8_t *lift = sc.lift[tile & 3];
+    const uint32_t *far = sc.far[tile & 3], *apart = sc.apart[tile & 3];
+    auto see = [&](int t) { return t <= p && (t >= lo || t < a.sinks); };
+    float mx = -INFINITY;
+#pragma unroll 1
+    for (int c = 0; c < kTok; c += 16) {
+        float x[16];
+        tmem_ld16(cS + c, x);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (far[c / 32] >> ((c & 16) + i) & 1u && isfinite(x[i])) {
+                const int k = lift[c + i], h = k >> 1;
+                x[i] = fminf(fmaxf(x[i] * exp2i(h) * exp2i(k - h), -3e38f), 3e38f);
+            }
+            if (see(T + c + i)) mx = max3(mx, x[i] * crow, mx);
+        }
+        tmem_st16(cS + c, reinterpret_cast<const uint32_t *>(x));
+    }
+    st_wait();
+    const bool need = !(mx <= row.m + kLazy), move = need && row.m != -INFINITY;
+    float scale = move ? ex2(row.m - mx) : 1.0f;
+    row.l *= scale;
+    if (need) row.m = fmaf(mx, 0.0f, mx);
+    const float ref = row.m == -INFINITY ? 0.0f : row.m;
+#pragma unroll 1
+    for (int i = -1; i < kTok; ++i) { // (first the rescaling alone)
+        if (i >= 0 && !(apart[i / 32] >> (i & 31) & 1u)) continue;
+        const int t = T + max(i, 0);
+        const bool add = i >= 0 && see(t);
+        const int64_t r = i < 0 ? 0 : pages_row(a.st, max(pages_page(a.b, a.st, s.k.b, t), 0), s.h, t);
+        const unsigned char *v = a.st.v + r * a.st.row_bytes;
+        const float2 q = __ldg(a.st.vp + r);
+        float x[16], w = 0.0f;
+        tmem_ld16(cS + (max(i, 0) & ~15), x);
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+            if (k == (i & 15) && add) w = ex2(__fsub_rn(__fmul_rn(x[k], crow), ref));
+        const float most = fmaxf(fabsf(q.y), fabsf(fmaf((float)((1 << BITS) - 1), q.x, q.y)));
+        int e = row.eref;
+        if (w > 0.0f && isfinite(most)) e = max(e, f16_exponent(most) - 60);
+        const int h = (row.eref - e) >> 1, u = -e >> 1;
+        const float move1 = scale * exp2i(h), move2 = exp2i(row.eref - e - h), unit1 = exp2i(u), unit2 = exp2i(-e - u);
+        row.eref = e, scale = 1.0f;
+#pragma unroll 1
+        for (int c = 0; c < 32 * ND; c += 16) {
+            float o[16];
+            tmem_ld16(cO + c, o);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const int n = c + k;
+                const float code = BITS == 8 ? (float)v[n] : (float)(v[n / 2] >> (4 * (n & 1)) & 15);
+                const float y = fmaf(code, q.x, q.y);
+                o[k] = o[k] * move1 * move2;
+                if (add) o[k] += isfinite(y) ? w * (y * unit1 * unit2) : y;
+            }
+            tmem_st16(cO + c, reinterpret_cast<const uint32_t *>(o));
+            st_wait();
+        }
+    }
+    return row;
 }
 
 // Floats of one part: [D / 4][256 rows] float4 of O, then [256 rows] (m, l).
@@ -1045,18 +1122,22 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
             for (int j = 0; j < n; ++j) {
                 const int T = tl.token(j);
                 const bool edge = tl.edge(T);
-                if (edge) ++edges;
+                if (!kCodes && edge) ++edges;
                 if (dual && (j & 1) != X) continue;
                 if (!(ok = warp_wait(&sh.s_full[X], ns & 1, status))) break;
                 ++ns;
                 tc_after();
                 bool late = edge; // the weights go out in one piece
+                bool odd = false; // codes: tokens of the tile stand apart
                 if constexpr (kCodes) {
                     const uint32_t tile = s.item / 2 + j;
                     if (!(ok = warp_wait(&sh.range[tile & 3], tile >> 2 & 1, status))) break;
                     // B has A's queries where it shares its rows, loaded before the first S
                     const bool first = j < (dual ? 2 : 1);
-                    if (const int ke = sc.kexp[tile & 3]; first || ke != kref) {
+                    int ke = sc.kexp[tile & 3];
+                    odd = ke >= kOdd / 2;
+                    if (odd) ke -= kOdd;
+                    if (first || ke != kref) {
                         kref = ke;
                         crow = score_units(c2, sc.qexp[(dual ? 0 : X * kRows) + row] + ke);
                     }
@@ -1087,6 +1168,10 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                             m4[3] = max3(m4[3], z[i + 6], z[i + 7]);
                         }
                     };
+                    if (kCodes && odd) {
+                        const RowState r = settle_apart<BITS, ND>(sh.args, sc, s, s.item / 2 + j, T, p, lo, cS, crow, RowState{m, l, eref});
+                        m = r.m, l = r.l, eref = r.eref;
+                    }
                     tmem_ld64(cS, x);
                     if (edge) hide(x, T), hide(x + 32, T + 32);
 #pragma unroll
@@ -1170,16 +1255,16 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                         }
                     }
                     l += (a0 + a1) + (a2 + a3);
-                    if (kCodes && late) {
+                    if (kCodes && late) { // O is not at the exponent of this tile's values
                         const int e = sc.vexp[(s.item / 2 + j) & 3];
                         if (__any_sync(0xffffffffu, e != eref)) scale_weights(cS, e - eref);
                     }
                 }
-                if (edge) { // the tile's V has been through the fixing warps
+                if (!kCodes && edge) { // the tile's V has been through the fixing warps
                     const uint32_t it = s.item + 2 * j + 1;
                     if (!(ok = warp_wait(&sh.full[it % kStages], (it / kStages) & 1, status))) break;
                     const uint32_t *fl = sh.flags[(edges - 1) & 3];
-                    if (fl[0] | fl[1] | fl[2] | fl[3]) add_unfinite<BITS, ND, F16>(sh.args, fl, s.k.b, s.h, T, p, lo, cO);
+                    if (fl[0] | fl[1] | fl[2] | fl[3]) add_unfinite<ND, F16>(sh.args, fl, s.k.b, s.h, T, p, lo, cO);
                 }
                 st_wait();
                 tc_before();
@@ -1336,7 +1421,6 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                 if constexpr (D > 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + 64) : "memory");
             }
             if constexpr (kCodes) { // the converting warps fetch their own
-                for (int j = 0; j < s.n; ++j) ne += tile_edge(a, k, tile_token(k, s.t0 + j));
                 item += 2 * s.n;
                 more = walk_next(a, TB, w);
                 continue;
@@ -1418,7 +1502,6 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
         };
         while (ok && next_seg()) {
             const Seg &s = *sp;
-            uint32_t ne = s.edges;
             int ve = 0; // the values' exponent
             int T = tile_token(s.k, s.t0);
             int rows = rows_of(s, T, lookup(s, T));
@@ -1437,26 +1520,58 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                 const bool kf = isfinite(kb) && isfinite(kp.x), vf = isfinite(vb) && isfinite(vp.x);
                 const uint32_t km = __reduce_max_sync(0xffffffffu, kf ? __float_as_uint(kb) : 0u);
                 const uint32_t vm = __reduce_max_sync(0xffffffffu, vf ? __float_as_uint(vb) : 0u);
-                const uint32_t bad = __ballot_sync(0xffffffffu, !vf);
-                if (lane == 0 && cw < 4) {
-                    sc.most[tile & 1][cw][0] = __uint_as_float(km), sc.most[tile & 1][cw][1] = __uint_as_float(vm);
-                    if (edge) sh.flags[ne & 3][cw] = bad;
+                if (lane == 0 && cw < 4) sc.most[tile & 1][cw][0] = __uint_as_float(km), sc.most[tile & 1][cw][1] = __uint_as_float(vm);
+                if (edge) {
+                    const uint32_t bad = __ballot_sync(0xffffffffu, !vf);
+                    const uint32_t kl = __reduce_min_sync(0xffffffffu, kf && kb > 0.0f ? __float_as_uint(kb) : 0x7f7fffffu);
+                    const uint32_t vl = __reduce_min_sync(0xffffffffu, vf && vb > 0.0f ? __float_as_uint(vb) : 0x7f7fffffu);
+                    if (lane == 0 && cw < 4) {
+                        sc.most[tile & 1][cw][2] = __uint_as_float(kl), sc.most[tile & 1][cw][3] = __uint_as_float(vl);
+                        sc.apart[tile & 3][cw] = bad;
+                    }
                 }
                 if (ct < kTok)
-                    sc.token[tile & 1][ct] = make_float4(kp.x, fmaf(half, kp.x, kp.y), edge && !vf ? 0.0f : vp.x,
-                                                         edge && !vf ? 0.0f : fmaf(half, vp.x, vp.y));
+                    sc.token[tile & 1][ct] = make_float4(kp.x, fmaf(half, kp.x, kp.y), vp.x, fmaf(half, vp.x, vp.y));
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.conv);
                 if (!(ok = warp_wait(&sh.conv, met++ & 1, status))) break;
                 float kmost = 0.0f, vmost = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) kmost = fmaxf(kmost, sc.most[tile & 1][i][0]), vmost = fmaxf(vmost, sc.most[tile & 1][i][1]);
-                const int ke = f16_exponent(kmost), own = f16_exponent(vmost);
+                int ke = f16_exponent(kmost), own = f16_exponent(vmost);
+                bool split = false;
+                if (edge) {
+                    float kl = 3e38f, vl = 3e38f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        kl = fminf(kl, sc.most[tile & 1][i][2]), vl = fminf(vl, sc.most[tile & 1][i][3]);
+                        split |= sc.apart[tile & 3][i] != 0;
+                    }
+                    const int k2 = f16_exponent(kl) + kSpan, v2 = f16_exponent(vl) + kSpan;
+                    split |= k2 < ke || v2 < own;
+                    ke = min(ke, k2), own = min(own, v2);
+                }
                 // O moves when this does, so it starts with room for values four times as
                 // large, and stays while they fit and lose nothing by it; zeros take any
                 if (j == 0 || own > ve || (own < ve - kKeep && vmost > 0.0f)) ve = min(own + 2, 127);
+                if (split) {
+                    const int lift = kf ? max(f16_exponent(kb) - ke, 0) : 0;
+                    const bool apart = !vf || f16_exponent(vb) > ve;
+                    const uint32_t far = __ballot_sync(0xffffffffu, lift > 0), out = __ballot_sync(0xffffffffu, apart);
+                    if (ct < kTok) {
+                        sc.lift[tile & 3][ct] = (uint8_t)lift;
+                        float4 &q = sc.token[tile & 1][ct];
+                        const float f0 = exp2i(-(lift >> 1)), f1 = exp2i(-(lift - (lift >> 1)));
+                        q.x = q.x * f0 * f1, q.y = q.y * f0 * f1;
+                        if (apart) q.z = q.w = 0.0f;
+                        if (lane == 0) sc.far[tile & 3][cw] = far, sc.apart[tile & 3][cw] = out;
+                    }
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&sh.conv);
+                    if (!(ok = warp_wait(&sh.conv, met++ & 1, status))) break;
+                }
                 if (ct == 0) {
-                    sc.kexp[tile & 3] = ke, sc.vexp[tile & 3] = ve;
+                    sc.kexp[tile & 3] = ke + (split ? kOdd : 0), sc.vexp[tile & 3] = ve;
                     bar_arrive(&sh.range[tile & 3]);
                 }
                 const float kf2 = exp2i(-ke), vf2 = exp2i(-ve);
@@ -1492,7 +1607,6 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                     __syncwarp();
                     if (lane == 0) bar_arrive(&sh.full[slot]);
                 }
-                ne += edge;
                 T = Tn, rows = rowsn;
             }
         }

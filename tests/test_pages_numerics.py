@@ -197,3 +197,55 @@ def test_windows_as_large_as_none(env, bits, window, sinks, new, kv):
     want, wlse = c.attend(q, 0.1)
     got, lse = c.check(q, 0.1, window, sinks)
     assert torch.equal(got, want) and torch.equal(lse, wlse)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("side", ["keys", "values", "both"])
+@pytest.mark.parametrize("big", [1e6, 1e12, 1e38])
+@pytest.mark.parametrize("at", [0, 1, 24, 69])
+def test_a_token_out_of_sight_takes_no_precision(env, bits, side, big, at):
+    """Codes: huge keys or values in one newest token leave the rows that do not see it
+    as exact as before; those that do see it are right too."""
+    torch, K = env
+    new, kv = 70, 200
+    c = Case(env, [new], [kv], heads=1, bits=bits)
+    k, v = c.k.float(), c.v.float()
+    x = kv - new + at
+    if side != "values":
+        k[x] = k[x].sign() * big
+    if side != "keys":
+        v[x] = v[x].sign() * big
+    rewrite(c, k=k, v=v)
+    q = c.queries()
+    for window, sinks in ((0, 0), (16, 2)):
+        out, lse = c.attend(q, 0.1, window, sinks)
+        o, l, tol, ltol = c.reference(q, 0.1, window, sinks)
+        hidden = torch.ones(new, dtype=torch.bool, device="cuda")
+        hidden[at:at + window if window else new] = False
+        assert bool(((out.double() - o).abs() <= tol)[hidden].all())
+        assert bool(((lse.double() - l).abs() <= ltol)[hidden].all())
+        if side == "values":
+            assert bool(((out.double() - o).abs() <= tol)[~hidden].all())
+        else:  # one weight is all of them, or nothing
+            assert bool(torch.isfinite(out[~hidden]).all())
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("at", [0, 5, 24, 63])
+def test_a_value_that_is_not_finite(env, bits, at):
+    """An infinite value among a newest token's: its channel in the rows that see it (codes:
+    every channel, since the row's parameters are not finite), every other output as exact."""
+    torch, K = env
+    new, kv = 70, 200
+    c = Case(env, [new], [kv], heads=1, bits=bits)
+    q = c.queries()
+    v = c.v.clone()
+    v[kv - new + at, 0, 5] = math.inf
+    rewrite(c, v=v)
+    out, lse = c.attend(q, 0.1)
+    o, l, tol, ltol = c.reference(q, 0.1)
+    assert bool(((lse.double() - l).abs() <= ltol).all())
+    good = torch.ones(out.shape, dtype=torch.bool, device="cuda")
+    good[at:, :, 5 if bits == 16 else slice(None)] = False
+    assert bool(((out.double() - o).abs() <= tol)[good].all())
+    assert not bool(torch.isfinite(out[~good]).any())
