@@ -46,6 +46,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxG = 8;
 constexpr float kLazy = 8.0f; // a reference moves when a logit exceeds it by 2^8
+constexpr int kKeep = 8;      // how far the value scales may fall before O's exponent follows
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 
@@ -493,13 +494,29 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(BITS, ND))
                             const uint32_t b = __float_as_uint(fabsf(vp[s][i].x));
                             if (b < 0x7f800000u) most = max(most, b);
                         }
-                    // p <= 2^kLazy: weights below 2^14
-                    const int e = f16_exponent(__reduce_max_sync(0xffffffffu, most)) + (int)kLazy;
-                    if (e > eref) {
-                        const float f = exp2i(max(eref - e, -126));
-                        eref = e;
+                    most = __reduce_max_sync(0xffffffffu, most);
+                    // p <= 2^kLazy: weights below 2^14.  O follows the scales both ways (down
+                    // as far as fp32 lets it), so that large ones of small weight take nothing
+                    // from later tiles.
+                    const int e = f16_exponent(most) + (int)kLazy;
+                    if (e > eref || (e + kKeep < eref && most > 0)) {
+                        int n = e;
+                        if (e < eref) {
+                            uint32_t big = 0;
 #pragma unroll
-                        for (int i = 0; i < STEPS; ++i) o[i][0] *= f, o[i][1] *= f, o[i][2] *= f, o[i][3] *= f;
+                            for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) big = max(big, __float_as_uint(fabsf(o[i][k])));
+                            big = __reduce_max_sync(0xffffffffu, big);
+                            if (big > 0 && big < 0x7f800000u) n = min(max(e, eref + (int)(big >> 23) - 227), eref); // below 2^101
+                        }
+                        const int d = eref - n, h = d >> 1;
+                        const float f0 = exp2i(h), f1 = exp2i(d - h);
+                        eref = n;
+#pragma unroll
+                        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) o[i][k] = o[i][k] * f0 * f1;
                     }
                     fv = exp2i(-eref);
                 }

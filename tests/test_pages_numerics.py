@@ -59,7 +59,7 @@ def test_runs_of_unlike_values(env, bits, kind, new, sizes):
 
 
 @pytest.mark.parametrize("bits,kind", [(16, "bf16"), (8, "bf16"), (4, "bf16")])
-@pytest.mark.parametrize("new", [70])
+@pytest.mark.parametrize("new", [1, 70])
 @pytest.mark.parametrize("big", [1e6, 1e9, 1e12])
 def test_large_values_of_small_weight(env, bits, kind, new, big):
     """Tokens whose values are far larger and whose weights are as much smaller: what
@@ -78,10 +78,11 @@ def test_large_values_of_small_weight(env, bits, kind, new, big):
 
 @pytest.mark.parametrize("bits", [16, 8, 4])
 @pytest.mark.parametrize("sizes", [(1e30, 1e-8), (1e-30, 1e30), (1e30, 0, 1e-30, 1e30)])
-def test_runs_of_extreme_values(env, bits, sizes):
+@pytest.mark.parametrize("new", [1, 130])
+def test_runs_of_extreme_values(env, bits, sizes, new):
     """Sums that no exponent of the small values holds."""
     torch, K = env
-    c = Case(env, [130], [800], heads=1, bits=bits)
+    c = Case(env, [new], [800], heads=1, bits=bits)
     t = torch.arange(800, device="cuda") // 128
     size = torch.tensor(sizes, device="cuda")[t % len(sizes)].float()
     rewrite(c, v=c.v.float() * size[:, None, None])
