@@ -2835,7 +2835,7 @@ struct PagesScratch {
     float *p = nullptr;
     int64_t floats = 0;
     cudaEvent_t done = nullptr;  // after the last attention call outside a capture
-    cudaStream_t last = nullptr; // its stream
+    unsigned long long last = 0; // its stream's id: handles come back, and one may name a stream per thread
     bool used = false;
     std::mutex mu;
 };
@@ -3120,11 +3120,14 @@ int32_t kivi_pages_attention_dev(kivi_pages *h, const kivi_pages_batch *batch, i
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     CUDA_TRY(cudaStreamIsCapturing(st, &cap), "pages_attention");
     const bool live = cap == cudaStreamCaptureStatusNone;
-    if (live && x->used && x->last != st) CUDA_TRY(cudaStreamWaitEvent(st, x->done, 0), "pages_attention");
+    unsigned long long id = 0;
+    if (live) CUDA_TRY(cudaStreamGetId(st, &id), "pages_attention");
+    if (live && x->used && (x->last != id || st == cudaStreamPerThread))
+        CUDA_TRY(cudaStreamWaitEvent(st, x->done, 0), "pages_attention");
     CUDA_TRY(kivi::launch_pages_attention(a, st), "pages_attention");
     if (live) {
         CUDA_TRY(cudaEventRecord(x->done, st), "pages_attention");
-        x->last = st;
+        x->last = id;
         x->used = true;
     }
     return set_err(err, KIVI_OK);

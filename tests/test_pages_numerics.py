@@ -250,3 +250,58 @@ def test_a_value_that_is_not_finite(env, bits, at):
     good[at:, :, 5 if bits == 16 else slice(None)] = False
     assert bool(((out.double() - o).abs() <= tol)[good].all())
     assert not bool(torch.isfinite(out[~good]).any())
+
+
+# ------------------------------------------------------------------ shared state
+
+
+def test_threads_on_their_default_streams(env):
+    """cudaStreamPerThread is one handle for a stream of each host thread: two threads'
+    calls share the device's scratch safely."""
+    import threading
+
+    torch, K = env
+    cases = [Case(env, [1], [20011], heads=1, group=5, seed=1), Case(env, [300], [4000], heads=1, group=4, page=64, seed=2)]
+    queries = [c.queries() for c in cases]
+    want = [c.attend(q, 0.1)[0] for c, q in zip(cases, queries)]
+    outs = [[torch.empty_like(q) for _ in range(40)] for q in queries]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            c = cases[i]
+            for o in outs[i]:
+                c.store.attention_dev(c.step, queries[i], c.heads * c.group, 0.1, o, stream=2)
+        except Exception as e:  # noqa: BLE001  (reported by the test's own thread)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for w, o in zip(want, outs):
+        assert all(torch.equal(x, w) for x in o)
+
+
+def test_streams_made_anew(env):
+    """A stream that is gone and one with its handle are two streams."""
+    import ctypes as C
+
+    torch, K = env
+    rt = C.CDLL("libcudart.so.12")
+    c = Case(env, [1], [20011], heads=1, group=5)
+    q = c.queries()
+    want, _ = c.attend(q, 0.1)
+    outs = [torch.empty_like(q) for _ in range(60)]
+    torch.cuda.synchronize()
+    for o in outs:
+        s = C.c_void_p()
+        assert rt.cudaStreamCreateWithFlags(C.byref(s), 1) == 0  # non-blocking
+        c.store.attention_dev(c.step, q, c.heads * c.group, 0.1, o, stream=s.value)
+        assert rt.cudaStreamDestroy(s) == 0  # its work goes on
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
