@@ -2842,6 +2842,13 @@ struct PagesScratch {
 std::mutex g_pages_mu;
 PagesScratch *g_pages_scratch[kMaxHintDevices] = {nullptr};
 
+// Zeroes device memory before it returns: streams that do not wait for the legacy one may
+// be given work on it next.
+cudaError_t zero_now(void *p, size_t bytes) {
+    cudaError_t e = cudaMemsetAsync(p, 0, bytes, cudaStreamLegacy);
+    return e == cudaSuccess ? cudaStreamSynchronize(cudaStreamLegacy) : e;
+}
+
 void free_scratch(PagesScratch *x) {
     dfree(x->p);
     if (x->done) cudaEventDestroy(x->done);
@@ -2861,7 +2868,7 @@ cudaError_t acquire_scratch(int device, PagesScratch **out) {
         cudaError_t e;
         if ((e = kivi::pages_scratch_floats(&x->floats)) != cudaSuccess ||
             (e = dalloc(&x->p, (size_t)x->floats)) != cudaSuccess ||
-            (e = cudaMemset(x->p + x->floats - kivi::kPagesCounters, 0, kivi::kPagesCounters * sizeof(float))) != cudaSuccess ||
+            (e = zero_now(x->p + x->floats - kivi::kPagesCounters, kivi::kPagesCounters * sizeof(float))) != cudaSuccess ||
             (e = cudaEventCreateWithFlags(&x->done, cudaEventDisableTiming)) != cudaSuccess) {
             free_scratch(x);
             return e;
@@ -3018,7 +3025,7 @@ int32_t kivi_pages_new(const kivi_pages_config *config, void *d_keys, void *d_va
     cudaError_t e;
     if ((e = acquire_scratch(device, &h->scratch)) != cudaSuccess ||
         (e = dalloc(&st.status, 1)) != cudaSuccess ||
-        (e = cudaMemset(st.status, 0, sizeof(unsigned int))) != cudaSuccess ||
+        (e = zero_now(st.status, sizeof(unsigned int))) != cudaSuccess ||
         (st.bits == 16 && (e = kivi::pages_tensor_maps(st, &h->maps)) != cudaSuccess)) {
         rc = cuda_fail(err, e, "kivi_pages_new");
         kivi_pages_free(h);
@@ -3140,7 +3147,7 @@ int32_t kivi_pages_status(kivi_pages *h, kivi_error *err) {
     unsigned int flag = 0;
     CUDA_TRY(cudaMemcpy(&flag, h->st.status, sizeof(flag), cudaMemcpyDeviceToHost), "pages_status");
     if (!flag) return set_err(err, KIVI_OK);
-    CUDA_TRY(cudaMemset(h->st.status, 0, sizeof(flag)), "pages_status");
+    CUDA_TRY(zero_now(h->st.status, sizeof(flag)), "pages_status");
     if (flag & kivi::kPagesGaveUp)
         return set_msg(err, KIVI_ERR_CUDA, "attention kernel gave up waiting for its copies (flag %u)", flag);
     return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "%s%s%s",

@@ -305,3 +305,22 @@ def test_streams_made_anew(env):
         assert rt.cudaStreamDestroy(s) == 0  # its work goes on
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+def test_a_new_store_on_a_busy_device(env):
+    """A handle made while the default stream is busy is ready when it is returned: what
+    another stream's call reports is not cleared later."""
+    torch, K = env
+    c = Case(env, [1], [40], heads=1)
+    q, s = c.queries(), torch.cuda.Stream()
+    out = torch.empty_like(q)
+    c.table[0, 0] = -1
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)
+    store = K.KvPages(c.config, *c.data)
+    store.attention_dev(c.step, q, c.group, 0.1, out, stream=s)
+    s.synchronize()
+    with pytest.raises(K.KiviError) as e:
+        store.status()
+    assert "page" in e.value.message
+    store.status()
