@@ -517,8 +517,11 @@ uint64_t kivi_guard_sequence_length(const kivi_guard *guard);
  * several streams: all handles of a device share one scratch (40 MB, there while
  * any handle is) for the attention's partial states, and an attention call on
  * another stream than the device's previous one waits for that one on the
- * device.  Inside a stream capture it does not: order captured attention calls of
- * one device yourself.  Writing and attending are ordered by the caller's streams.
+ * device.  Inside a stream capture it does not, and a replay is ordered with
+ * nothing but its stream: where graphs may run beside one another or beside other
+ * attention calls of the device, give the handles a workspace of their own
+ * (kivi_pages_set_workspace) before the capture, one for each graph or stream.
+ * Writing and attending are ordered by the caller's streams.
  */
 #define KIVI_DTYPE_F32 0
 #define KIVI_DTYPE_F16 1
@@ -593,6 +596,16 @@ int32_t kivi_pages_attention_dev(kivi_pages *pages, const kivi_pages_batch *batc
                                  float scale, uint64_t window, uint64_t sinks, void *d_out,
                                  uint64_t out_token_stride, uint64_t out_head_stride, float *d_lse,
                                  void *stream, kivi_error *err);
+/* Bytes of an attention workspace on a device. */
+int32_t kivi_pages_workspace_size(int32_t device, uint64_t *bytes, kivi_error *err);
+/* The workspace of the handle's later attention calls in place of the device's
+ * scratch (null: the scratch again): `bytes` of the caller's device memory, 16-byte
+ * aligned, which must outlive the handle and every graph that captured a call with
+ * it.  Handles may share one.  Calls that use one workspace, replays among them,
+ * must follow one another: that order is the caller's.  Waits for the legacy
+ * stream; not during a capture. */
+int32_t kivi_pages_set_workspace(kivi_pages *pages, void *d_workspace, uint64_t bytes,
+                                 kivi_error *err);
 /* What the handle's calls found wrong on the device since the last report: page
  * numbers outside the store, or offsets and lengths outside their arrays, were
  * clamped (KIVI_ERR_INVALID_ARGUMENT; the outputs concerned are unspecified),

@@ -2849,6 +2849,11 @@ cudaError_t zero_now(void *p, size_t bytes) {
     return e == cudaSuccess ? cudaStreamSynchronize(cudaStreamLegacy) : e;
 }
 
+// The counters at the end of a scratch or workspace.
+cudaError_t zero_counters(float *p, int64_t floats) {
+    return zero_now(p + floats - kivi::kPagesCounters, kivi::kPagesCounters * sizeof(float));
+}
+
 void free_scratch(PagesScratch *x) {
     dfree(x->p);
     if (x->done) cudaEventDestroy(x->done);
@@ -2868,7 +2873,7 @@ cudaError_t acquire_scratch(int device, PagesScratch **out) {
         cudaError_t e;
         if ((e = kivi::pages_scratch_floats(&x->floats)) != cudaSuccess ||
             (e = dalloc(&x->p, (size_t)x->floats)) != cudaSuccess ||
-            (e = zero_now(x->p + x->floats - kivi::kPagesCounters, kivi::kPagesCounters * sizeof(float))) != cudaSuccess ||
+            (e = zero_counters(x->p, x->floats)) != cudaSuccess ||
             (e = cudaEventCreateWithFlags(&x->done, cudaEventDisableTiming)) != cudaSuccess) {
             free_scratch(x);
             return e;
@@ -2894,6 +2899,7 @@ struct kivi_pages {
     int device = 0;
     kivi::PagesMaps maps{};
     PagesScratch *scratch = nullptr;
+    float *workspace = nullptr; // the caller's, of scratch->floats; null: the device's scratch
 };
 
 namespace {
@@ -3114,7 +3120,7 @@ int32_t kivi_pages_attention_dev(kivi_pages *h, const kivi_pages_batch *batch, i
     a.qsign = std::signbit(scale) ? -1.0f : 1.0f;
     a.window = (int)std::min<uint64_t>(window, 0x7fffffffull);
     a.sinks = window ? (int)std::min<uint64_t>(sinks, 0x7fffffffull) : 0;
-    a.part = h->scratch->p;
+    a.part = h->workspace ? h->workspace : h->scratch->p;
     a.part_floats = h->scratch->floats;
     a.maps = &h->maps;
     if (!kivi::pages_attention_supported(a))
@@ -3122,6 +3128,10 @@ int32_t kivi_pages_attention_dev(kivi_pages *h, const kivi_pages_batch *batch, i
                        a.G, a.b.batch);
     DeviceGuard dg(h->device);
     cudaStream_t st = (cudaStream_t)stream;
+    if (h->workspace) { // ordered by the caller
+        CUDA_TRY(kivi::launch_pages_attention(a, st), "pages_attention");
+        return set_err(err, KIVI_OK);
+    }
     PagesScratch *x = h->scratch;
     std::lock_guard<std::mutex> lk(x->mu);
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
@@ -3137,6 +3147,31 @@ int32_t kivi_pages_attention_dev(kivi_pages *h, const kivi_pages_batch *batch, i
         x->last = id;
         x->used = true;
     }
+    return set_err(err, KIVI_OK);
+}
+
+int32_t kivi_pages_workspace_size(int32_t device, uint64_t *bytes, kivi_error *err) {
+    if (!bytes) return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "null size");
+    DeviceGuard dg(device);
+    if (!dg.ok) return set_msg(err, KIVI_ERR_CUDA, "cannot select device %d", device);
+    int64_t floats = 0;
+    CUDA_TRY(kivi::pages_scratch_floats(&floats), "pages_workspace_size");
+    *bytes = (uint64_t)floats * sizeof(float);
+    return set_err(err, KIVI_OK);
+}
+
+int32_t kivi_pages_set_workspace(kivi_pages *h, void *d_workspace, uint64_t bytes, kivi_error *err) {
+    if (!h) return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "null pages");
+    const uint64_t need = (uint64_t)h->scratch->floats * sizeof(float);
+    if (d_workspace && bytes < need)
+        return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "workspace of %llu bytes, need %llu", (unsigned long long)bytes,
+                       (unsigned long long)need);
+    if ((uintptr_t)d_workspace % 16) return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "a workspace must be 16-byte aligned");
+    if (d_workspace) {
+        DeviceGuard dg(h->device);
+        CUDA_TRY(zero_counters(static_cast<float *>(d_workspace), h->scratch->floats), "pages_set_workspace");
+    }
+    h->workspace = static_cast<float *>(d_workspace);
     return set_err(err, KIVI_OK);
 }
 

@@ -1249,4 +1249,4 @@ from .econ import (  # noqa: E402  (re-exported at the top level, as lib.rs does
 
 # ---------------------------------------------------------------- paged store
 
-from .pages import KvPages, PagesBatch, PagesConfig  # noqa: E402
+from .pages import KvPages, PagesBatch, PagesConfig, pages_workspace_size  # noqa: E402

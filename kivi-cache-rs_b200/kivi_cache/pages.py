@@ -44,6 +44,8 @@ def signatures(P, sz, i32, f32, e):
         "kivi_pages_read_dev": ([P, bat, i32, P, P, sz, sz, P, e], i32),
         "kivi_pages_attention_dev": ([P, bat, i32, P, sz, sz, sz, f32, sz, sz, P, sz, sz, P, P, e],
                                      i32),
+        "kivi_pages_workspace_size": ([i32, u64p, e], i32),
+        "kivi_pages_set_workspace": ([P, P, sz, e], i32),
         "kivi_pages_status": ([P, e], i32),
     }
 
@@ -85,6 +87,13 @@ def _rows(x, dtype, strides, heads, dim, total, what):
         raise _bad(f"{what}: the elements of a row must be contiguous, their stride is {inner}")
     # the stride of a dimension of one says nothing
     return x.data_ptr(), code, token if total > 1 else heads * dim, head if heads > 1 and total else dim
+
+
+def pages_workspace_size(device=0):
+    """Bytes of an attention workspace on `device` (KvPages.set_workspace)."""
+    size, err = C.c_uint64(), _Err()
+    _check(lib().kivi_pages_workspace_size(int(device), C.byref(size), C.byref(err)), err)
+    return int(size.value)
 
 
 @dataclass(frozen=True)
@@ -239,6 +248,20 @@ class KvPages:
                              ot, oh, _ptr(d_lse), _stream(stream), C.byref(err))
         if rc:
             _check(rc, err)
+
+    def set_workspace(self, d_workspace, nbytes=None):
+        """Later attention calls keep their partial states in `d_workspace`, a contiguous
+        CUDA tensor (or a pointer with `nbytes`) of pages_workspace_size() bytes, instead of
+        the device's scratch; None: the scratch again.  Before a capture whose graph may run
+        beside other attention calls.  Handles may share one; calls that use it, replays
+        among them, must follow one another."""
+        if d_workspace is not None and not isinstance(d_workspace, int):
+            if d_workspace.get_device() != self.device or not d_workspace.is_contiguous():
+                raise _bad(f"a workspace must be contiguous memory of device {self.device}")
+            nbytes = d_workspace.numel() * d_workspace.element_size()
+        err = _Err()
+        _check(lib().kivi_pages_set_workspace(self._h, _ptr(d_workspace), nbytes or 0, C.byref(err)), err)
+        self._workspace = d_workspace
 
     def status(self):
         """Waits for the device; raises KiviError if a call since the last

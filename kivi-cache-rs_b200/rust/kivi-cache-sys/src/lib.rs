@@ -296,5 +296,7 @@ extern "C" {
     pub fn kivi_pages_write_dev(pages: *mut kivi_pages, batch: *const kivi_pages_batch, dtype: i32, d_keys: *const c_void, d_values: *const c_void, token_stride: u64, head_stride: u64, stream: *mut c_void, err: *mut kivi_error) -> i32;
     pub fn kivi_pages_read_dev(pages: *const kivi_pages, batch: *const kivi_pages_batch, dtype: i32, d_keys: *mut c_void, d_values: *mut c_void, token_stride: u64, head_stride: u64, stream: *mut c_void, err: *mut kivi_error) -> i32;
     pub fn kivi_pages_attention_dev(pages: *mut kivi_pages, batch: *const kivi_pages_batch, dtype: i32, d_query: *const c_void, num_q_heads: u64, query_token_stride: u64, query_head_stride: u64, scale: f32, window: u64, sinks: u64, d_out: *mut c_void, out_token_stride: u64, out_head_stride: u64, d_lse: *mut f32, stream: *mut c_void, err: *mut kivi_error) -> i32;
+    pub fn kivi_pages_workspace_size(device: i32, bytes: *mut u64, err: *mut kivi_error) -> i32;
+    pub fn kivi_pages_set_workspace(pages: *mut kivi_pages, d_workspace: *mut c_void, bytes: u64, err: *mut kivi_error) -> i32;
     pub fn kivi_pages_status(pages: *mut kivi_pages, err: *mut kivi_error) -> i32;
 }

@@ -324,3 +324,34 @@ def test_a_new_store_on_a_busy_device(env):
         store.status()
     assert "page" in e.value.message
     store.status()
+
+
+def test_graphs_with_workspaces_beside_one_another(env):
+    """Two captured steps, each with a workspace of its own, replayed on two streams beside
+    live calls on a third."""
+    torch, K = env
+    specs = [dict(new=[1], kv=[20011], group=5, heads=1), dict(new=[300], kv=[4000], group=4, heads=1, page=64)]
+    cases = [Case(env, seed=i, **s) for i, s in enumerate(specs + specs[:1])]
+    queries = [c.queries() for c in cases]
+    want = [c.attend(q, 0.1)[0] for c, q in zip(cases, queries)]
+    outs, graphs, streams = [torch.empty_like(q) for q in queries], [], [torch.cuda.Stream() for _ in range(3)]
+    for c, q, o, s in zip(cases[:2], queries, outs, streams):
+        c.store.set_workspace(torch.empty(K.pages_workspace_size() // 4, device="cuda"))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            c.store.attention_dev(c.step, q, c.heads * c.group, 0.1, o, stream=s)
+        graphs.append(g)
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+            c = cases[2]
+            c.store.attention_dev(c.step, queries[2], c.heads * c.group, 0.1, outs[2], stream=streams[2])
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    for c in cases:
+        c.store.status()
