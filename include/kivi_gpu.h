@@ -609,7 +609,9 @@ int32_t kivi_pages_set_workspace(kivi_pages *pages, void *d_workspace, uint64_t 
 /* What the handle's calls found wrong on the device since the last report: page
  * numbers outside the store, or offsets and lengths outside their arrays, were
  * clamped (KIVI_ERR_INVALID_ARGUMENT; the outputs concerned are unspecified),
- * or a bounded wait gave up (KIVI_ERR_CUDA).  Waits for the device. */
+ * or a bounded wait gave up (KIVI_ERR_CUDA).  Waits for the device, and with a
+ * report readies the handle's workspace and the device's scratch for the next
+ * call, whatever state this one left them in. */
 int32_t kivi_pages_status(kivi_pages *pages, kivi_error *err);
 
 #ifdef __cplusplus

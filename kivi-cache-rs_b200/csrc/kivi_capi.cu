@@ -3183,6 +3183,13 @@ int32_t kivi_pages_status(kivi_pages *h, kivi_error *err) {
     CUDA_TRY(cudaMemcpy(&flag, h->st.status, sizeof(flag), cudaMemcpyDeviceToHost), "pages_status");
     if (!flag) return set_err(err, KIVI_OK);
     CUDA_TRY(zero_now(h->st.status, sizeof(flag)), "pages_status");
+    // A call that gave up left some of its counters raised, and the next ones would join
+    // their parts too early or never.
+    {
+        std::lock_guard<std::mutex> lk(h->scratch->mu);
+        CUDA_TRY(zero_counters(h->scratch->p, h->scratch->floats), "pages_status");
+        if (h->workspace) CUDA_TRY(zero_counters(h->workspace, h->scratch->floats), "pages_status");
+    }
     if (flag & kivi::kPagesGaveUp)
         return set_msg(err, KIVI_ERR_CUDA, "attention kernel gave up waiting for its copies (flag %u)", flag);
     return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "%s%s%s",

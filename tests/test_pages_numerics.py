@@ -355,3 +355,30 @@ def test_graphs_with_workspaces_beside_one_another(env):
         assert all(torch.equal(o, w) for o, w in zip(outs, want))
     for c in cases:
         c.store.status()
+
+
+def test_a_report_readies_the_workspace(env):
+    """Counters that a call left raised are cleared with its report."""
+    torch, K = env
+    c = Case(env, [1], [20011], heads=1, group=5)
+    q = c.queries()
+    want, _ = c.attend(q, 0.1)
+    w = torch.empty(K.pages_workspace_size() // 4, dtype=torch.int32, device="cuda").fill_(7)
+    c.store.set_workspace(w)
+    assert bool((w[-2048:] == 0).all())
+    w[-2048:] = 1
+    c.kv_lens[0] = 1 << 30
+    c.store.read_dev(c.step, *[torch.empty(1, 1, 128, dtype=c.dtype, device="cuda") for _ in range(2)])
+    with pytest.raises(K.KiviError) as e:
+        c.store.status()
+    assert "lengths" in e.value.message and bool((w[-2048:] == 0).all())
+    c.kv_lens[0] = 20011
+    assert torch.equal(c.attend(q, 0.1)[0], want)
+    c.store.set_workspace(None)
+    assert torch.equal(c.attend(q, 0.1)[0], want)
+    for bad in (w[:100], w.cpu(), torch.empty(2, w.numel(), dtype=torch.int32, device="cuda").T):
+        with pytest.raises(K.KiviError):
+            c.store.set_workspace(bad)
+    with pytest.raises(K.KiviError):
+        c.store.set_workspace(w.data_ptr() + 4, 4 * w.numel())
+    assert torch.equal(c.attend(q, 0.1)[0], want)
