@@ -65,7 +65,11 @@ def _code(dtype):
     raise _bad(f"unknown element type {dtype!r}: use one of {sorted(DTYPES)}")
 
 
-def _rows(x, dtype, strides, heads, dim, total, what):
+def _place(device):
+    return "the CPU" if device < 0 else f"device {device}"
+
+
+def _rows(x, dtype, strides, heads, dim, total, what, device):
     """(pointer, type code, token stride, head stride) of dense rows
     [total, heads, dim]: a tensor's own, or a pointer's as given (contiguous
     where no strides are)."""
@@ -74,6 +78,8 @@ def _rows(x, dtype, strides, heads, dim, total, what):
             raise _bad(f"{what}: a pointer needs dtype=")
         token, head = strides if strides is not None else (heads * dim, dim)
         return x, _code(dtype), token, head
+    if x.get_device() != device:
+        raise _bad(f"{what}: on {_place(x.get_device())}, the pages are on {_place(device)}")
     if x.shape != (total, heads, dim):
         raise _bad(f"{what}: expected shape {(total, heads, dim)}, got {tuple(x.shape)}")
     code = _types.get(x.dtype)
@@ -155,6 +161,10 @@ class PagesBatch:
             raise _bad("pointers need batch= and table_width=")
         if min(batch, table_width, total_tokens, max_tokens) < 0:
             raise _bad("negative size")
+        devices = {x.get_device() for x in self.tensors if not isinstance(x, int)}
+        if len(devices) > 1:
+            raise _bad("block_table, cu_tokens and kv_lens lie on different devices")
+        self.device = devices.pop() if devices else None  # None: pointers, the caller's to vouch for
         self.total_tokens = int(total_tokens)
         self._c = _PagesBatch(_ptr(block_table),
                               table_width if table_stride is None else table_stride, table_width,
@@ -180,6 +190,8 @@ class KvPages:
                 raise _bad(f"page memory of {x.numel() * x.element_size()} bytes, need {size * unit}")
             if device is None:
                 device = x.device.index
+            if x.device.index != device:
+                raise _bad(f"page memory on {_place(x.device.index)}, not on {_place(device)}")
         self.device = 0 if device is None else int(device)
         _check(lib().kivi_pages_new(C.byref(c), _ptr(d_keys), _ptr(d_values), _ptr(d_key_params),
                                     _ptr(d_value_params), self.device, C.byref(h), C.byref(err)), err)
@@ -200,10 +212,15 @@ class KvPages:
         except Exception:
             pass
 
+    def _batch_here(self, batch):
+        if batch.device is not None and batch.device != self.device:
+            raise _bad(f"the batch is on {_place(batch.device)}, the pages are on {_place(self.device)}")
+
     def _sides(self, batch, d_keys, d_values, dtype, strides):
-        total = batch.total_tokens
-        k, code, token, head = _rows(d_keys, dtype, strides, self._heads, self._dim, total, "keys")
-        v, *other = _rows(d_values, dtype, strides, self._heads, self._dim, total, "values")
+        self._batch_here(batch)
+        total, device = batch.total_tokens, self.device
+        k, code, token, head = _rows(d_keys, dtype, strides, self._heads, self._dim, total, "keys", device)
+        v, *other = _rows(d_values, dtype, strides, self._heads, self._dim, total, "values", device)
         if other != [code, token, head]:
             raise _bad("keys and values must have the same type and strides")
         return k, v, code, token, head
@@ -232,17 +249,18 @@ class KvPages:
         query and out [total_tokens, num_q_heads, head_dim].  With ``window`` a
         token sees its ``window`` last tokens (itself among them) and the first
         ``sinks``.  ``d_lse``: fp32 [total_tokens, num_q_heads] or None."""
-        dim, total = self._dim, batch.total_tokens
-        q, code, qt, qh = _rows(d_query, dtype, query_strides, num_q_heads, dim, total, "query")
-        o, ocode, ot, oh = _rows(d_out, dtype, out_strides, num_q_heads, dim, total, "out")
+        self._batch_here(batch)
+        dim, total, device = self._dim, batch.total_tokens, self.device
+        q, code, qt, qh = _rows(d_query, dtype, query_strides, num_q_heads, dim, total, "query", device)
+        o, ocode, ot, oh = _rows(d_out, dtype, out_strides, num_q_heads, dim, total, "out", device)
         if ocode != code:
             raise _bad("query and out must have the same type")
         if window < 0 or sinks < 0:
             raise _bad("window and sinks must not be negative")
         if d_lse is not None and not isinstance(d_lse, int) and (
                 str(d_lse.dtype) != "torch.float32" or not d_lse.is_contiguous()
-                or tuple(d_lse.shape) != (total, num_q_heads)):
-            raise _bad("lse must be contiguous fp32 [total_tokens, num_q_heads]")
+                or tuple(d_lse.shape) != (total, num_q_heads) or d_lse.get_device() != device):
+            raise _bad(f"lse must be contiguous fp32 [total_tokens, num_q_heads] on {_place(device)}")
         err = _Err()
         rc = self._attention(self._h, batch._ref, code, q, num_q_heads, qt, qh, scale, window, sinks, o,
                              ot, oh, _ptr(d_lse), _stream(stream), C.byref(err))

@@ -68,6 +68,42 @@ def test_batches_refused_by_the_python_layer():
         K.PagesBatch(16, 16, 16, 1, 1)
 
 
+@pytest.fixture
+def store():
+    """A handle's Python side on device 0, whose entries may not be reached."""
+    def entry(*_):
+        raise AssertionError("reached the library")
+
+    s = K.KvPages.__new__(K.KvPages)
+    s._h, s.device, s.config, s._heads, s._dim = None, 0, None, 2, 64
+    s._write = s._read = s._attention = entry
+    return s
+
+
+def test_memory_of_another_place_is_refused(store):
+    """CPU tensors and another device's never become pointers that a kernel follows."""
+    torch = pytest.importorskip("torch")
+    i32 = dict(dtype=torch.int32)
+    here = K.PagesBatch(16, 16, 16, 3, 3, batch=2, table_width=4)
+    cpu = K.PagesBatch(torch.zeros(2, 4, **i32), torch.zeros(3, **i32), torch.zeros(2, **i32), 3, 3)
+    elsewhere = K.PagesBatch(16, 16, 16, 3, 3, batch=2, table_width=4)
+    elsewhere.device = 1
+    x, q = torch.zeros(3, 2, 64).bfloat16(), torch.zeros(3, 8, 64).bfloat16()
+    at = dict(dtype="bf16")
+    calls = [lambda: store.write_dev(here, x, x), lambda: store.read_dev(here, x, x),
+             lambda: store.attention_dev(here, q, 8, 0.1, 16, **at), lambda: store.attention_dev(here, 16, 8, 0.1, q, **at),
+             lambda: store.attention_dev(here, 16, 8, 0.1, 16, d_lse=torch.zeros(3, 8), **at)]
+    for b in (cpu, elsewhere):
+        calls += [lambda b=b: store.write_dev(b, 16, 16, **at), lambda b=b: store.read_dev(b, 16, 16, **at),
+                  lambda b=b: store.attention_dev(b, 16, 8, 0.1, 16, **at)]
+    for call in calls:
+        with pytest.raises(K.KiviError) as e:
+            call()
+        assert e.value.variant == "InvalidArgument" and ("CPU" in e.value.message or "device" in e.value.message)
+    with pytest.raises(AssertionError):
+        store.write_dev(here, 16, 16, **at)
+
+
 def test_structs_follow_the_header():
     for name in ("kivi_pages_config", "kivi_pages_batch"):
         assert _c_struct_fields(name) == _rust_struct_fields(name), name
