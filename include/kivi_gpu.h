@@ -546,11 +546,12 @@ typedef struct kivi_pages_batch {
     const int32_t *block_table;
     uint64_t table_stride;  /* entries from one row to the next */
     uint64_t table_width;   /* entries of a row */
-    const int32_t *cu_tokens; /* [batch + 1], ascending from 0 to total_tokens */
+    const int32_t *cu_tokens; /* [batch + 1], ascending from 0 to total_tokens; dense rows past
+                               * cu_tokens[batch] are nobody's and left alone */
     const int32_t *kv_lens;   /* [batch] */
     uint64_t batch;
     uint64_t total_tokens;  /* rows of the dense arrays */
-    uint64_t max_tokens;    /* at least every sequence's newest tokens */
+    uint64_t max_tokens;    /* at least every sequence's newest tokens (0 only without rows) */
 } kivi_pages_batch;
 
 typedef struct kivi_pages kivi_pages;

@@ -2932,6 +2932,9 @@ int32_t check_pages_batch(const kivi_pages *h, const kivi_pages_batch *b, kivi::
     if (!h || !b) return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, h ? "null batch" : "null pages");
     if (b->batch > 0 && (!b->cu_tokens || !b->kv_lens || (b->table_width > 0 && !b->block_table)))
         return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "null block table, offsets or lengths");
+    if (b->total_tokens > 0 && (b->batch == 0 || b->max_tokens == 0))
+        return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "%llu rows of %llu sequences with at most %llu newest tokens each",
+                       (unsigned long long)b->total_tokens, (unsigned long long)b->batch, (unsigned long long)b->max_tokens);
     const uint64_t i31 = 0x7fffffffull; // less some tiles: the kernels' token numbers are 32 bits
     if (b->batch > i31 - 1 || b->total_tokens > i31 || b->table_width > (i31 - 511) / (uint64_t)h->st.page ||
         b->table_stride > (1ull << 40))

@@ -382,3 +382,41 @@ def test_a_report_readies_the_workspace(env):
     with pytest.raises(K.KiviError):
         c.store.set_workspace(w.data_ptr() + 4, 4 * w.numel())
     assert torch.equal(c.attend(q, 0.1)[0], want)
+
+
+def test_rows_without_sequences_are_refused(env):
+    """Rows that no call could fill are an error, not outputs left as they were."""
+    torch, K = env
+    c = Case(env, [3, 2], [30, 40], heads=2)
+    q = c.queries()
+    out = torch.zeros_like(q)
+    k, v = torch.zeros(5, 2, 128, dtype=c.dtype, device="cuda"), torch.zeros(5, 2, 128, dtype=c.dtype, device="cuda")
+    before = K.kernel_launches()
+    for batch in (c.batch(c.cu, 5, 0), K.PagesBatch(c.table, c.cu, c.kv_lens, 5, 3, batch=0)):
+        for call in (lambda: c.store.attention_dev(batch, q, 8, 0.1, out), lambda: c.store.write_dev(batch, k, v),
+                     lambda: c.store.read_dev(batch, k, v)):
+            with pytest.raises(K.KiviError) as e:
+                call()
+            assert e.value.variant == "InvalidArgument" and "rows" in e.value.message
+    assert K.kernel_launches() == before
+    c.store.status()
+
+
+@pytest.mark.parametrize("new", [[3, 2], [1, 1]])
+def test_rows_of_nobody_are_left_alone(env, new):
+    """A step padded to more rows than its sequences have."""
+    torch, K = env
+    c = Case(env, new, [30, 40], heads=2)
+    n = sum(new)
+    want, _ = c.attend(c.queries(), 0.1)
+    step = c.batch(c.cu, n + 3, max(new))
+    q = torch.zeros(n + 3, 8, 128, dtype=c.dtype, device="cuda")
+    c.g.manual_seed(5)
+    q[:n] = c.queries()
+    out = torch.full_like(q, 7.0)
+    c.store.attention_dev(step, q, 8, 0.1, out)
+    assert torch.equal(out[:n], c.attend(q[:n].contiguous(), 0.1)[0]) and bool((out[n:] == 7).all())
+    k, v = torch.full((n + 3, 2, 128), 7.0, dtype=c.dtype, device="cuda"), torch.empty(n + 3, 2, 128, dtype=c.dtype, device="cuda")
+    c.store.read_dev(step, k, v)
+    assert bool((k[n:] == 7).all()) and not bool((k[:n] == 7).all())
+    c.store.status()
