@@ -2982,10 +2982,23 @@ int32_t pages_dense(int32_t dtype, const void *k, const void *v, uint64_t token,
     return KIVI_OK;
 }
 
+// Whether two of rows x heads rows of D elements meet: two tokens or heads apart by less
+// than D, or a token on one way and a head back.
+bool pages_rows_meet(uint64_t rows, uint64_t heads, uint64_t token, uint64_t head, uint64_t D) {
+    if ((heads > 1 && head < D) || (rows > 1 && token < D)) return true;
+    if (rows <= 1 || heads <= 1 || token >= (heads - 1) * head + D || head >= (rows - 1) * token + D) return false;
+    for (uint64_t h = 1; h < heads; ++h) { // interleaved rows
+        const uint64_t at = h * head, t = at / token;
+        if (t >= 1 && t < rows && at - t * token < D) return true;
+        if (t + 1 < rows && (t + 1) * token - at < D) return true;
+    }
+    return false;
+}
+
 // Rows that are written may not overlap (a stride of 0 is a broadcast input).
 int32_t check_pages_target(uint64_t rows, uint64_t heads, uint64_t token, uint64_t head, uint64_t D,
                            kivi_error *err) {
-    if ((heads > 1 && head < D) || (rows > 1 && token < D))
+    if (pages_rows_meet(rows, heads, token, head, D))
         return set_msg(err, KIVI_ERR_INVALID_ARGUMENT, "output rows of %llu elements overlap", (unsigned long long)D);
     return KIVI_OK;
 }

@@ -420,3 +420,32 @@ def test_rows_of_nobody_are_left_alone(env, new):
     c.store.read_dev(step, k, v)
     assert bool((k[n:] == 7).all()) and not bool((k[:n] == 7).all())
     c.store.status()
+
+
+def test_interleaved_outputs(env):
+    """Any strides whose rows do not meet are taken; where a token one way and a head back
+    meet, the call is refused."""
+    torch, K = env
+    c = Case(env, [5], [40], heads=2, dim=64)
+    q = c.queries()  # [5, 8, 64]
+    want, _ = c.attend(q, 0.1)
+    room = torch.zeros(1 << 16, dtype=c.dtype, device="cuda")
+
+    def meet(rows, heads, token, head):
+        at = sorted(t * token + h * head for t in range(rows) for h in range(heads))
+        return any(b - a < 64 for a, b in zip(at, at[1:]))
+
+    strides = [(64, 64), (64, 128), (128, 64), (512, 64), (64, 320), (500, 64), (511, 72), (192, 320), (64 * 9, 64 * 2), (64 * 2, 64 * 9),
+               (96, 640), (128, 192), (320, 320), (640, 79), (640, 80), (1000, 64), (130, 650), (65, 325), (64 * 3, 64 * 16)]
+    taken = 0
+    for token, head in strides:
+        out = room.as_strided((5, 8, 64), (token, head, 1))
+        if meet(5, 8, token, head):
+            with pytest.raises(K.KiviError) as e:
+                c.store.attention_dev(c.step, q, 8, 0.1, out)
+            assert e.value.variant == "InvalidArgument" and "overlap" in e.value.message
+        else:
+            c.store.attention_dev(c.step, q, 8, 0.1, out)
+            assert torch.equal(out, want)
+            taken += 1
+    assert 6 <= taken <= len(strides) - 6
