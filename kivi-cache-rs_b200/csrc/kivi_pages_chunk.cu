@@ -71,6 +71,9 @@ __host__ __device__ constexpr int stages_of(int bits) { return bits == 16 ? 5 : 
 constexpr int kPanel = 16384;             // 128 rows x 64 channels
 constexpr long long kWait = 2000000000LL; // ~1 s
 constexpr float kLazy = 8.0f;
+// f16 weights are formed times 2^kBoost: a reference may lag by 2^kLazy, so they stay below
+// 2^15, and what f16's least step leaves of a small one is 2^-32 of the row's largest.
+constexpr int kBoost = 7;
 constexpr float kFar = 16777216.0f;      // 2^24: no bits below 1
 constexpr int kPolyPairs = 1;             // of every four pairs of weights, on the FMA pipe
 // registers of a softmax thread and of the others
@@ -637,7 +640,7 @@ __device__ __noinline__ RowState settle_apart(const PagesAttn &a, const SharedCo
         tmem_ld16(cS + (max(i, 0) & ~15), x);
 #pragma unroll
         for (int k = 0; k < 16; ++k)
-            if (k == (i & 15) && add) w = ex2(__fsub_rn(__fmul_rn(x[k], crow), ref));
+            if (k == (i & 15) && add) w = ex2(__fsub_rn(__fmul_rn(x[k], crow), ref) + kBoost);
         const float most = fmaxf(fabsf(q.y), fabsf(fmaf((float)((1 << BITS) - 1), q.x, q.y)));
         int e = row.eref;
         if (w > 0.0f && isfinite(most)) e = max(e, f16_exponent(most) - 60);
@@ -1224,6 +1227,7 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                             for (int i = 0; i < 128; ++i) x[i] = __fmul_rn(__fadd_rn(__fmul_rn(x[i], crow), ref), inv);
                         }
                     }
+                    if constexpr (F16) off += kBoost;
                     float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
 #pragma unroll
                     for (int hlf = 0; hlf < 2; ++hlf) {
@@ -1278,6 +1282,7 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
             if (ok && nX > 0) ok = warp_wait(&sh.o_full[X], no++ & 1, status);
             tc_after();
             float fa = kCodes ? exp2i(eref) : 1.0f, fb = 0.0f;
+            if constexpr (F16) fa *= exp2i(-kBoost), l *= exp2i(-kBoost);
             if (dual) {
                 // through B's query tile, not in use here
                 float2 *ml = reinterpret_cast<float2 *>(sq + NP * kPanel);

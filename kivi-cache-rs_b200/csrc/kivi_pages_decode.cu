@@ -222,6 +222,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(BITS, ND))
     static_assert(BITS == 16 || F16, "codes become f16 operands");
     using L = Lay<BITS, ND>;
     constexpr int D = L::D, TT = L::TT, TK = L::TK, STEPS = 2 * ND;
+    // f16 weights over 16-bit pages are formed times 2^kBoost (below 2^15 with kLazy): what
+    // f16's least step leaves of a small one is 2^-32 of the row's largest
+    constexpr int kBoost = BITS == 16 && F16 ? 7 : 0;
     __shared__ long long s_sum[kWarps + 1];
     __shared__ long long s_base;
     __shared__ int s_seq, s_last;
@@ -520,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(BITS, ND))
                     }
                     fv = exp2i(-eref);
                 }
-                const float r0 = m0 == -INFINITY ? 0.0f : m0, r1 = m1 == -INFINITY ? 0.0f : m1;
+                const float r0 = (m0 == -INFINITY ? 0.0f : m0) - kBoost, r1 = (m1 == -INFINITY ? 0.0f : m1) - kBoost;
                 // ---- weights, and O^T += V^T P^T
 #pragma unroll
                 for (int s = 0; s < TT; ++s) {
@@ -591,10 +594,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(BITS, ND))
             __syncthreads(); // the last segment's reads
             if (g == 0) {
                 s_m[warp][2 * j] = m0, s_m[warp][2 * j + 1] = m1;
-                s_l[warp][2 * j] = l0, s_l[warp][2 * j + 1] = l1;
+                s_l[warp][2 * j] = l0 * exp2i(-kBoost), s_l[warp][2 * j + 1] = l1 * exp2i(-kBoost);
             }
             {
-                const float fo[2] = {BITS < 16 ? exp2i(eref) : 1.0f, BITS < 16 ? exp2i(eref) * (BITS == 4 ? 0.0625f : 1.0f) : 1.0f};
+                const float fo[2] = {BITS < 16 ? exp2i(eref) : exp2i(-kBoost),
+                                     BITS < 16 ? exp2i(eref) * (BITS == 4 ? 0.0625f : 1.0f) : exp2i(-kBoost)};
                 float *r0p = reinterpret_cast<float *>(s_o4[warp][2 * j]), *r1p = reinterpret_cast<float *>(s_o4[warp][2 * j + 1]);
 #pragma unroll
                 for (int i = 0; i < STEPS; ++i)

@@ -449,3 +449,27 @@ def test_interleaved_outputs(env):
             assert torch.equal(out, want)
             taken += 1
     assert 6 <= taken <= len(strides) - 6
+
+
+@pytest.mark.parametrize("bits,kind", [(16, "f16"), (16, "bf16"), (8, "f16"), (4, "bf16")])
+@pytest.mark.parametrize("new", [1, 2])
+def test_many_small_weights(env, bits, kind, new):
+    """One token holds almost all of the weight and no value, as first tokens do; the sum of
+    3000 others, 2^-23 of it each, is the output.  As many sequences as fill the device, so
+    that one row's tiles meet in one sum.  An f16 weight is exact to 2^-32 of its row's
+    largest, whatever bits that leaves it."""
+    torch, K = env
+    n, seqs = 3000, 150
+    c = Case(env, [new] * seqs, [n] * seqs, heads=1, group=4, bits=bits, kind=kind, page=64)
+    k, v = torch.zeros_like(c.k), torch.ones_like(c.v)
+    v[:, :, ::2] = 0.5
+    k[::n, 0, 0], v[::n] = 16.0, 0.0
+    rewrite(c, k=k, v=v)
+    q = torch.zeros_like(c.queries())
+    q[:, :, 0] = 1.0
+    for log2 in (20.3, 22.6, 23.4):
+        scale = log2 * math.log(2) / 16
+        out, lse = c.attend(q, scale)
+        o, l, tol, ltol = c.reference(q, scale)
+        assert bool(((out.double() - o).abs() <= tol + n * 2.0**-32).all())
+        assert bool(((lse.double() - l).abs() <= ltol).all())
