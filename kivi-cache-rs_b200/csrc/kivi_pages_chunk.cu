@@ -53,6 +53,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "kivi_internal.cuh"
 #include "kivi_pages.cuh"
@@ -1684,7 +1685,7 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
 }
 
 template <int BITS, int ND, bool F16> cudaError_t launch_chunk(const PagesAttn &a, int sms, cudaStream_t s) {
-    static bool configured[64] = {false};
+    static std::atomic<bool> configured[64]; // calls may come from several threads
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
@@ -1733,15 +1734,12 @@ cudaError_t launch_pages_chunk(const PagesAttn &a, cudaStream_t s) {
 // Tensor maps over 16-bit pages: rows of D elements, boxes of one page's tokens
 // (at most a tile's) x 64 channels, 128-byte swizzle, zeros past the last channel.
 cudaError_t pages_tensor_maps(const PagesStore &st, PagesMaps *maps) {
-    static PFN_cuTensorMapEncodeTiled encode = nullptr;
-    if (!encode) {
-        void *fn = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found);
-        if (e != cudaSuccess) return e;
-        if (found != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
-        encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled>(fn);
-    }
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found);
+    if (e != cudaSuccess) return e;
+    if (found != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
+    const PFN_cuTensorMapEncodeTiled encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled>(fn);
     const cuuint64_t dims[2] = {(cuuint64_t)st.D, (cuuint64_t)st.num_pages * st.H * st.page};
     const cuuint64_t strides[1] = {(cuuint64_t)st.row_bytes};
     const cuuint32_t box[2] = {64, (cuuint32_t)std::min(st.page, kTok)}, steps[2] = {1, 1};
