@@ -4,7 +4,7 @@
 // (a row of codes costs a range, a division and a reciprocal, and five packed
 // instructions a pair): 16 x 2048 bf16 tokens of 8 x 128 into 8-bit pages take 81 us
 // (150 MB of DRAM traffic, issue slots 75% busy), their read-back 38 us (145 MB, 3.8 TB/s,
-// 72%); eight ragged sequences of up to 8192 tokens are read back in 50 us (5.6 TB/s).
+// 72%); eight ragged sequences of up to 8192 tokens are read back in 49 us (5.7 TB/s).
 #include <math.h>
 
 #include <algorithm>
@@ -92,6 +92,7 @@ struct Work {
     int L, R, steps, log_parts;
 };
 constexpr int kAhead = 2; // steps whose loads are in flight at once
+constexpr int kSms = 148; // of a B200
 
 // The token of this warp: its slot in the store, or false where it has none.
 struct Place {
@@ -403,7 +404,7 @@ bool divide(const PagesStore &st, const PagesBatch &b, Work *w, unsigned *ctas) 
     // pages 84 and 140 us; 7900 fp32 tokens of 4 x 64 into 4-bit pages 13.6 and 17.0 us;
     // 16 single tokens 14.8 and 8.9 us.
     w->log_parts = 0;
-    while ((1 << w->log_parts) < w->steps && ((int64_t)b.total << w->log_parts) < 148 * 16) ++w->log_parts;
+    while ((1 << w->log_parts) < w->steps && ((int64_t)b.total << w->log_parts) < kSms * 16) ++w->log_parts;
     const int64_t n = (((int64_t)b.total << w->log_parts) + 7) / 8;
     *ctas = (unsigned)n;
     return n <= 0x7fffffff;

@@ -19,36 +19,44 @@
 //
 // The maximum that P refers to moves only when a row exceeds it by 2^8: P stays
 // within its type and O is rarely rescaled.  A row sees tokens by its position;
-// unseen scores are replaced by -inf, and in tiles of which some row does not see
-// some token, V rows that nobody sees are zeroed and infinities and NaN are taken
+// unseen scores are replaced by -inf and weigh 0, and in tiles of which some row does not
+// see some token, V rows that nobody sees are zeroed and infinities and NaN are taken
 // out before O += P V (0 times infinity is not 0) and added to the rows that do
 // see them apart.
+//
+// Rounded below fp32: P, to the operand type, and codes' keys and values, to f16, once.
+// P in two parts, as the decode kernel has it, would double O += P V, a half of the tensor
+// pipe's work; error against 64 bits of a 2048-token chunk's bf16 outputs 0.0023, of which
+// their own rounding is 0.0017.
 //
 // Work split: blocks x kv heads x cached tiles form one flat list, and each of
 // the persistent CTAs (one per SM) takes an equal run of it: no last wave, any
 // mix of lengths.  A (block, head) that spans CTAs leaves partial states in the
-// handle's scratch; the CTA that finishes last joins them in CTA order.
+// device's scratch (or the handle's workspace); the CTA that finishes last joins them in
+// CTA order.
 //
 // Warps: 0-3 softmax of A, 4-7 of B, 8 MMA issue, 9 the run's segments and the copies
 // (TMA tensor maps over the pages, a box per page and 64 channels), 10-11 the masked
 // tiles' V rows.  8- and 4-bit pages: instead of copies, warps 10-15 turn the codes into
 // f16 operand tiles in shared memory, each tile's keys and values scaled by a power of
-// two into f16's upper end (undone in the softmax's factor and O's exponent).
+// two into f16's upper end (undone in the softmax's factor and O's exponent, which moves
+// with the values').
 //
 // What bounds it: per cached tile and pair of row tiles the tensor pipe has 2048 cycles
 // of work and the special function unit as many exponentials (three quarters of them
 // stay there, one quarter are polynomials on the FMA pipe), but a row tile's chain S ->
 // softmax -> P V -> next S is about 3400: a 2048-token chunk over 10240 bf16 tokens, 32
-// heads over 8, takes 291 us in short bursts and 333 us back to back (1.06 and 0.93
-// PFLOP/s, tensor pipe 49% active), an 8192-token prompt under a window of 1024 245 us, of which a block's start and end (queries in, rows out,
-// about 20000 cycles for every 10 tiles) are half.  With 8-bit pages ragged 1024-token
-// chunks over 8000 take 709 us (0.54 PFLOP/s): the converting warps share the issue slots
-// with the softmax (529 us without the conversion's arithmetic, 457 us without its
-// loads as well).
-// Measured and left out: 16 softmax warps, two to a row (301-319 us for the chunk above);
-// S in halves of 64 tokens, double-buffered (310 us; 416 us with the next half's maximum
-// taken between the exponentials); half or none of the exponentials on the FMA pipe (314
-// us each).
+// heads over 8, takes 297 us in short bursts and 338 us back to back (1.04 and 0.92
+// PFLOP/s, tensor pipe 49% active), an 8192-token prompt under a window of 1024 254 us: a
+// block there is ten tiles, some 34000 cycles, and 5000 for queries in and 4500 for rows out
+// beside them, three of the tiles masked.  With 8-bit pages ragged 1024-token
+// chunks over 8000 take 728 us (0.52 PFLOP/s): the converting warps share the issue slots
+// with the softmax (of 709 us, 529 were left without the conversion's arithmetic and 457
+// without its loads as well).
+// Measured and left out, when the chunk above took 291: 16 softmax warps, two to a row
+// (301-319 us); S in halves of 64 tokens, double-buffered (310 us; 416 us with the next
+// half's maximum taken between the exponentials); half or none of the exponentials on the
+// FMA pipe (314 us each).
 #include <cudaTypedefs.h>
 #include <math.h>
 

@@ -18,19 +18,21 @@
 // 11 bits: the tensor pipe has the room.  With codes the operands are f16, whose ten
 // bits hold a code as it lies in its word (bf16's seven do not: twice the
 // instructions); a row's query is scaled by a power of two into f16's upper end, and
-// the weights by one that follows the largest value scale met, both undone in fp32.
+// the weights by one that follows the tile's largest value scale up and, where O allows it,
+// down, both undone in fp32.
 //
 // What bounds it: HBM for 16-bit pages (per token and kv head 4 D bytes, each read
 // once: 16 x 32768 tokens of 8 x 128 in 318 us, 6.7 TB/s; under a window of 4096 and 4
 // first tokens, 270 MB, 52 us).  For codes (2 D + 16 and D + 16 bytes) the work of taking
 // them apart: 433 warp instructions per 16 tokens at 4 bits, 223 of them on the half-rate
-// integer pipe, so 141 us for 396 MB (2.8 TB/s; issue slots and that pipe 54% busy).
+// integer pipe, so 142 us for 396 MB (2.8 TB/s; issue slots 53% and that pipe 55% busy).
 // More CTAs per SM (spills, or 16-token tiles) and larger tiles were no faster.
 //
 // Split: the visible tokens of all (sequence, kv head) rows form one flat list
 // of tiles, and CTA i takes tiles [i per, (i + 1) per): one wave, no tail, any
 // mix of lengths.  A row that spans CTAs leaves partial states (m, l, o) in the
-// handle's scratch, and the CTA that finishes last joins them in CTA order, so
+// device's scratch (or the handle's workspace), and the CTA that finishes last joins them
+// in CTA order, so
 // the result does not depend on which one that is.
 #include <math.h>
 
@@ -144,7 +146,8 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// Resident CTAs per SM: what the registers allow without spilling.
+// Resident CTAs per SM: what the registers allow with no spill, or a small one (8 bits at
+// head_dim 128: 108 bytes stored and 192 loaded; 4 bits at 96: 8 each).
 __host__ __device__ constexpr int ctas_per_sm(int bits, int nd) { return nd == 4 || (bits < 16 && nd == 3) ? 3 : 4; }
 
 // Geometry of the lanes' shares for head_dim D = 32 ND.
