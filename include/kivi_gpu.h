@@ -588,10 +588,10 @@ int32_t kivi_pages_read_dev(const kivi_pages *pages, const kivi_pages_batch *bat
  * dtype (F16 or BF16) is the type of d_query and d_out and, for 16-bit pages,
  * the store's.  Strides in elements; d_lse, when not null, gets the rows'
  * natural log-sum-exp [total_tokens][num_q_heads] (-inf where nothing is seen),
- * with which outputs over disjoint tokens can be joined.  Over codes, what a row
- * sees is held in f16 times powers of two that 32 or 128 tokens share: of tokens
- * there whose keys or values lie 2^20 and more below the largest, bits are lost.
- * Scores are fp32: past 2^24 in magnitude they have no bits below 1, and one that
+ * with which outputs over disjoint tokens can be joined.  Over codes and f16 pages
+ * weights pass through f16 times powers of two: what lies 2^-31 below the row's
+ * largest weight times the largest values that its token's neighbours (up to 128)
+ * hold may be lost.  Scores are fp32: past 2^24 in magnitude they have no bits below 1, and one that
  * is infinite makes its row NaN.  Up to 256 query heads
  * per kv head and, unless max_tokens is 1 with at most 8 of them, 16384
  * sequences; more is KIVI_ERR_UNSUPPORTED. */

@@ -473,17 +473,17 @@ struct Shared {
 
 // Codes: the operands are f16, a tile's keys and values times 2^-exponent (largest
 // finite one below 2^14; of the values' kKeep more are left free rather than O moved),
-// a row's query likewise, and a token's (scale, centre).  In an edge tile the largest one
-// may be a token that some rows do not see, so its exponent leaves out (flags) tokens
-// 2^kSpan above the smallest: their keys get exponents of their own, undone in their
-// columns of S, and their values are added apart.
-constexpr int kKeep = 6, kSpan = 20, kOdd = 1024;
+// a row's query likewise, and a token's (scale, centre).  The largest token may be one that
+// some rows do not see, or that weighs nothing, so tokens 2^kSpan apart do not share an
+// exponent: the tile's is that of its largest token, or of the largest outside that one's 32
+// if it is as far below, and tokens above it or 2^kSpan below stand apart.  Their keys get
+// exponents of their own, undone in their columns of S, and their values are added apart.
+constexpr int kKeep = 6, kSpan = 12, kOdd = 1024;
 struct SharedCodes {
     int kexp[4], vexp[4];  // of tile counter & 3, as far as lift; kOdd more where tokens stand apart
-    uint32_t apart[4][4];  // tokens of an edge tile whose values are added apart
-    uint32_t far[4][4];    // and those whose keys have exponents of their own
-    uint8_t lift[4][kTok]; // how far these lie above the tile's
-    float most[2][4][4];   // a tile's largest key and value per warp, an edge tile's smallest, by tile parity
+    uint32_t apart[4][4];  // tokens whose values are added apart
+    int16_t lift[4][kTok]; // how far the exponents of keys with one of their own lie above the tile's
+    float4 range[2][4];    // largest key and value, smallest but 0 of both (values: -1 if some are not finite), per warp, by tile parity
     float4 token[2][kTok]; // key scale, key centre, value scale, value centre
     int qexp[2 * kRows];
 };
@@ -613,8 +613,8 @@ template <int BITS, int ND>
 __device__ __noinline__ RowState settle_apart(const PagesAttn &a, const SharedCodes &sc, const Seg &s, uint32_t tile, int T, int p,
                                               int lo, uint32_t cS, float crow, RowState row) {
     const uint32_t cO = cS + (kColO - kColS);
-    const uint8_t *lift = sc.lift[tile & 3];
-    const uint32_t *far = sc.far[tile & 3], *apart = sc.apart[tile & 3];
+    const int16_t *lift = sc.lift[tile & 3];
+    const uint32_t *apart = sc.apart[tile & 3];
     auto see = [&](int t) { return t <= p && (t >= lo || t < a.sinks); };
     float mx = -INFINITY;
 #pragma unroll 1
@@ -623,8 +623,8 @@ __device__ __noinline__ RowState settle_apart(const PagesAttn &a, const SharedCo
         tmem_ld16(cS + c, x);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            if (far[c / 32] >> ((c & 16) + i) & 1u && isfinite(x[i])) {
-                const int k = lift[c + i], h = k >> 1;
+            if (const int k = lift[c + i]; k != 0 && isfinite(x[i])) {
+                const int h = k >> 1;
                 x[i] = fminf(fmaxf(x[i] * exp2i(h) * exp2i(k - h), -3e38f), 3e38f);
             }
             if (see(T + c + i)) mx = max3(mx, x[i] * crow, mx);
@@ -666,7 +666,7 @@ __device__ __noinline__ RowState settle_apart(const PagesAttn &a, const SharedCo
                 const float code = BITS == 8 ? (float)v[n] : (float)(v[n / 2] >> (4 * (n & 1)) & 15);
                 const float y = fmaf(code, q.x, q.y);
                 o[k] = o[k] * move1 * move2;
-                if (add) o[k] += isfinite(y) ? w * (y * unit1 * unit2) : y;
+                if (add && (w > 0.0f || !isfinite(y))) o[k] += isfinite(y) ? w * (y * unit1 * unit2) : y;
             }
             tmem_st16(cO + c, reinterpret_cast<const uint32_t *>(o));
             st_wait();
@@ -1148,6 +1148,7 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                     const bool first = j < (dual ? 2 : 1);
                     int ke = sc.kexp[tile & 3];
                     odd = ke >= kOdd / 2;
+                    late |= odd;
                     if (odd) ke -= kOdd;
                     if (first || ke != kref) {
                         kref = ke;
@@ -1534,51 +1535,54 @@ __global__ void __launch_bounds__(threads_of(BITS), 1)
                 const bool kf = isfinite(kb) && isfinite(kp.x), vf = isfinite(vb) && isfinite(vp.x);
                 const uint32_t km = __reduce_max_sync(0xffffffffu, kf ? __float_as_uint(kb) : 0u);
                 const uint32_t vm = __reduce_max_sync(0xffffffffu, vf ? __float_as_uint(vb) : 0u);
-                if (lane == 0 && cw < 4) sc.most[tile & 1][cw][0] = __uint_as_float(km), sc.most[tile & 1][cw][1] = __uint_as_float(vm);
-                if (edge) {
-                    const uint32_t bad = __ballot_sync(0xffffffffu, !vf);
-                    const uint32_t kl = __reduce_min_sync(0xffffffffu, kf && kb > 0.0f ? __float_as_uint(kb) : 0x7f7fffffu);
-                    const uint32_t vl = __reduce_min_sync(0xffffffffu, vf && vb > 0.0f ? __float_as_uint(vb) : 0x7f7fffffu);
-                    if (lane == 0 && cw < 4) {
-                        sc.most[tile & 1][cw][2] = __uint_as_float(kl), sc.most[tile & 1][cw][3] = __uint_as_float(vl);
-                        sc.apart[tile & 3][cw] = bad;
-                    }
+                const uint32_t kl = __reduce_min_sync(0xffffffffu, kf && kb > 0.0f ? __float_as_uint(kb) : 0x7f7fffffu);
+                const uint32_t vl = __reduce_min_sync(0xffffffffu, vf && vb > 0.0f ? __float_as_uint(vb) : 0x7f7fffffu);
+                const uint32_t bad = __ballot_sync(0xffffffffu, !vf);
+                if (lane == 0 && cw < 4) {
+                    sc.range[tile & 1][cw] =
+                        make_float4(__uint_as_float(km), __uint_as_float(vm), __uint_as_float(kl), bad ? -1.0f : __uint_as_float(vl));
                 }
                 if (ct < kTok)
                     sc.token[tile & 1][ct] = make_float4(kp.x, fmaf(half, kp.x, kp.y), vp.x, fmaf(half, vp.x, vp.y));
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.conv);
                 if (!(ok = warp_wait(&sh.conv, met++ & 1, status))) break;
-                float kmost = 0.0f, vmost = 0.0f;
+                float4 g = sc.range[tile & 1][0]; // of the tile: largest, smallest but 0 (or -1)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) kmost = fmaxf(kmost, sc.most[tile & 1][i][0]), vmost = fmaxf(vmost, sc.most[tile & 1][i][1]);
-                int ke = f16_exponent(kmost), own = f16_exponent(vmost);
-                bool split = false;
-                if (edge) {
-                    float kl = 3e38f, vl = 3e38f;
-#pragma unroll
+                for (int i = 1; i < 4; ++i) {
+                    const float4 x = sc.range[tile & 1][i];
+                    g.x = fmaxf(g.x, x.x), g.y = fmaxf(g.y, x.y), g.z = fminf(g.z, x.z), g.w = fminf(g.w, x.w);
+                }
+                int ke = f16_exponent(g.x), own = f16_exponent(g.y);
+                const bool split = !(g.x <= g.z * (float)(1 << kSpan) && g.y <= g.w * (float)(1 << kSpan));
+                if (split) { // the largest of the other warps
+                    float k2 = 0.0f, v2 = 0.0f;
+                    bool ks = false, vs = false;
                     for (int i = 0; i < 4; ++i) {
-                        kl = fminf(kl, sc.most[tile & 1][i][2]), vl = fminf(vl, sc.most[tile & 1][i][3]);
-                        split |= sc.apart[tile & 3][i] != 0;
+                        const float4 x = sc.range[tile & 1][i];
+                        if (x.x == g.x && !ks) ks = true;
+                        else k2 = fmaxf(k2, x.x);
+                        if (x.y == g.y && !vs) vs = true;
+                        else v2 = fmaxf(v2, x.y);
                     }
-                    const int k2 = f16_exponent(kl) + kSpan, v2 = f16_exponent(vl) + kSpan;
-                    split |= k2 < ke || v2 < own;
-                    ke = min(ke, k2), own = min(own, v2);
+                    if (k2 > 0.0f && f16_exponent(k2) < ke - kSpan) ke = f16_exponent(k2);
+                    if (v2 > 0.0f && f16_exponent(v2) < own - kSpan) own = f16_exponent(v2);
                 }
                 // O moves when this does, so it starts with room for values four times as
                 // large, and stays while they fit and lose nothing by it; zeros take any
-                if (j == 0 || own > ve || (own < ve - kKeep && vmost > 0.0f)) ve = min(own + 2, 127);
+                if (j == 0 || own > ve || (own < ve - kKeep && g.y > 0.0f)) ve = min(own + 2, 127);
                 if (split) {
-                    const int lift = kf ? max(f16_exponent(kb) - ke, 0) : 0;
-                    const bool apart = !vf || f16_exponent(vb) > ve;
-                    const uint32_t far = __ballot_sync(0xffffffffu, lift > 0), out = __ballot_sync(0xffffffffu, apart);
+                    auto outside = [](float x, int e) { return x > 0.0f && (f16_exponent(x) > e || f16_exponent(x) < e - kSpan); };
+                    const int lift = kf && outside(kb, ke) ? f16_exponent(kb) - ke : 0, h = -lift >> 1;
+                    const bool apart = !vf || outside(vb, own);
+                    const uint32_t out = __ballot_sync(0xffffffffu, apart);
                     if (ct < kTok) {
-                        sc.lift[tile & 3][ct] = (uint8_t)lift;
+                        sc.lift[tile & 3][ct] = (int16_t)lift;
                         float4 &q = sc.token[tile & 1][ct];
-                        const float f0 = exp2i(-(lift >> 1)), f1 = exp2i(-(lift - (lift >> 1)));
+                        const float f0 = exp2i(h), f1 = exp2i(-lift - h);
                         q.x = q.x * f0 * f1, q.y = q.y * f0 * f1;
                         if (apart) q.z = q.w = 0.0f;
-                        if (lane == 0) sc.far[tile & 3][cw] = far, sc.apart[tile & 3][cw] = out;
+                        if (lane == 0) sc.apart[tile & 3][cw] = out;
                     }
                     __syncwarp();
                     if (lane == 0) bar_arrive(&sh.conv);

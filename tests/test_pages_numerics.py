@@ -473,3 +473,15 @@ def test_many_small_weights(env, bits, kind, new):
         o, l, tol, ltol = c.reference(q, scale)
         assert bool(((out.double() - o).abs() <= tol + n * 2.0**-32).all())
         assert bool(((lse.double() - l).abs() <= ltol).all())
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("new,window,sinks", [([130], 0, 0), ([37, 64, 130], 5, 4), ([300], 64, 0), ([3], 0, 0)])
+@pytest.mark.parametrize("spread", [2.0, 3.0, 6.0])
+def test_tokens_of_unlike_size(env, bits, new, window, sinks, spread):
+    """Codes: values of 10^+-spread from token to token, and keys as unlike, seen and not."""
+    torch, K = env
+    c = Case(env, new, [n + 400 for n in new], heads=1, bits=bits)
+    size = torch.rand(c.v.shape[0], 2, 1, 1, generator=c.g, device="cuda") * 2 - 1
+    rewrite(c, k=c.k.float() * 10 ** (spread * (size[:, 0] - 1)), v=c.v.float() * 10 ** (spread * size[:, 1]))
+    c.check(c.queries(), 0.3, window, sinks)
