@@ -4,7 +4,7 @@
 // (a row of codes costs a range, a division and a reciprocal, and five packed
 // instructions a pair): 16 x 2048 bf16 tokens of 8 x 128 into 8-bit pages take 81 us
 // (150 MB of DRAM traffic, issue slots 75% busy), their read-back 38 us (145 MB, 3.8 TB/s,
-// 72%); eight ragged sequences of up to 8192 tokens are read back in 49 us (5.7 TB/s).
+// 72%); eight ragged sequences of up to 8192 tokens are read back in 50 us (5.6 TB/s).
 #include <math.h>
 
 #include <algorithm>

@@ -46,11 +46,11 @@
 // of work and the special function unit as many exponentials (three quarters of them
 // stay there, one quarter are polynomials on the FMA pipe), but a row tile's chain S ->
 // softmax -> P V -> next S is about 3400: a 2048-token chunk over 10240 bf16 tokens, 32
-// heads over 8, takes 297 us in short bursts and 338 us back to back (1.04 and 0.92
-// PFLOP/s, tensor pipe 49% active), an 8192-token prompt under a window of 1024 254 us: a
+// heads over 8, takes 297 us in short bursts and 340 us back to back (1.04 and 0.91
+// PFLOP/s, tensor pipe 49% active), an 8192-token prompt under a window of 1024 256 us: a
 // block there is ten tiles, some 34000 cycles, and 5000 for queries in and 4500 for rows out
 // beside them, three of the tiles masked.  With 8-bit pages ragged 1024-token
-// chunks over 8000 take 728 us (0.52 PFLOP/s): the converting warps share the issue slots
+// chunks over 8000 take 725 us (0.53 PFLOP/s): the converting warps share the issue slots
 // with the softmax (of 709 us, 529 were left without the conversion's arithmetic and 457
 // without its loads as well).
 // Measured and left out, when the chunk above took 291: 16 softmax warps, two to a row
